@@ -40,7 +40,7 @@
 extern "C" {
 #endif
 
-#define RR_ABI_VERSION 9
+#define RR_ABI_VERSION 10
 
 /* error codes */
 #define RR_OK             0
@@ -327,6 +327,100 @@ int rr_set_timeout(rr_handle* h, int32_t ms);
  * copies and the int8 screens' query pieces, at the runtime's least priority) — as queue addresses (equal addresses =
  * one shared in-order queue). Shards on one device share one set of streams. Synchronises the handle. */
 int rr_stream_queues(rr_handle* h, int i, uint64_t* out);
+
+/* ---- the embedding encoder's operators ------------------------------------------------------------------
+ *
+ * The operators of the encoder whose output the retriever searches with (the forward pass of batch_processor.py:88-91),
+ * for inference: an encoder layer in 8-bit integers. Unlike the calls above they need no handle and keep nothing:
+ *   - Every tensor is a device pointer on `device`, caller-owned; results are written to caller-owned buffers.
+ *   - The work is enqueued on `stream` (a hipStream_t of `device`; null: its null stream) and the call returns at once;
+ *     nothing synchronises, allocates or touches another stream, so the calls can be captured into a HIP graph. The calling
+ *     thread's current device is left as it was.
+ *   - Where a call needs scratch memory the caller passes it (`workspace`, at least as many bytes as the matching
+ *     ..._workspace function returns, 16-byte aligned). It holds nothing between calls; calls that may run at the same
+ *     time need one each.
+ *   - Strides count elements. The last dimension is contiguous; rows may start at any address that is aligned to the
+ *     element (16-byte aligned rows are read fastest). Outputs must not overlap inputs, except where said.
+ *   - Any number of threads may call at once.
+ * Arguments are checked before anything is enqueued (RR_E_INVALID / RR_E_UNSUPPORTED). Integers that live in device memory
+ * (lengths, offsets) are not: the kernels clamp them to the buffers instead.
+ */
+
+/* element types of these operators */
+#define RR_TYPE_F32  0
+#define RR_TYPE_BF16 1
+#define RR_TYPE_F16  2
+#define RR_TYPE_I8   3
+
+/* activation of rr_linear_i8 */
+#define RR_ACT_NONE 0
+#define RR_ACT_GELU 1   /* 0.5 y (1 + erf(y / sqrt 2)) */
+
+/* norms of rr_block_norm */
+#define RR_NORM_NONE  0
+#define RR_NORM_LAYER 1   /* (v - mean) / sqrt(var + eps) * weight + bias */
+#define RR_NORM_RMS   2   /* v / sqrt(mean(v^2) + eps) * weight + bias    */
+
+#define RR_LINEAR_KMAX 131071   /* inner size of rr_linear_i8: the 32-bit sum of k products of 8-bit values is exact */
+#define RR_NORM_COLMAX 32768    /* row length of rr_block_norm */
+#define RR_ATTN_DMAX   128      /* head size of rr_cross_attention (a multiple of 8) */
+
+/* 8-bit rows: scale[r] = max|x[r]| / 127 (fp32), q[r][c] = clamp(rint(x[r][c] / scale[r]), -127, 127) — the rule of the
+ * index's int8 copies. A row of zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and q = 0, so every
+ * product with it is NaN. x: [rows][cols] of `type` (F32, BF16, F16), row stride ldx; q: row stride ldq. */
+int rr_quantize_rows(int device, void* stream, int type, const void* x, int64_t ldx, int64_t rows, int32_t cols,
+                     int8_t* q, int64_t ldq, float* scale);
+
+/* out[m][n] = act((sum_k x8[m][k] * w[n][k]) * (x_scale[m] * w_scale[n]) + bias[n]): a linear layer with 8-bit weights
+ * (w [n][k], a scale per output channel) and 8-bit rows (a scale per row). x_type RR_TYPE_I8: x holds the 8-bit rows and
+ * x_scale [m] their scales. Otherwise x is F32 / BF16 / F16, x_scale is null and the rows are made as rr_quantize_rows
+ * makes them. The integer sum is exact, the rest is fp32, rounded once to out_type (F32, BF16, F16). bias ([n] fp32) may be
+ * null. 1 <= k <= RR_LINEAR_KMAX, n >= 1; m = 0 does nothing. */
+int rr_linear_i8(int device, void* stream, int x_type, const void* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                 int64_t ldw, const float* w_scale, const float* bias, int act, int out_type, void* out, int64_t ldo,
+                 int64_t m, int32_t n, int32_t k, void* workspace, int64_t workspace_bytes);
+
+/* Bytes of workspace rr_linear_i8 needs for these sizes (0: none), or a negative RR_E* code. */
+int64_t rr_linear_i8_workspace(int x_type, int64_t m, int32_t n, int32_t k);
+
+/* The norms around a block, with what joins the block to the residual stream:
+ *     u      = post_norm(y)                       the norm after the block (RR_NORM_NONE: u = y)
+ *     stream = residual_scale * x + gate * u      x null: stream = gate * u; gate null: 1
+ *     normed = next_norm(stream)                  the norm before the next block (RR_NORM_NONE: not computed)
+ *     (q, q_scale) = the 8-bit rows of normed     as rr_quantize_rows
+ * (a post-norm encoder layer, LayerNorm(x + y), is post_norm NONE, next_norm LAYER). All of it in fp32 from the inputs on,
+ * each output rounded once; normed comes from the unrounded stream, the 8-bit rows from the unrounded normed. y, x, gate,
+ * weights, biases, stream and normed are of `type` (F32, BF16, F16). gate: [gate_rows][cols], row r uses gate row
+ * r / rows_per_gate (rows <= gate_rows * rows_per_gate). Weights and biases: [cols] or null (1 and 0). stream, normed and q
+ * may each be null, not all of them; q and q_scale go together; normed and q need next_norm. stream may be x or y itself
+ * (same pointer and stride), normed too. cols <= RR_NORM_COLMAX. */
+int rr_block_norm(int device, void* hip_stream, int type, int64_t rows, int32_t cols, const void* y, int64_t ldy,
+                  const void* x, int64_t ldx, float residual_scale, const void* gate, int64_t ldg, int64_t gate_rows,
+                  int64_t rows_per_gate, int post_norm, const void* post_weight, const void* post_bias, int next_norm,
+                  const void* next_weight, const void* next_bias, float eps, void* stream, int64_t lds, void* normed,
+                  int64_t ldn, int8_t* q, int64_t ldq, float* q_scale);
+
+/* Attention of queries to an encoder's states, whose number may be another than the queries': for every sequence and head
+ *     out_i = sum_j p_ij v_j,   p_i = softmax over the sequence's keys j of scale * q_i . k_j
+ * heads is a multiple of kv_heads; head h reads key head h / (heads / kv_heads). Statistics and sums are fp32.
+ * Queries: q_offsets null: q is [batch][max_q][heads][d] (strides q_bs, q_ts, q_hs, out's o_bs, o_ts, o_hs). Else q is
+ * packed, [total_q][heads][d], sequence b the rows [q_offsets[b], q_offsets[b + 1]) (int32, batch + 1 of them); rows that no
+ * sequence holds are left as they were in out, and max_q only sizes the launch.
+ * Keys and values: k_offsets null: [batch][max_k][kv_heads][d] (strides k_bs.., v_bs..); else packed, as the queries.
+ * key_lengths ([batch] int32, or null): a sequence has at most that many keys, its first ones. key_mask ([batch][max_k]
+ * bytes, row stride mask_stride, or null; dense keys only): keys with a zero byte do not take part. Keys that do not take
+ * part may hold anything, NaN too. A query without a key gets zeros. d: a multiple of 8 up to RR_ATTN_DMAX. */
+int rr_cross_attention(int device, void* stream, int type, const void* q, int64_t q_bs, int64_t q_ts, int64_t q_hs,
+                       const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs, int64_t v_ts,
+                       int64_t v_hs, void* out, int64_t o_bs, int64_t o_ts, int64_t o_hs, int32_t batch, int32_t heads,
+                       int32_t kv_heads, int32_t d, int32_t max_q, int32_t max_k, int64_t total_q, int64_t total_k,
+                       const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* key_lengths,
+                       const uint8_t* key_mask, int64_t mask_stride, float scale, void* workspace,
+                       int64_t workspace_bytes);
+
+/* Bytes of workspace rr_cross_attention needs (0: none), or a negative RR_E* code. */
+int64_t rr_cross_attention_workspace(int type, int32_t batch, int32_t heads, int32_t kv_heads, int32_t d, int32_t max_q,
+                                     int32_t max_k);
 
 /* ---- timing (benchmarks) ----------------------------------------------------------------------- */
 

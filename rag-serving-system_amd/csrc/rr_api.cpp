@@ -6,6 +6,7 @@
 // local shard; shards exchange their top-k candidates with one RCCL all-gather (new: the reference
 // has no collective).
 #include "rag_retrieval.h"
+#include "rr_encoder.h"
 #include "rr_internal.h"
 
 #include <rccl/rccl.h>
@@ -27,10 +28,10 @@
 #include <vector>
 
 namespace {
-
 thread_local std::string g_err;
+}
 
-int fail(int code, const char* fmt, ...) {
+int rr::fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -39,6 +40,10 @@ int fail(int code, const char* fmt, ...) {
   g_err = buf;
   return code;
 }
+
+namespace {
+
+using rr::fail;
 
 #define HIP_TRY(expr)                                                                            \
   do {                                                                                           \

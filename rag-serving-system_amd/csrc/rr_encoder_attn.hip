@@ -1,0 +1,398 @@
+// rr_encoder_attn.hip — attention of queries to an encoder's states (rr_cross_attention).
+//
+// One pass over a sequence's keys with the running maximum m and sum l of the softmax (in powers of two: the scores are
+// scaled by scale * log2 e), S^T = K Q^T and O^T = V^T P^T: in both products a lane's column is one query, so the softmax
+// weights a lane computes are the ones the second product takes from it, and no value changes lanes between the two.
+#include "rr_encoder_device.h"
+
+namespace rr {
+namespace enc {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kRows = 16;   // query rows of a tile: (query, head of the key head's group) pairs
+
+struct AttnParams {
+  AttnArgs a;
+  float c;          // scale * log2 e
+  int group;        // heads per key head
+  int tiles;        // row tiles the launch was sized for
+  int splits;       // pieces of the keys, each a workgroup's; joined by attn_join_kernel when more than one
+};
+
+struct Span {
+  int64_t first;    // packed row, 0 for dense
+  int n;
+};
+__device__ __forceinline__ Span queries_of(const AttnArgs& a, int b) {
+  if (!a.q_offsets) return {0, a.max_q};
+  int64_t lo = a.q_offsets[b], hi = a.q_offsets[b + 1];
+  lo = lo < 0 ? 0 : lo > a.total_q ? a.total_q : lo;
+  hi = hi < lo ? lo : hi > a.total_q ? a.total_q : hi;
+  return {lo, (int)(hi - lo)};
+}
+__device__ __forceinline__ Span keys_of(const AttnArgs& a, int b) {
+  Span s{0, a.max_k};
+  if (a.k_offsets) {
+    int64_t lo = a.k_offsets[b], hi = a.k_offsets[b + 1];
+    lo = lo < 0 ? 0 : lo > a.total_k ? a.total_k : lo;
+    hi = hi < lo ? lo : hi > a.total_k ? a.total_k : hi;
+    s = {lo, (int)(hi - lo)};
+  }
+  if (a.key_lengths) {
+    const int len = a.key_lengths[b];
+    s.n = len < 0 ? 0 : len < s.n ? len : s.n;
+  }
+  return s;
+}
+
+// ---- the two products of one wave over a block of keys ------------------------------------------------------------
+// Lane (i = lane % 16, g = lane / 16). DP: the head size rounded up to a whole tile.
+template <int TY, int DP> struct Core;
+
+// 16-bit types: 32 keys a block. Lane i, g holds the scores of query i with keys 4g + r and 16 + 4g + r (r < 4): the eight
+// keys that its slots 8g .. 8g + 7 of the second product's contraction stand for.
+template <int TY, int DP>
+struct Core16 {
+  static constexpr int kKeys = 32, kMine = 8, kTiles = DP / 16, kSteps = DP / 32;
+  static constexpr int VW = DP / 16;   // values of a V row a lane loads: tile t's row i is dimension VW i + t
+  using E = typename Elem<TY>::type;
+  typedef E e8 __attribute__((ext_vector_type(8)));
+  u32x4 q[kSteps];
+  u32x4 kf[2][kSteps];
+  unsigned vr[8][VW / 2];
+
+  static __device__ __forceinline__ int key(int g, int j) { return (j < 4 ? 0 : 12) + 4 * g + j; }
+  static __device__ __forceinline__ int dim(int t, int i) { return VW * i + t; }
+  static __device__ __forceinline__ f32x4 mma(u32x4 x, u32x4 y, f32x4 c) {
+    if constexpr (TY == T_BF16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ void load_q(const E* row, bool there, int d, int g) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      q[s] = u32x4{0, 0, 0, 0};
+      if (there && 32 * s + 8 * g < d) q[s] = load_as<u32x4>(row + 32 * s + 8 * g);
+    }
+  }
+  __device__ __forceinline__ void load_k(const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int key = kb + 16 * h + i;
+      key = key < n ? key : n - 1;
+      const E* row = base + key * ts;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        kf[h][s] = u32x4{0, 0, 0, 0};
+        if (32 * s + 8 * g < d) kf[h][s] = load_as<u32x4>(row + 32 * s + 8 * g);
+      }
+    }
+  }
+  __device__ __forceinline__ void load_v(const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
+    typedef unsigned vv __attribute__((ext_vector_type(VW / 2)));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      int k = kb + key(g, j);
+      k = k < n ? k : n - 1;
+      vv v = 0;
+      if (VW * i < d) v = load_as<vv>(base + k * ts + VW * i);
+#pragma unroll
+      for (int p = 0; p < VW / 2; ++p) {
+        if constexpr (VW == 2) vr[j][p] = v[0];
+        else vr[j][p] = v[p];
+      }
+    }
+  }
+  __device__ __forceinline__ void scores(float* s) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) c = mma(kf[h][st], q[st], c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * h + r] = c[r];
+    }
+  }
+  // valid: bit j says whether key j of this lane takes part; the V rows of the others may hold anything and become zeros
+  __device__ __forceinline__ void accumulate(const float* p, unsigned valid, f32x4* acc) {
+    e8 pe;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pe[j] = (E)p[j];
+    const u32x4 pb = __builtin_bit_cast(u32x4, pe);
+    if (valid != 0xffu) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int w = 0; w < VW / 2; ++w) vr[j][w] = (valid >> j & 1) ? vr[j][w] : 0u;
+    }
+#pragma unroll
+    for (int w = 0; w < VW / 2; ++w) {
+      u32x4 lo, hi;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        lo[x] = __builtin_amdgcn_perm(vr[2 * x + 1][w], vr[2 * x][w], 0x05040100u);
+        hi[x] = __builtin_amdgcn_perm(vr[2 * x + 1][w], vr[2 * x][w], 0x07060302u);
+      }
+      acc[2 * w] = mma(lo, pb, acc[2 * w]);
+      acc[2 * w + 1] = mma(hi, pb, acc[2 * w + 1]);
+    }
+  }
+};
+template <int DP> struct Core<T_BF16, DP> : Core16<T_BF16, DP> {};
+template <int DP> struct Core<T_F16, DP> : Core16<T_F16, DP> {};
+
+// fp32: 16 keys a block, contractions of four; lane i, g holds the scores of query i with keys 4g + r.
+template <int DP>
+struct Core<T_F32, DP> {
+  static constexpr int kKeys = 16, kMine = 4, kTiles = DP / 16, kSteps = DP / 16, kWide = DP / 64;
+  using E = float;
+  f32x4 q[kSteps], kf[kSteps], vr[4][kWide];
+
+  static __device__ __forceinline__ int key(int g, int j) { return 4 * g + j; }
+  static __device__ __forceinline__ int dim(int t, int i) { return 64 * (t / 4) + 4 * i + t % 4; }
+  __device__ __forceinline__ void load_q(const float* row, bool there, int d, int g) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      q[s] = f32x4{0, 0, 0, 0};
+      if (there && 16 * s + 4 * g < d) q[s] = load_as<f32x4>(row + 16 * s + 4 * g);
+    }
+  }
+  __device__ __forceinline__ void load_k(const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
+    int key = kb + i;
+    key = key < n ? key : n - 1;
+    const float* row = base + key * ts;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      kf[s] = f32x4{0, 0, 0, 0};
+      if (16 * s + 4 * g < d) kf[s] = load_as<f32x4>(row + 16 * s + 4 * g);
+    }
+  }
+  __device__ __forceinline__ void load_v(const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int k = kb + key(g, j);
+      k = k < n ? k : n - 1;
+#pragma unroll
+      for (int w = 0; w < kWide; ++w) {
+        vr[j][w] = f32x4{0, 0, 0, 0};
+        if (64 * w + 4 * i < d) vr[j][w] = load_as<f32x4>(base + k * ts + 64 * w + 4 * i);
+      }
+    }
+  }
+  __device__ __forceinline__ void scores(float* s) const {
+    f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) c = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[st][x], q[st][x], c, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = c[r];
+  }
+  __device__ __forceinline__ void accumulate(const float* p, unsigned valid, f32x4* acc) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int w = 0; w < kWide; ++w)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float v = (valid >> j & 1) ? vr[j][w][t] : 0.f;
+          acc[4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[j], acc[4 * w + t], 0, 0, 0);
+        }
+  }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// where the row's results go, null if the row is not there
+template <class E>
+__device__ __forceinline__ E* out_row(const AttnParams& p, const Span& sq, int b, int kvh, int64_t row) {
+  const AttnArgs& a = p.a;
+  const int64_t qi = row / p.group;
+  const int h = kvh * p.group + (int)(row % p.group);
+  if (qi >= sq.n) return nullptr;
+  return static_cast<E*>(a.out) + (a.q_offsets ? sq.first * a.o_ts : b * a.o_bs) + qi * a.o_ts + h * a.o_hs;
+}
+
+// One workgroup: one tile of 16 query rows and one piece of the keys; each wave takes every fourth block of keys, the four
+// waves' sums are joined in LDS.
+template <int TY, int DP>
+__global__ __launch_bounds__(64 * kWaves) void attn_rows_kernel(AttnParams p) {
+  using C = Core<TY, DP>;
+  using E = typename C::E;
+  constexpr int kLd = DP + 4;
+  __shared__ float so[kWaves][kRows][kLd];
+  __shared__ float sm[kWaves][kRows], sl[kWaves][kRows];
+  const AttnArgs& a = p.a;
+  const int b = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x % p.splits, tile0 = blockIdx.x / p.splits;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const Span sq = queries_of(a, b), sk = keys_of(a, b);
+  const int64_t rows = (int64_t)sq.n * p.group;
+  const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
+  const E* vbase = static_cast<const E*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
+  const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+
+  // tiles behind the ones the launch was sized for (a sequence longer than max_q) take all keys in one piece
+  for (int64_t tile = tile0; tile * kRows < rows; tile += p.tiles) {
+    const bool whole = p.splits == 1 || tile >= p.tiles;
+    if (whole && split) break;
+    const int pieces = whole ? 1 : p.splits;
+    C core;
+    {
+      const int64_t row = tile * kRows + i;
+      const int64_t qi = row / p.group;
+      const int h = kvh * p.group + (int)(row % p.group);
+      const E* q = static_cast<const E*>(a.q) + (a.q_offsets ? sq.first * a.q_ts : b * a.q_bs) + qi * a.q_ts + h * a.q_hs;
+      core.load_q(q, qi < sq.n, a.d, g);
+    }
+    f32x4 acc[C::kTiles] = {};
+    float m = -INFINITY, l = 0.f;
+    for (int kb = (split * kWaves + wave) * C::kKeys; kb < sk.n; kb += pieces * kWaves * C::kKeys) {
+      core.load_k(kbase, a.k_ts, kb, sk.n, a.d, i, g);
+      core.load_v(vbase, a.v_ts, kb, sk.n, a.d, i, g);
+      unsigned valid = 0;
+#pragma unroll
+      for (int j = 0; j < C::kMine; ++j) {
+        const int k = kb + C::key(g, j);
+        valid |= (k < sk.n && (!mask || mask[k]) ? 1u : 0u) << j;
+      }
+      float s[C::kMine];
+      core.scores(s);
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < C::kMine; ++j) top = fmaxf(top, (valid >> j & 1) ? s[j] * p.c : -INFINITY);
+      // the maximum is a reference only: it moves when a score passes it by 2^8
+      if (__any(top > m + 8.f)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float to = fmaxf(m, top);
+        const float f = to == m ? 1.f : exp2_fast(m - to);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < C::kTiles; ++t) acc[t] *= f;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      float w[C::kMine];
+#pragma unroll
+      for (int j = 0; j < C::kMine; ++j) {
+        w[j] = (valid >> j & 1) ? exp2_fast(fmaf(s[j], p.c, -ref)) : 0.f;
+        l += w[j];
+      }
+      core.accumulate(w, valid, acc);
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    __syncthreads();   // (a tile before this one may still be read)
+#pragma unroll
+    for (int t = 0; t < C::kTiles; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) so[wave][i][C::dim(t, 4 * g + r)] = acc[t][r];
+    if (g == 0) {
+      sm[wave][i] = m;
+      sl[wave][i] = l;
+    }
+    __syncthreads();
+    float* ws = whole ? nullptr
+                      : a.ws + ((((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits + split) * kRows * (DP + 2);
+    for (int x = threadIdx.x; x < kRows * DP; x += 64 * kWaves) {
+      const int row = x / DP, d = x % DP;
+      float top = sm[0][row];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][row]);
+      float o = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = sm[w][row] == top ? 1.f : exp2_fast(sm[w][row] - top);
+        o += f * so[w][row][d];
+        sum += f * sl[w][row];
+      }
+      if (whole) {
+        E* to = out_row<E>(p, sq, b, kvh, tile * kRows + row);
+        if (to && d < a.d) to[d] = (E)(sum == 0.f ? 0.f : o / sum);
+      } else {
+        ws[2 * kRows + x] = o;
+        if (d == 0) {
+          ws[row] = top;
+          ws[kRows + row] = sum;
+        }
+      }
+    }
+  }
+}
+
+// joins the pieces of a tile
+template <int TY, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
+  using E = typename Elem<TY>::type;
+  const AttnArgs& a = p.a;
+  const int b = blockIdx.z, kvh = blockIdx.y, tile = blockIdx.x;
+  const Span sq = queries_of(a, b);
+  const float* ws = a.ws + (((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits * kRows * (DP + 2);
+  for (int x = threadIdx.x; x < kRows * DP; x += 256) {
+    const int row = x / DP, d = x % DP;
+    E* to = out_row<E>(p, sq, b, kvh, (int64_t)tile * kRows + row);
+    if (!to || d >= a.d) continue;
+    float top = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ws[s * kRows * (DP + 2) + row]);
+    float o = 0.f, sum = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float* w = ws + s * kRows * (DP + 2);
+      const float f = w[row] == top ? 1.f : exp2_fast(w[row] - top);
+      o += f * w[2 * kRows + x];
+      sum += f * w[kRows + row];
+    }
+    to[d] = (E)(sum == 0.f ? 0.f : o / sum);
+  }
+}
+
+int padded_d(int type, int d) { return d > 64 ? 128 : d > 32 || type == T_F32 ? 64 : 32; }
+
+// Pieces of the keys: enough workgroups for four on each of 256 CUs, and at least 256 keys in each.
+int split_count(int64_t groups, int max_k) {
+  int64_t n = (1024 + groups - 1) / groups;
+  const int64_t most = (max_k + 255) / 256;
+  n = n < most ? n : most;
+  return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+}
+
+template <int TY, int DP>
+hipError_t run(const AttnParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)(p.tiles * p.splits), p.a.kv_heads, p.a.batch);
+  attn_rows_kernel<TY, DP><<<grid, 64 * kWaves, 0, s>>>(p);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (p.splits > 1) {
+    attn_join_kernel<TY, DP><<<dim3(p.tiles, p.a.kv_heads, p.a.batch), 256, 0, s>>>(p);
+    return hipGetLastError();
+  }
+  return hipSuccess;
+}
+
+// Row tiles a launch is sized for: at most 2^20 (a grid holds below 2^32 threads), workgroups loop over the rest.
+int64_t row_tiles(int heads, int kv_heads, int max_q) {
+  const int64_t n = ((int64_t)max_q * (heads / kv_heads) + kRows - 1) / kRows;
+  return n < (1 << 20) ? n : 1 << 20;
+}
+
+}  // namespace
+
+int64_t attention_workspace(int type, int batch, int heads, int kv_heads, int d, int max_q, int max_k) {
+  const int64_t tiles = row_tiles(heads, kv_heads, max_q), groups = tiles * batch * kv_heads;
+  if (groups == 0) return 0;
+  const int n = split_count(groups, max_k);
+  return n == 1 ? 0 : groups * n * kRows * (padded_d(type, d) + 2) * 4;
+}
+
+hipError_t launch_attention(int type, const AttnArgs& a, hipStream_t s) {
+  AttnParams p{a, (float)(a.scale * 1.4426950408889634), a.heads / a.kv_heads,
+               (int)row_tiles(a.heads, a.kv_heads, a.max_q), 1};
+  p.splits = split_count((int64_t)p.tiles * a.batch * a.kv_heads, a.max_k);
+  const int dp = padded_d(type, a.d);
+  if (type == T_F32) return dp == 64 ? run<T_F32, 64>(p, s) : run<T_F32, 128>(p, s);
+  if (type == T_BF16) return dp == 32 ? run<T_BF16, 32>(p, s) : dp == 64 ? run<T_BF16, 64>(p, s) : run<T_BF16, 128>(p, s);
+  return dp == 32 ? run<T_F16, 32>(p, s) : dp == 64 ? run<T_F16, 64>(p, s) : run<T_F16, 128>(p, s);
+}
+
+}  // namespace enc
+}  // namespace rr

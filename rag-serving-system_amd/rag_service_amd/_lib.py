@@ -42,7 +42,19 @@ RR_KERNEL_AUTO = 0
 RR_KERNEL_FUSED = 1
 RR_KERNEL_EXACT = 2
 RR_KERNEL_SCREEN_FALLBACK = 3
-RR_ABI_VERSION = 9
+RR_ABI_VERSION = 10
+RR_TYPE_F32 = 0
+RR_TYPE_BF16 = 1
+RR_TYPE_F16 = 2
+RR_TYPE_I8 = 3
+RR_ACT_NONE = 0
+RR_ACT_GELU = 1
+RR_NORM_NONE = 0
+RR_NORM_LAYER = 1
+RR_NORM_RMS = 2
+RR_LINEAR_KMAX = 131071
+RR_NORM_COLMAX = 32768
+RR_ATTN_DMAX = 128
 
 DTYPES = {"fp32": RR_DTYPE_F32, "float32": RR_DTYPE_F32, "f32": RR_DTYPE_F32,
           "bf16": RR_DTYPE_BF16, "bfloat16": RR_DTYPE_BF16, "fp32-split": RR_DTYPE_F32_SPLIT}
@@ -92,6 +104,17 @@ SIGNATURES = {
     "rr_set_option": (_c_int, [_vp, ctypes.c_char_p, _c_i64]),
     "rr_get_option": (_c_int, [_vp, ctypes.c_char_p, _i64p]),
     "rr_build_info": (ctypes.c_char_p, []),
+    # the embedding encoder's operators (rag_service_amd.ops): device pointers and streams as plain addresses
+    "rr_quantize_rows": (_c_int, [_c_int, _vp, _c_int, _vp, _c_i64, _c_i64, _c_i32, _vp, _c_i64, _vp]),
+    "rr_linear_i8": (_c_int, [_c_int, _vp, _c_int, _vp, _c_i64, _vp, _vp, _c_i64, _vp, _vp, _c_int, _c_int, _vp, _c_i64,
+                              _c_i64, _c_i32, _c_i32, _vp, _c_i64]),
+    "rr_linear_i8_workspace": (_c_i64, [_c_int, _c_i64, _c_i32, _c_i32]),
+    "rr_block_norm": (_c_int, [_c_int, _vp, _c_int, _c_i64, _c_i32, _vp, _c_i64, _vp, _c_i64, ctypes.c_float, _vp, _c_i64,
+                               _c_i64, _c_i64, _c_int, _vp, _vp, _c_int, _vp, _vp, ctypes.c_float, _vp, _c_i64, _vp,
+                               _c_i64, _vp, _c_i64, _vp]),
+    "rr_cross_attention": (_c_int, [_c_int, _vp, _c_int] + [_vp, _c_i64, _c_i64, _c_i64] * 4 + [_c_i32] * 6 + [_c_i64] * 2
+                           + [_vp] * 4 + [_c_i64, ctypes.c_float, _vp, _c_i64]),
+    "rr_cross_attention_workspace": (_c_i64, [_c_int] + [_c_i32] * 6),
 }
 
 

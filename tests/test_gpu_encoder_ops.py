@@ -1,0 +1,473 @@
+"""The embedding encoder's operators (rag_service_amd.ops) against their definitions in 64 bits (encoder_plain.py)."""
+import math
+
+import pytest
+import torch
+
+import encoder_plain as plain
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def ops(hip):
+    from rag_service_amd import ops
+    return ops
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rand(g, *shape, scale=1.0):
+    return torch.randn(*shape, generator=g) * scale
+
+
+# ---- 8-bit rows -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (1, 1024), (65, 1000), (33, 4096), (300, 130), (2, 20011)])
+def test_quantize_rows(ops, dtype, rows, cols):
+    x = rand(gen(rows * 7 + cols), rows, cols, scale=3.0).to(dtype)
+    q, s = ops.quantize_rows(x.cuda())
+    wq, ws = plain.rows8(x)
+    assert torch.equal(s.cpu(), ws)
+    assert torch.equal(q.cpu(), wq)
+
+
+def test_quantize_rows_special_values(ops):
+    x = torch.zeros(9, 37)
+    x[1, 5] = float("nan")
+    x[2, 36] = float("inf")
+    x[3, 0] = float("-inf")
+    x[4] = 1e-45                       # the smallest subnormal: its scale underflows to 0
+    x[5] = torch.linspace(-3.4e38, 3.4e38, 37)
+    x[6] = 2.0 ** -140                 # a subnormal scale
+    x[7, 3] = -127.0
+    x[7, 4:8] = torch.tensor([0.5, 1.5, -2.5, 126.5])      # halves go to the even neighbour
+    x[8] = -0.0
+    q, s = ops.quantize_rows(x.cuda())
+    wq, ws = plain.rows8(x)
+    assert torch.equal(torch.isnan(s.cpu()), torch.isnan(ws))
+    assert torch.equal(torch.nan_to_num(s.cpu()), torch.nan_to_num(ws))
+    assert torch.equal(q.cpu(), wq)
+
+
+def test_quantize_rows_strided_and_shaped(ops):
+    base = rand(gen(1), 4, 6, 50).cuda()
+    x = base[:, 1:5, 3:40].contiguous().view(4, 4, 37)
+    part = base.view(24, 50)[::2, 5:31]                    # every other row, an odd start
+    for t in (x, part):
+        q, s = ops.quantize_rows(t)
+        wq, ws = plain.rows8(t)
+        assert q.shape == t.shape and s.shape == t.shape[:-1]
+        assert torch.equal(q.cpu(), wq) and torch.equal(s.cpu(), ws)
+
+
+# ---- the 8-bit product ----------------------------------------------------------------------------------------------
+
+def weights(g, n, k):
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8)
+    return w, (0.5 + torch.rand(n, generator=g)) / (64 * math.sqrt(k)), rand(g, n, scale=0.2)
+
+
+SIZES = [(1, 1, 1), (1, 1024, 4096), (1, 1024, 1024), (2, 777, 1000), (5, 64, 17), (16, 1024, 1024), (17, 130, 4096),
+         (31, 33, 65), (32, 1024, 2048), (48, 256, 512), (64, 2048, 1024), (65, 1000, 1000), (100, 96, 100), (129, 257, 128),
+         (200, 1024, 1024), (257, 255, 192), (613, 1024, 256), (300, 640, 4096), (1031, 777, 1000), (1500, 1024, 128)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_linear_int8_float_rows(ops, dtype, m, n, k, act):
+    g = gen(m + 3 * n + 5 * k)
+    x = rand(g, m, k, scale=2.0).to(dtype)
+    w, sw, b = weights(g, n, k)
+    got = ops.linear_int8(x.cuda(), w.cuda(), sw.cuda(), bias=b.cuda(), act=act)
+    assert got.dtype == dtype and got.shape == (m, n)
+    q, sx = plain.rows8(x)
+    want, tol = plain.linear(q, sx, w, sw, b, act, dtype)
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("out", TYPES, ids=str)
+def test_linear_int8_rows(ops, out, m, n, k):
+    g = gen(m + 5 * n + 3 * k)
+    q = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+    sx = 0.01 + torch.rand(m, generator=g)
+    w, sw, _ = weights(g, n, k)
+    got = ops.linear_int8(q.cuda(), w.cuda(), sw.cuda(), x_scale=sx.cuda(), out_dtype=out)
+    want, tol = plain.linear(q, sx, w, sw, None, "none", out)
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_linear_int8_extremes(ops, m):
+    """The longest inner size with every product at its largest: the 32-bit sum must still be exact. -128 is a valid value."""
+    k, n = 131071, 40
+    q = torch.full((m, k), -128, dtype=torch.int8)
+    w = torch.full((n, k), -128, dtype=torch.int8)
+    w[1] = 127
+    one = torch.ones(max(m, n))
+    got = ops.linear_int8(q.cuda(), w.cuda(), one[:n].cuda(), x_scale=one[:m].cuda())
+    want = torch.full((m, n), 128 * 128 * k, dtype=torch.float64)
+    want[:, 1] = -128 * 127 * k
+    assert ((got.double().cpu() - want).abs() <= 2.0 ** -24 * want.abs()).all()
+
+
+def test_linear_int8_strides_and_alignment(ops):
+    g = gen(5)
+    for m, n, k, off in [(70, 130, 256, 1), (3, 50, 64, 5), (300, 256, 512, 16), (1, 64, 1024, 3)]:
+        xs = torch.randint(-127, 128, (m, k + 37), generator=g, dtype=torch.int8).cuda()
+        ws = torch.randint(-127, 128, (n, k + 19), generator=g, dtype=torch.int8).cuda()
+        x, w = xs[:, off:off + k], ws[:, off:off + k]
+        sx, sw = torch.rand(m, generator=g), torch.rand(n, generator=g)
+        got = ops.linear_int8(x, w, sw.cuda(), x_scale=sx.cuda())
+        want, tol = plain.linear(x, sx, w, sw, None, "none", torch.float32)
+        assert ((got.double().cpu() - want).abs() <= tol).all()
+        xf = rand(g, m, k + 9).to(torch.bfloat16).cuda()[:, 1:k + 1]
+        got = ops.linear_int8(xf, w, sw.cuda())
+        q, sx = plain.rows8(xf)
+        want, tol = plain.linear(q, sx, w, sw, None, "none", torch.bfloat16)
+        assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
+def test_linear_int8_bad_rows_stay_in_their_rows(ops):
+    g = gen(8)
+    for m in (4, 80):
+        x = rand(g, m, 96)
+        x[1, 95] = float("nan")
+        x[2, 0] = float("inf")
+        x[3] = 0
+        w, sw, b = weights(g, 33, 96)
+        got = ops.linear_int8(x.cuda(), w.cuda(), sw.cuda(), bias=b.cuda()).cpu()
+        assert got[1].isnan().all() and got[2].isnan().all()
+        assert torch.equal(got[3], b)
+        q, sx = plain.rows8(x)
+        want, tol = plain.linear(q, sx, w, sw, b, "none", torch.float32)
+        keep = [i for i in range(m) if i not in (1, 2)]
+        assert ((got[keep].double() - want[keep]).abs() <= tol[keep]).all()
+
+
+def test_linear_int8_empty(ops):
+    w, sw, _ = weights(gen(1), 8, 16)
+    assert ops.linear_int8(torch.zeros(0, 16).cuda(), w.cuda(), sw.cuda()).shape == (0, 8)
+    assert ops.linear_int8(torch.zeros(2, 0, 16).cuda(), w.cuda(), sw.cuda()).shape == (2, 0, 8)
+
+
+# ---- block norm -----------------------------------------------------------------------------------------------------
+
+def norm_case(ops, dtype, rows, cols, post, nxt, gate_rows, rs, residual=True, weighted=True, rows8=False, seed=0):
+    g = gen(rows + 11 * cols + seed)
+    y, x = rand(g, rows, cols).to(dtype), rand(g, rows, cols, scale=2.0).to(dtype) if residual else None
+    gate = rand(g, gate_rows, cols, scale=0.5).to(dtype) if gate_rows else None
+    per = -(-rows // gate_rows) if gate_rows else 1
+    vec = {}
+    for which, kind in (("post", post), ("next", nxt)):
+        vec[which + "_weight"] = (1 + rand(g, cols, scale=0.1)).to(dtype) if weighted and kind != "none" else None
+        vec[which + "_bias"] = rand(g, cols, scale=0.1).to(dtype) if weighted and kind == "layer" else None
+    to = lambda t: None if t is None else t.cuda()  # noqa: E731
+    r = ops.block_norm(to(y), to(x), residual_scale=rs, gate=to(gate), rows_per_gate=per, post_norm=post, next_norm=nxt,
+                       eps=1e-5, rows8=rows8, **{k: to(v) for k, v in vec.items()})
+    want = plain.block_norm(y, x, rs, gate, per, post, vec["post_weight"], vec["post_bias"], nxt, vec["next_weight"],
+                            vec["next_bias"], 1e-5)
+    plain.within(r.stream, *want["stream"], dtype)
+    if nxt == "none":
+        assert r.normed is None and r.rows8 is None
+        return
+    plain.within(r.normed, *want["normed"], dtype)
+    if rows8:
+        o, e = want["normed"]
+        s = r.scale.double().cpu()
+        amax, worst = o.abs().amax(-1), e.amax(-1) * (1 + 2 ** -6)
+        assert ((s * 127 - amax).abs() <= worst + 4 * plain.U * amax).all()
+        # a value is its own within half a step of the scale, and what the fp32 value was off
+        off = (r.rows8.double().cpu() * s[:, None] - o).abs()
+        assert (off <= s[:, None] * (0.5 + 2 ** -12) + worst[:, None] * 2).all()
+        assert (r.rows8.abs().amax(-1) == 127).all()
+
+
+COLS = [1, 2, 63, 64, 65, 255, 256, 500, 768, 1000, 1001, 1024, 1537, 2048, 3000, 4096, 5000, 8192, 12345]
+
+
+@pytest.mark.parametrize("cols", COLS)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_block_norm_widths(ops, dtype, cols):
+    norm_case(ops, dtype, 5, cols, "none", "layer", 0, 1.0, rows8=cols > 2)
+    norm_case(ops, dtype, 3, cols, "rms", "rms", 2, 0.5, rows8=cols > 2)
+
+
+@pytest.mark.parametrize("post", ["none", "layer", "rms"])
+@pytest.mark.parametrize("nxt", ["none", "layer", "rms"])
+@pytest.mark.parametrize("gate_rows", [0, 1, 4])
+def test_block_norm_forms(ops, post, nxt, gate_rows):
+    for dtype in TYPES:
+        for residual in (True, False):
+            for weighted in (True, False):
+                norm_case(ops, dtype, 13, 200, post, nxt, gate_rows, 0.7, residual, weighted, rows8=nxt != "none")
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 300, 5000])
+def test_block_norm_rows(ops, rows):
+    norm_case(ops, torch.bfloat16, rows, 1024, "none", "layer", 0, 1.0, rows8=True)
+    norm_case(ops, torch.bfloat16, rows, 320, "rms", "layer", min(rows, 7), 1.0)
+
+
+@pytest.mark.parametrize("cols", [20000, 32768])
+def test_block_norm_widest(ops, cols):
+    norm_case(ops, torch.bfloat16, 3, cols, "layer", "rms", 1, 1.0, rows8=True)
+
+
+def test_block_norm_offset_rows(ops):
+    """A mean far larger than the spread: the variance is taken from centred values."""
+    g = gen(3)
+    y = (rand(g, 6, 777) + 1000.0)
+    r = ops.block_norm(y.cuda(), next_norm="layer", stream=False)
+    want = plain.block_norm(y, None, 1.0, None, 1, "none", None, None, "layer", None, None, 1e-5)
+    plain.within(r.normed, *want["normed"], torch.float32)
+    assert r.stream is None
+
+
+def test_block_norm_bad_rows_stay_in_their_rows(ops):
+    g = gen(9)
+    y = rand(g, 6, 130)
+    y[1, 129] = float("nan")
+    y[2, 0] = float("inf")
+    y[3] = 0
+    r = ops.block_norm(y.cuda(), next_norm="layer", rows8=True)
+    assert r.normed[1].isnan().all() and r.normed[2].isnan().all()
+    assert (r.normed[3] == 0).all() and r.scale[3] == 0 and (r.rows8[3] == 0).all()
+    assert r.scale[1].isnan() and (r.rows8[1] == 0).all() and (r.rows8[2] == 0).all()
+    ok = [0, 4, 5]
+    want = plain.block_norm(y[ok], None, 1.0, None, 1, "none", None, None, "layer", None, None, 1e-5)
+    plain.within(r.normed[ok], *want["normed"], torch.float32)
+
+
+def test_block_norm_strides(ops):
+    g = gen(4)
+    base = rand(g, 9, 140).to(torch.bfloat16).cuda()
+    res = rand(g, 9, 333).to(torch.bfloat16).cuda()
+    for lo, cols in ((1, 128), (3, 99), (8, 64)):
+        y, x = base[:, lo:lo + cols], res[:, 2 * lo + 1:2 * lo + 1 + cols]
+        r = ops.block_norm(y, x)
+        want = plain.block_norm(y, x, 1.0, None, 1, "none", None, None, "layer", None, None, 1e-5)
+        plain.within(r.stream, *want["stream"], torch.bfloat16)
+        plain.within(r.normed, *want["normed"], torch.bfloat16)
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------
+
+def check_attention(got, q, k, v, there, scale):
+    """there: (batch, keys) bool."""
+    for i in range(q.shape[0]):
+        want, err = plain.attention(q[i], k[i], v[i], there[i], scale)
+        plain.within(got[i], want, err, q.dtype)
+
+
+def qkv(g, b, lq, lk, h, hkv, d, dtype):
+    return ((rand(g, b, lq, h, d) * 1.5).to(dtype), rand(g, b, lk, hkv, d).to(dtype), rand(g, b, lk, hkv, d).to(dtype))
+
+
+ATTN = [  # batch, queries, keys, heads, kv heads, d
+    (1, 1, 1, 1, 1, 8), (2, 1, 5, 2, 2, 64), (3, 1, 300, 4, 4, 64), (2, 1, 1000, 8, 2, 128), (1, 1, 5000, 4, 1, 64),
+    (2, 7, 33, 4, 4, 32), (2, 16, 64, 2, 2, 64), (2, 17, 31, 2, 1, 40), (1, 33, 65, 4, 2, 80), (2, 64, 64, 2, 2, 64),
+    (1, 100, 40, 4, 4, 96), (2, 129, 130, 2, 2, 64), (1, 200, 515, 2, 1, 128), (1, 260, 1, 2, 2, 64), (3, 40, 257, 6, 2, 24),
+    (1, 5, 2100, 2, 2, 120), (2, 300, 300, 3, 1, 16)]
+
+
+@pytest.mark.parametrize("shape", ATTN, ids=str)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_attention_dense(ops, dtype, shape):
+    b, lq, lk, h, hkv, d = shape
+    g = gen(sum(shape))
+    q, k, v = qkv(g, *shape, dtype)
+    got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda())
+    check_attention(got, q, k, v, torch.ones(b, lk, dtype=torch.bool), d ** -0.5)
+
+
+@pytest.mark.parametrize("shape", ATTN, ids=str)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_attention_lengths_and_masks(ops, dtype, shape):
+    """Masked keys hold NaN and infinities; the first sequence has no key left, lengths are out of range both ways."""
+    b, lq, lk, h, hkv, d = shape
+    b += 2
+    g = gen(sum(shape) + 1)
+    q, k, v = qkv(g, b, lq, lk, h, hkv, d, dtype)
+    lens = torch.randint(0, lk + 1, (b,), generator=g, dtype=torch.int32)
+    lens[0], lens[1] = -3, lk + 100
+    there = torch.arange(lk) < lens[:, None]
+    k2, v2 = k.clone(), v.clone()
+    k2[~there], v2[~there] = float("nan"), float("inf")
+    got = ops.cross_attention(q.cuda(), k2.cuda(), v2.cuda(), key_lengths=lens.cuda(), scale=0.2)
+    assert (got[0] == 0).all()
+    check_attention(got, q, k, v, there, 0.2)
+    mask = torch.rand(b, lk, generator=g) < 0.6
+    mask[2] = False
+    k2, v2 = k.clone(), v.clone()
+    k2[~mask], v2[~mask] = float("-inf"), float("nan")
+    got = ops.cross_attention(q.cuda(), k2.cuda(), v2.cuda(), key_mask=mask.cuda())
+    assert (got[2] == 0).all()
+    check_attention(got, q, k, v, mask, d ** -0.5)
+    both = mask & there
+    k2[~both], v2[~both] = float("nan"), float("nan")
+    got = ops.cross_attention(q.cuda(), k2.cuda(), v2.cuda(), key_mask=mask.to(torch.uint8).cuda(),
+                              key_lengths=lens.cuda())
+    check_attention(got, q, k, v, both, d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("h,hkv,d", [(4, 4, 64), (6, 2, 32), (8, 1, 128), (2, 2, 72)])
+def test_attention_packed(ops, dtype, h, hkv, d):
+    """Packed sequences of every length from none to hundreds, rows before the first and behind the last one; hints below
+    the longest sequence change nothing."""
+    g = gen(h + d)
+    ql, kl = [0, 1, 17, 3, 40, 130, 2, 300], [5, 0, 16, 33, 1, 257, 600, 64]
+    start = 3
+    qo = torch.tensor([start] + ql).cumsum(0).to(torch.int32)
+    ko = torch.tensor([start] + kl).cumsum(0).to(torch.int32)
+    tq, tk = int(qo[-1]) + 5, int(ko[-1]) + 2
+    q = rand(g, tq, h, d).to(dtype)
+    k, v = rand(g, tk, hkv, d).to(dtype), rand(g, tk, hkv, d).to(dtype)
+    for rows in (slice(0, start), slice(int(ko[-1]), None)):
+        k[rows], v[rows] = float("nan"), float("nan")
+    for max_q, max_k in ((300, 600), (1, 2000), (20, 1), (513, 0)):
+        got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), q_offsets=qo.cuda(), k_offsets=ko.cuda(), max_q=max_q,
+                                  max_k=max_k)
+        for i in range(len(ql)):
+            a, b, c, e = qo[i], qo[i + 1], ko[i], ko[i + 1]
+            want, err = plain.attention(q[a:b], k[c:e], v[c:e], torch.ones(kl[i], dtype=torch.bool), d ** -0.5)
+            plain.within(got[a:b], want, err, dtype)
+    lens = torch.tensor([2, 5, 16, 7, 1, 200, 0, 999], dtype=torch.int32)
+    got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), q_offsets=qo.cuda(), k_offsets=ko.cuda(), max_q=300, max_k=600,
+                              key_lengths=lens.cuda())
+    for i in range(len(ql)):
+        a, b, c, e = qo[i], qo[i + 1], ko[i], ko[i + 1]
+        there = torch.arange(kl[i]) < lens[i]
+        want, err = plain.attention(q[a:b], k[c:e], v[c:e], there, d ** -0.5)
+        plain.within(got[a:b], want, err, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_attention_mixed_forms_and_strides(ops, dtype):
+    """Dense queries over packed states; heads and tokens in other orders; states of one tensor that holds both."""
+    g = gen(2)
+    b, lq, h, d = 3, 9, 4, 64
+    kl = [20, 0, 77]
+    ko = torch.tensor([0] + kl).cumsum(0).to(torch.int32)
+    kv = rand(g, sum(kl), 2, h, d).to(dtype)
+    q = rand(g, b, h, lq, d + 8).to(dtype)
+    qv = q[..., 3:3 + d].transpose(1, 2)                   # (b, lq, h, d), not contiguous, an odd start
+    got = ops.cross_attention(q.cuda()[..., 3:3 + d].transpose(1, 2), kv.cuda()[:, 0], kv.cuda()[:, 1], k_offsets=ko.cuda(),
+                              max_k=77)
+    for i in range(b):
+        want, err = plain.attention(qv[i], kv[ko[i]:ko[i + 1], 0], kv[ko[i]:ko[i + 1], 1],
+                                    torch.ones(kl[i], dtype=torch.bool), d ** -0.5)
+        plain.within(got[i], want, err, dtype)
+
+
+def test_attention_large_scores(ops):
+    """Scores of thousands: the maximum is found before anything overflows; a first key far below the others."""
+    g = gen(6)
+    for dtype in TYPES:
+        q, k, v = qkv(g, 2, 3, 400, 2, 2, 64, dtype)
+        k = k * 30
+        k[:, 0] = -k[:, 0]
+        got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)
+        check_attention(got, q, k, v, torch.ones(2, 400, dtype=torch.bool), 1.0)
+        for scale in (0.0, -0.3):
+            got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), scale=scale)
+            check_attention(got, q, k, v, torch.ones(2, 400, dtype=torch.bool), scale)
+
+
+def test_attention_no_keys_no_queries(ops):
+    q = torch.ones(2, 3, 2, 16).cuda()
+    kv = torch.ones(2, 0, 2, 16).cuda()
+    assert (ops.cross_attention(q, kv, kv) == 0).all()
+    assert ops.cross_attention(q[:, :0], torch.ones(2, 4, 2, 16).cuda(), torch.ones(2, 4, 2, 16).cuda()).shape == (2, 0, 2, 16)
+    assert ops.cross_attention(q[:0], kv[:0], kv[:0]).shape == (0, 3, 2, 16)
+
+
+def test_attention_offsets_out_of_range_are_clamped(ops):
+    """Offsets in device memory cannot be checked by the call: the kernels keep to the buffers."""
+    q, k = torch.ones(10, 1, 16).cuda(), torch.ones(12, 1, 16).cuda()
+    qo = torch.tensor([-5, 4, 1000], dtype=torch.int32).cuda()
+    ko = torch.tensor([7, 3, 2000], dtype=torch.int32).cuda()
+    got = ops.cross_attention(q, k, k * 2, q_offsets=qo, k_offsets=ko, max_q=10, max_k=12)
+    assert (got[:4] == 0).all() and (got[4:] == 2).all()
+
+
+# ---- streams, graphs ------------------------------------------------------------------------------------------------
+
+def layer(ops, x, st):
+    """One post-norm encoder layer: the operators together, as HipEncoder chains them."""
+    n = ops.quantize_rows(x)
+    t, h, d = x.shape[0], st["heads"], x.shape[1] // st["heads"]
+    q = ops.linear_int8(n[0], *st["wq"], x_scale=n[1], bias=st["bq"], out_dtype=x.dtype).view(t, h, d)
+    kv = ops.linear_int8(n[0], *st["wkv"], x_scale=n[1], bias=st["bkv"], out_dtype=x.dtype).view(t, 2, h, d)
+    c = ops.cross_attention(q, kv[:, 0], kv[:, 1], q_offsets=st["qo"], k_offsets=st["qo"], key_lengths=st["lens"],
+                            max_q=st["max"], max_k=st["max"])
+    a = ops.linear_int8(c.view(t, h * d), *st["wo"], bias=st["bq"])
+    r = ops.block_norm(a, x, next_weight=st["g"], next_bias=st["be"], stream=False, rows8=True)
+    f = ops.linear_int8(r.rows8, *st["w1"], x_scale=r.scale, bias=st["b1"], act="gelu", out_dtype=x.dtype)
+    f = ops.linear_int8(f, *st["w2"], bias=st["bq"])
+    return ops.block_norm(f, r.normed, next_weight=st["g"], next_bias=st["be"], stream=False).normed
+
+
+def layer_state(g, hidden, heads, inner, lens, dtype):
+    def lin(n, k):
+        w, s, _ = weights(g, n, k)
+        return w.cuda(), s.cuda()
+    qo = torch.tensor([0] + [n + 1 for n in lens]).cumsum(0).to(torch.int32)
+    return {"heads": heads, "qo": qo.cuda(), "lens": torch.tensor(lens, dtype=torch.int32).cuda(), "max": max(lens) + 1,
+            "wq": lin(hidden, hidden), "wkv": lin(2 * hidden, hidden), "wo": lin(hidden, hidden), "w1": lin(inner, hidden),
+            "w2": lin(hidden, inner), "bq": rand(g, hidden, scale=0.1).cuda(), "bkv": rand(g, 2 * hidden, scale=0.1).cuda(),
+            "b1": rand(g, inner, scale=0.1).cuda(), "g": (1 + rand(g, hidden, scale=0.1)).to(dtype).cuda(),
+            "be": rand(g, hidden, scale=0.1).to(dtype).cuda()}, int(qo[-1])
+
+
+def test_layer_in_a_graph(ops):
+    """The layer captured and replayed on new inputs, with eager work between the replays: every replay equals the eager
+    result bit for bit; a second captured layer shares no scratch memory with the first."""
+    g = gen(12)
+    st, t = layer_state(g, 256, 4, 512, [5, 33, 1, 80], torch.bfloat16)
+    xs = [rand(g, t, 256).to(torch.bfloat16).cuda() for _ in range(4)]
+    want = [layer(ops, x, st) for x in xs]
+    a, b = xs[0].clone(), xs[1].clone()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        layer(ops, a, st)
+    torch.cuda.synchronize()
+    graphs = []
+    for x in (a, b):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer(ops, x, st)
+        graphs.append((graph, y))
+    for i in range(4):
+        a.copy_(xs[i])
+        b.copy_(xs[(i + 1) % 4])
+        graphs[0][0].replay()
+        graphs[1][0].replay()
+        assert torch.equal(layer(ops, xs[i], st), want[i])
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[0][1], want[i]) and torch.equal(graphs[1][1], want[(i + 1) % 4])
+
+
+def test_layer_on_two_streams(ops):
+    g = gen(13)
+    st, t = layer_state(g, 256, 4, 512, [40] * 6, torch.float16)
+    xs = [rand(g, t, 256).to(torch.float16).cuda() for _ in range(2)]
+    want = [layer(ops, x, st) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(layer(ops, xs[j], st))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for y in got[j]:
+            assert torch.equal(y, want[j])
