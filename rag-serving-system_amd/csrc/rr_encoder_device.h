@@ -3,6 +3,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include "rr_device.h"
 #include "rr_encoder.h"
 
 namespace rr {
@@ -37,46 +38,87 @@ __device__ __forceinline__ void store_as(void* p, V v) {
   __builtin_memcpy(p, &v, sizeof(V));
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-__device__ __forceinline__ unsigned wave_max(unsigned v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const unsigned t = __shfl_xor(v, o);
-    v = v > t ? v : t;
-  }
-  return v;
-}
-// over a workgroup of W waves; `red` W words of LDS, free again after the call's last barrier
+// Sums and maxima over the W waves of a row, every lane gets them. `red`: LDS words, 2 W for each row of the workgroup, used
+// in turn (the first half, the second, ...): one barrier a call, since a half is written again only after a barrier that
+// follows its last reads.
 template <int W>
-__device__ __forceinline__ float group_sum(float v, float* red) {
-  v = wave_sum(v);
-  if constexpr (W == 1) return v;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = 0.f;
+struct RowReduce {
+  float* red;
+  int turn = 0;
+  __device__ __forceinline__ float sum(float v) {
+    v = wave_sum_f32(v);
+    if constexpr (W == 1) return v;
+    float* r = put(v);
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < W; ++i) s += red[i];
-  return s;
-}
-template <int W>
-__device__ __forceinline__ unsigned group_max(unsigned v, float* red) {
-  v = wave_max(v);
-  if constexpr (W == 1) return v;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __uint_as_float(v);
-  __syncthreads();
-  unsigned s = 0;
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const unsigned t = __float_as_uint(red[i]);
-    s = s > t ? s : t;
+    for (int i = 0; i < W; ++i) s += r[i];
+    return s;
   }
-  return s;
+  __device__ __forceinline__ unsigned max(unsigned v) {
+    v = wave_max_u32(v);
+    if constexpr (W == 1) return v;
+    float* r = put(__uint_as_float(v));
+    unsigned s = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const unsigned t = __float_as_uint(r[i]);
+      s = s > t ? s : t;
+    }
+    return s;
+  }
+
+ private:
+  __device__ __forceinline__ float* put(float v) {
+    float* r = red + turn * W;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x / 64 % W] = v;
+    __syncthreads();
+    return r;
+  }
+};
+
+// 16 bytes of a row in registers: N values of type E, of which those at and behind `left` are not read (zeros) or written.
+template <class E>
+struct Chunk {
+  static constexpr int N = 16 / sizeof(E);
+  u32x4 raw;
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(E) == 4) return __uint_as_float(raw[i]);
+    const unsigned h = i % 2 ? raw[i / 2] >> 16 : raw[i / 2] & 0xffffu;
+    if constexpr (std::is_same<E, __bf16>::value) return __uint_as_float(h << 16);
+    else return (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+  }
+  __device__ __forceinline__ void load(const E* p, int left) {
+    if (left >= N) {
+      raw = load_as<u32x4>(p);
+    } else {
+      E v[N] = {};
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < left) v[i] = p[i];
+      __builtin_memcpy(&raw, v, 16);
+    }
+  }
+  __device__ __forceinline__ void fill(float x) {
+    E v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (E)x;
+    __builtin_memcpy(&raw, v, 16);
+  }
+};
+template <class E>
+__device__ __forceinline__ void store_chunk(E* p, const float* v, int left) {
+  constexpr int N = 16 / sizeof(E);
+  E o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = (E)v[i];
+  if (left >= N) {
+    __builtin_memcpy(p, o, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < left) p[i] = o[i];
+  }
 }
 
 // The 8-bit row rule. The row's largest magnitude travels as its bit pattern: patterns of |x| order as their values do,
@@ -90,6 +132,24 @@ __device__ __forceinline__ float row_divisor(float scale) { return scale > 0.f ?
 __device__ __forceinline__ int to_i8(float v, float divisor) {
   const float t = fminf(fmaxf(rintf(v / divisor), -127.0f), 127.0f);
   return (int)t;
+}
+// N values to N bytes; values at and behind `left` are not written
+template <int N>
+__device__ __forceinline__ void store_i8(int8_t* p, const float* v, float divisor, int left) {
+  unsigned o[N / 4];
+#pragma unroll
+  for (int w = 0; w < N / 4; ++w) {
+    o[w] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[w] |= (unsigned)(to_i8(v[4 * w + i], divisor) & 255) << (8 * i);
+  }
+  if (left >= N) {
+    __builtin_memcpy(p, o, N);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < left) p[i] = (int8_t)(o[i / 4] >> (8 * (i % 4)));
+  }
 }
 
 }  // namespace enc

@@ -6,12 +6,47 @@ namespace enc {
 namespace {
 
 // ---- 8-bit rows ----------------------------------------------------------------------------------------------------
-// One workgroup per row, two passes over it (the second one from cache).
-template <int TY>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const void* xv, int64_t ldx, int64_t rows, int cols, int cols_pad,
-                                                            int8_t* q, int64_t ldq, float* scale) {
+// A row in the registers of W waves, S times 16 bytes a lane; W = 1: four rows a workgroup. cols_pad: columns written, zeros
+// behind the row's own.
+template <int TY, int W, int S>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_rows_kernel(const void* xv, int64_t ldx, int64_t rows,
+                                                                             int cols, int cols_pad, int8_t* q, int64_t ldq,
+                                                                             float* scale) {
   using E = typename Elem<TY>::type;
-  __shared__ float red[4];
+  constexpr int N = Chunk<E>::N, kGroups = W == 1 ? 4 : 1;
+  __shared__ float red[2 * W];
+  RowReduce<W> over{red};
+  const int t = threadIdx.x % (64 * W);
+  for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / (64 * W); r < rows; r += (int64_t)gridDim.x * kGroups) {
+    const E* x = static_cast<const E*>(xv) + r * ldx;
+    Chunk<E> c[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) c[s].load(x + (s * 64 * W + t) * N, cols - (s * 64 * W + t) * N);
+    unsigned m = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int i = 0; i < N; ++i) m = mag(c[s][i]) > m ? mag(c[s][i]) : m;
+    const float sc = row_scale(over.max(m));
+    const float div = row_divisor(sc);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = sc == sc ? c[s][i] : 0.f;
+      store_i8<N>(q + r * ldq + (s * 64 * W + t) * N, v, div, cols_pad - (s * 64 * W + t) * N);
+    }
+    if (t == 0) scale[r] = sc;
+  }
+}
+
+// Rows of any length: one workgroup per row, two passes over it (the second one from cache).
+template <int TY>
+__global__ __launch_bounds__(256) void quantize_long_rows_kernel(const void* xv, int64_t ldx, int64_t rows, int cols,
+                                                                 int cols_pad, int8_t* q, int64_t ldq, float* scale) {
+  using E = typename Elem<TY>::type;
+  __shared__ float red[8];
+  RowReduce<4> over{red};
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const E* x = static_cast<const E*>(xv) + r * ldx;
     unsigned m = 0;
@@ -19,11 +54,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* xv, int6
       const unsigned t = mag((float)x[c]);
       m = t > m ? t : m;
     }
-    const float s = row_scale(group_max<4>(m, red));
+    const float s = row_scale(over.max(m));
     const float div = row_divisor(s);
-    const bool dead = !(s == s);
     for (int c = threadIdx.x; c < cols_pad; c += 256)
-      q[r * ldq + c] = c < cols && !dead ? (int8_t)to_i8((float)x[c], div) : 0;
+      q[r * ldq + c] = c < cols && s == s ? (int8_t)to_i8((float)x[c], div) : 0;
     if (threadIdx.x == 0) scale[r] = s;
   }
 }
@@ -115,12 +149,33 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t t
 
 }  // namespace
 
+namespace {
+template <int TY>
+hipError_t quantize(const void* x, int64_t ldx, int64_t rows, int cols, int cols_pad, int8_t* q, int64_t ldq, float* scale,
+                    hipStream_t s) {
+  constexpr int N = Chunk<typename Elem<TY>::type>::N;
+  auto go = [&](auto kernel, int waves) {
+    const int groups = waves == 1 ? 4 : 1;
+    kernel<<<grid_of((rows + groups - 1) / groups), 64 * waves * groups, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale);
+    return hipGetLastError();
+  };
+  const int chunks = (cols_pad + N - 1) / N;
+  if (chunks <= 64) return go(quantize_rows_kernel<TY, 1, 1>, 1);
+  if (chunks <= 64 * 2) return go(quantize_rows_kernel<TY, 1, 2>, 1);
+  if (chunks <= 64 * 4) return go(quantize_rows_kernel<TY, 1, 4>, 1);
+  if (chunks <= 64 * 8) return go(quantize_rows_kernel<TY, 4, 2>, 4);
+  if (chunks <= 64 * 16) return go(quantize_rows_kernel<TY, 4, 4>, 4);
+  if (chunks <= 64 * 32) return go(quantize_rows_kernel<TY, 8, 4>, 8);
+  quantize_long_rows_kernel<TY><<<grid_of(rows), 256, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale);
+  return hipGetLastError();
+}
+}  // namespace
+
 hipError_t launch_quantize_rows(int type, const void* x, int64_t ldx, int64_t rows, int cols, int cols_pad, int8_t* q,
                                 int64_t ldq, float* scale, hipStream_t s) {
-  auto kernel = type == T_F32 ? quantize_rows_kernel<T_F32> : type == T_BF16 ? quantize_rows_kernel<T_BF16>
-                                                                             : quantize_rows_kernel<T_F16>;
-  kernel<<<grid_of(rows), 256, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale);
-  return hipGetLastError();
+  return type == T_F32    ? quantize<T_F32>(x, ldx, rows, cols, cols_pad, q, ldq, scale, s)
+         : type == T_BF16 ? quantize<T_BF16>(x, ldx, rows, cols, cols_pad, q, ldq, scale, s)
+                          : quantize<T_F16>(x, ldx, rows, cols, cols_pad, q, ldq, scale, s);
 }
 
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {

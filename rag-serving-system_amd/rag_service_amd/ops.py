@@ -31,17 +31,28 @@ def _torch():
 
 
 _FLOAT_CODES: dict = {}
+_RAW_STREAM = None
 
 
 def _float_codes():
     if not _FLOAT_CODES:
+        global _RAW_STREAM
         torch = _torch()
+        # the current stream's handle without a Stream object (0.1 instead of 2 us a call), where this torch has it
+        _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
         _FLOAT_CODES.update({torch.float32: RR_TYPE_F32, torch.bfloat16: RR_TYPE_BF16, torch.float16: RR_TYPE_F16})
     return _FLOAT_CODES
 
 
 def _tensor(name: str, t, dtypes, device=None, shape=None):
     """t is a torch tensor on a GPU (on `device`), of one of `dtypes` and of `shape`, and asks for no gradient."""
+    try:
+        if (t.dtype in dtypes and t.is_cuda and not t.requires_grad and (device is None or t.device == device)
+                and (shape is None or t.shape == shape)):
+            return t
+    except AttributeError:
+        pass
     torch = _torch()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
@@ -60,6 +71,8 @@ def _tensor(name: str, t, dtypes, device=None, shape=None):
 
 def _rows(name: str, t):
     """t as (rows, cols) without a copy: its last dimension contiguous, its rows evenly spaced."""
+    if t.dim() == 2 and t.is_contiguous() and t.shape[1] > 0:
+        return t
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{name} has shape {tuple(t.shape)}; expected (..., columns)")
     if t.dim() != 2:
@@ -75,7 +88,8 @@ def _rows(name: str, t):
 
 
 def _ld(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else cols
 
 
 def _vector(name: str, t, dtypes, device, n: int):
@@ -83,7 +97,7 @@ def _vector(name: str, t, dtypes, device, n: int):
     if t is None:
         return None
     _tensor(name, t, dtypes, device, (n,))
-    return t if t.is_contiguous() else t.contiguous()
+    return t.contiguous()
 
 
 def _ptr(t):
@@ -92,7 +106,8 @@ def _ptr(t):
 
 def _place(t):
     """(device index, stream handle) that a call on t's device uses."""
-    return t.device.index, _torch().cuda.current_stream(t.device).cuda_stream
+    index = t.get_device()
+    return index, _RAW_STREAM(index)
 
 
 def _scratch(nbytes: int, like):
@@ -109,8 +124,8 @@ def quantize_rows(x):
     _tensor("x", x, codes)
     x2 = _rows("x", x)
     rows, cols = x2.shape
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     device, stream = _place(x)
     _check(load_library().rr_quantize_rows(device, stream, codes[x.dtype], x2.data_ptr(), _ld(x2), rows, cols,
                                            q.data_ptr(), cols, scale.data_ptr()))
@@ -152,7 +167,7 @@ def linear_int8(x, w, w_scale, *, x_scale=None, bias=None, act: str = "none", ou
     lib = load_library()
     need = 0 if x_type == RR_TYPE_I8 else lib.rr_linear_i8_workspace(x_type, m, n, k)
     ws = _scratch(need, x)
-    out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    out = x.new_empty(x.shape[:-1] + (n,), dtype=out_dtype)
     device, stream = _place(x)
     _check(lib.rr_linear_i8(device, stream, x_type, x2.data_ptr(), _ld(x2), _ptr(x_scale), w.data_ptr(), _ld(w),
                             w_scale.data_ptr(), _ptr(bias), ACTS[act], codes[out_dtype], out.data_ptr(), n, m, n, k,
@@ -205,10 +220,10 @@ def block_norm(y, residual=None, *, residual_scale: float = 1.0, gate=None, rows
         if rows8:
             raise ValueError("rows8 needs a next norm")
         normed = False
-    h = torch.empty(y.shape, dtype=y.dtype, device=dev) if stream else None
-    o = torch.empty(y.shape, dtype=y.dtype, device=dev) if normed else None
-    q = torch.empty(y.shape, dtype=torch.int8, device=dev) if rows8 else None
-    s = torch.empty(y.shape[:-1], dtype=torch.float32, device=dev) if rows8 else None
+    h = y.new_empty(y.shape) if stream else None
+    o = y.new_empty(y.shape) if normed else None
+    q = y.new_empty(y.shape, dtype=torch.int8) if rows8 else None
+    s = y.new_empty(y.shape[:-1], dtype=torch.float32) if rows8 else None
     device, on = _place(y)
     _check(load_library().rr_block_norm(
         device, on, codes[y.dtype], rows, cols, y2.data_ptr(), _ld(y2), _ptr(x2), _ld(x2) if x2 is not None else 0,
@@ -271,7 +286,7 @@ def cross_attention(q, k, v, *, scale: Optional[float] = None, key_lengths=None,
         if max_k > 1 and key_mask.stride(1) != 1 or batch > 1 and key_mask.stride(0) < max_k:
             key_mask = key_mask.contiguous()
         stride = max(key_mask.stride(0), max_k)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = q.new_empty(q.shape)
     lib = load_library()
     code = codes[q.dtype]
     need = lib.rr_cross_attention_workspace(code, batch, heads, kv_heads, d, max_q, max_k)
