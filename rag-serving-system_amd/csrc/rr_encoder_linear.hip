@@ -147,6 +147,151 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t t
   }
 }
 
+
+// ---- the tiled product -----------------------------------------------------------------------------------------------
+// Workgroup tile: TN channels x TM rows, 128 bytes of k a step, both operands brought into LDS by the loads' LDS form (no
+// registers, no ds_write), two buffers in turn: one barrier a step, the next step's loads in flight during this step's matrix
+// instructions. Waves: WN x WM, each (TN / WN) x (TM / WM) in 32 x 32 x 32 instructions. LDS: rows of 128 bytes, the
+// 16-byte column c of row r at column c ^ (r / 2 % 8): the 16 lanes that read a column of 16 rows at once meet all 64 banks.
+// Wants rows at 16-byte addresses and k a multiple of 16 (the loads' unit); columns behind k and rows behind the end are out
+// of the buffer's range and read as zeros.
+constexpr int kStep = 128;
+
+__device__ __forceinline__ i32x4 buffer_of(const void* p, unsigned bytes) {
+  const uint64_t at = (uint64_t)p;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)at), __builtin_amdgcn_readfirstlane((int)(unsigned)(at >> 32)),
+               __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+// 16 bytes a lane from buffer + at to LDS address `to` + 16 * lane
+__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned at, unsigned to) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(at), "s"(buffer), "s"(to)
+      : "memory");
+}
+// every load of this wave has landed, its LDS reads are done, and so are the other waves'
+__device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int OT, int ACT, int TN, int TM, int WN, int WM>
+__global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearArgs a, int tiles_n, int64_t tiles) {
+  constexpr int kWaves = WN * WM, kN = TN / WN / 32, kM = TM / WM / 32;
+  constexpr int kBuf = (TN + TM) * kStep, kLoadsN = TN * kStep / (1024 * kWaves), kLoadsM = TM * kStep / (1024 * kWaves);
+  using O = typename Elem<OT>::type;
+  constexpr int kOutLd = kN * 32 * sizeof(O) + 16;   // bytes of an output row in LDS
+  constexpr int kLds = 2 * kBuf > kWaves * 32 * kOutLd ? 2 * kBuf : kWaves * 32 * kOutLd;
+  __shared__ __align__(1024) char lds[kLds];
+  __shared__ __align__(16) float chan[2][TN];   // the tile's channel scales and biases
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave % WN, wm = wave / WN;
+  const unsigned lds0 = (unsigned)(uintptr_t)lds;
+  // Workgroups go to the 8 XCDs in turn: each XCD takes a contiguous run of tiles, channels first, so that the tiles that
+  // share rows of x meet in one XCD's cache.
+  const int64_t per = tiles / 8, more = tiles % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
+  const int64_t tile = xcd * per + (xcd < more ? xcd : more) + at;
+  const int n0 = (int)(tile % tiles_n) * TN;
+  const int64_t m0 = tile / tiles_n * TM;
+  const int rows_n = a.n - n0 < TN ? a.n - n0 : TN, rows_m = a.m - m0 < TM ? (int)(a.m - m0) : TM;
+  const i32x4 bw = buffer_of(a.w + (int64_t)n0 * a.ldw, (unsigned)((rows_n - 1) * a.ldw + a.k));
+  const i32x4 bx = buffer_of(a.x + m0 * a.ldx, (unsigned)((rows_m - 1) * a.ldx + a.k));
+
+  // this lane's 16 bytes of load j: row 8 (j waves + wave) + lane / 8, LDS column lane % 8
+  unsigned from_w[kLoadsN], from_x[kLoadsM];
+  int col_w[kLoadsN], col_x[kLoadsM];
+#pragma unroll
+  for (int j = 0; j < kLoadsN; ++j) {
+    const int r = 8 * (j * kWaves + wave) + lane / 8;
+    col_w[j] = 16 * (lane % 8 ^ (r / 2 % 8));
+    from_w[j] = (unsigned)(r * a.ldw + col_w[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kLoadsM; ++j) {
+    const int r = 8 * (j * kWaves + wave) + lane / 8;
+    col_x[j] = 16 * (lane % 8 ^ (r / 2 % 8));
+    from_x[j] = (unsigned)(r * a.ldx + col_x[j]);
+  }
+  auto fetch = [&](int k0, int buf) {
+    const unsigned to = lds0 + buf * kBuf + wave * 1024;
+#pragma unroll
+    for (int j = 0; j < kLoadsN; ++j)
+      load_to_lds(bw, k0 + col_w[j] < a.k ? from_w[j] + k0 : ~15u, to + j * kWaves * 1024);
+#pragma unroll
+    for (int j = 0; j < kLoadsM; ++j)
+      load_to_lds(bx, k0 + col_x[j] < a.k ? from_x[j] + k0 : ~15u, to + TN * kStep + j * kWaves * 1024);
+  };
+  i32x16 acc[kN][kM] = {};
+  const int row = lane % 32, half = lane / 32, swz = row / 2 % 8;
+  fetch(0, 0);
+  for (int c = threadIdx.x; c < TN; c += 64 * kWaves) {
+    const int n = n0 + c < a.n ? n0 + c : a.n - 1;
+    chan[0][c] = a.w_scale[n];
+    chan[1][c] = a.bias ? a.bias[n] : 0.f;
+  }
+  int buf = 0;
+  for (int k0 = 0; k0 < a.k; k0 += kStep, buf ^= 1) {
+    step_barrier();
+    if (k0 + kStep < a.k) fetch(k0 + kStep, buf ^ 1);
+    const char* lw = lds + buf * kBuf + (wn * kN * 32 + row) * kStep;
+    const char* lx = lds + buf * kBuf + TN * kStep + (wm * kM * 32 + row) * kStep;
+#pragma unroll
+    for (int kk = 0; kk < kStep / 32; ++kk) {
+      const int c = 16 * ((2 * kk + half) ^ swz);
+      i32x4 fw[kN], fx[kM];
+#pragma unroll
+      for (int i = 0; i < kN; ++i) fw[i] = *reinterpret_cast<const i32x4*>(lw + i * 32 * kStep + c);
+#pragma unroll
+      for (int j = 0; j < kM; ++j) fx[j] = *reinterpret_cast<const i32x4*>(lx + j * 32 * kStep + c);
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+#pragma unroll
+        for (int j = 0; j < kM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
+    }
+  }
+  step_barrier();   // the buffers are free: each wave turns its results into rows there, 32 rows of x at a time
+  char* out = lds + wave * 32 * kOutLd;
+#pragma unroll
+  for (int j = 0; j < kM; ++j) {
+    const int64_t m = m0 + (wm * kM + j) * 32 + row;
+    const float sx = a.x_scale[m < a.m ? m : a.m - 1];
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int nl = i * 32 + 8 * g + 4 * half;
+        const f32x4 sw = *reinterpret_cast<const f32x4*>(&chan[0][wn * kN * 32 + nl]);
+        const f32x4 bias = *reinterpret_cast<const f32x4*>(&chan[1][wn * kN * 32 + nl]);
+        typedef O o4 __attribute__((ext_vector_type(4)));
+        o4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = (O)activate((float)acc[i][j][4 * g + x] * (sx * sw[x]) + bias[x], ACT);
+        *reinterpret_cast<o4*>(out + row * kOutLd + nl * sizeof(O)) = v;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wave's own LDS: no barrier)
+    constexpr int kPer = 16 / sizeof(O), kLanes = kN * 32 / kPer, kRowsAtOnce = 64 / kLanes;
+#pragma unroll
+    for (int r = 0; r < 32; r += kRowsAtOnce) {
+      const int rr = r + lane / kLanes, nl = lane % kLanes * kPer, n = n0 + wn * kN * 32 + nl;
+      const int64_t mm = m0 + (wm * kM + j) * 32 + rr;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(out + rr * kOutLd + nl * sizeof(O));
+      if (mm < a.m && n < a.n) {
+        O* to = static_cast<O*>(a.out) + mm * a.ldo + n;
+        if (n + kPer <= a.n) {
+          store_as(to, v);
+        } else {
+          O e[kPer];
+          __builtin_memcpy(e, &v, 16);
+#pragma unroll
+          for (int x = 0; x < kPer; ++x)
+            if (n + x < a.n) to[x] = e[x];
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
 }  // namespace
 
 namespace {
@@ -178,12 +323,31 @@ hipError_t launch_quantize_rows(int type, const void* x, int64_t ldx, int64_t ro
                           : quantize<T_F16>(x, ldx, rows, cols, cols_pad, q, ldq, scale, s);
 }
 
-hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
-  const int64_t tiles_n = ((int64_t)a.n + 63) / 64, tiles = tiles_n * (((int64_t)a.m + 63) / 64);
-  auto kernel = a.out_type == T_F32 ? linear_any_kernel<T_F32> : a.out_type == T_BF16 ? linear_any_kernel<T_BF16>
-                                                                                      : linear_any_kernel<T_F16>;
-  kernel<<<grid_of(tiles), 256, 0, s>>>(a, tiles_n, tiles);
+namespace {
+template <int OT>
+hipError_t linear(const LinearArgs& a, hipStream_t s) {
+  auto tiles_of = [&](int tn, int tm) { return (((int64_t)a.n + tn - 1) / tn) * (((int64_t)a.m + tm - 1) / tm); };
+  const bool rows16 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw | a.k) & 15) == 0 &&
+                      a.ldx < (1 << 22) && a.ldw < (1 << 22);
+  auto tile = [&](auto kernel, int tn, int tm, int threads) {
+    const int64_t tiles = tiles_of(tn, tm);
+    kernel<<<dim3((unsigned)tiles), threads, 0, s>>>(a, (a.n + tn - 1) / tn, tiles);
+    return hipGetLastError();
+  };
+  if (rows16 && tiles_of(256, 256) < (1 << 22)) {
+    if (tiles_of(256, 256) >= 192)
+      return tile(a.act ? linear_tile_kernel<OT, 1, 256, 256, 2, 4> : linear_tile_kernel<OT, 0, 256, 256, 2, 4>, 256, 256, 512);
+    if (tiles_of(128, 128) >= 96)
+      return tile(a.act ? linear_tile_kernel<OT, 1, 128, 128, 2, 2> : linear_tile_kernel<OT, 0, 128, 128, 2, 2>, 128, 128, 256);
+  }
+  const int64_t tiles = tiles_of(64, 64);
+  linear_any_kernel<OT><<<grid_of(tiles), 256, 0, s>>>(a, (a.n + 63) / 64, tiles);
   return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
+  return a.out_type == T_F32 ? linear<T_F32>(a, s) : a.out_type == T_BF16 ? linear<T_BF16>(a, s) : linear<T_F16>(a, s);
 }
 
 }  // namespace enc

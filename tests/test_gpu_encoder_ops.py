@@ -103,6 +103,21 @@ def test_linear_int8_rows(ops, out, m, n, k):
     assert ((got.double().cpu() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(1500, 1100, 144), (1300, 1290, 16), (1290, 1281, 1040), (1411, 1024, 272), (3600, 3400, 208),
+                                   (3585, 3333, 128), (4000, 3700, 32), (2600, 5000, 656)])
+@pytest.mark.parametrize("out", TYPES, ids=str)
+def test_linear_int8_many_tiles(ops, out, m, n, k):
+    """Sizes of many tiles whose last rows, channels and inner columns fill none."""
+    g = gen(m + n + k)
+    q = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8).cuda()
+    sx = (0.01 + torch.rand(m, generator=g)).cuda()
+    w, sw, b = (t.cuda() for t in weights(g, n, k))
+    for bias, act in ((None, "none"), (b, "gelu")):
+        got = ops.linear_int8(q, w, sw, x_scale=sx, out_dtype=out, bias=bias, act=act)
+        want, tol = plain.linear(q, sx, w, sw, bias, act, out)
+        assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_linear_int8_extremes(ops, m):
     """The longest inner size with every product at its largest: the 32-bit sum must still be exact. -128 is a valid value."""
