@@ -33,6 +33,9 @@ struct LinearArgs {
   int m, n, k;
 };
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
+// Few short floating-point rows: one launch makes their 8-bit rows too (x holds the floating-point rows, x_scale is unused).
+bool linear_fuses_rows(int64_t m, int k);
+hipError_t launch_linear_fused(int x_type, const LinearArgs& a, hipStream_t s);
 
 // ---- norms (rr_encoder_norm.hip) -----------------------------------------------------------------------------------
 struct NormArgs {

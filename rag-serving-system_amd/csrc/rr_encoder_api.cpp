@@ -71,6 +71,7 @@ int linear_sizes(int x_type, int64_t m, int32_t n, int32_t k) {
   if (k > RR_LINEAR_KMAX)
     return fail(RR_E_UNSUPPORTED, "rr_linear_i8: k=%d above %d (the 32-bit sum would no longer be exact)", k, RR_LINEAR_KMAX);
   if (m > INT_MAX) return fail(RR_E_UNSUPPORTED, "rr_linear_i8: m=%lld above 2^31 - 1", (long long)m);
+  if (n > 1 << 26) return fail(RR_E_UNSUPPORTED, "rr_linear_i8: n=%d above 2^26", n);
   return RR_OK;
 }
 
@@ -111,7 +112,7 @@ int rr_quantize_rows(int device, void* stream, int type, const void* x, int64_t 
 
 int64_t rr_linear_i8_workspace(int x_type, int64_t m, int32_t n, int32_t k) {
   if (int rc = linear_sizes(x_type, m, n, k); rc != RR_OK) return rc;
-  if (x_type == RR_TYPE_I8 || m == 0) return 0;
+  if (x_type == RR_TYPE_I8 || m == 0 || linear_fuses_rows(m, k)) return 0;
   return round_up(m * 4, 256) + m * round_up(k, 16);   // the rows' scales, then the 8-bit rows
 }
 
@@ -136,6 +137,7 @@ int rr_linear_i8(int device, void* stream, int x_type, const void* x, int64_t ld
   hipStream_t s = static_cast<hipStream_t>(stream);
   return enqueue(me, device, [&]() -> hipError_t {
     LinearArgs a{static_cast<const int8_t*>(x), ldx, x_scale, w, ldw, w_scale, bias, act, out_type, out, ldo, (int)m, n, k};
+    if (x_type != RR_TYPE_I8 && linear_fuses_rows(m, k)) return launch_linear_fused(x_type, a, s);
     if (x_type != RR_TYPE_I8) {
       float* sc = static_cast<float*>(workspace);
       int8_t* q = static_cast<int8_t*>(workspace) + round_up(m * 4, 256);

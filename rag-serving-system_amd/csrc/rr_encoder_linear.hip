@@ -65,8 +65,20 @@ __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const void* xv,
 // ---- the product ---------------------------------------------------------------------------------------------------
 // out^T = w x^T: the matrix instruction's rows are output channels and its columns rows of x, so a lane holds four
 // consecutive channels of one row and stores them together.
+template <int OT>
+__device__ __forceinline__ float gelu(float y) {
+  if constexpr (OT == T_F32) return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
+  // 16-bit results: erf to 1.5e-7 by Abramowitz and Stegun 7.1.26, a third of erff's instructions
+  // (613 x 4096 results of a 1024-long product: 18.2 us with erff, 9.9 with this)
+  const float z = fabsf(y) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float e = p * __builtin_amdgcn_exp2f(z * z * -1.4426950408889634f);   // 1 - erf(z)
+  return 0.5f * y * (y < 0.f ? e : 2.0f - e);
+}
+template <int OT>
 __device__ __forceinline__ float activate(float y, int act) {
-  return act == 1 ? 0.5f * y * (1.0f + erff(y * 0.70710678118654752f)) : y;
+  return act == 1 ? gelu<OT>(y) : y;
 }
 
 template <int OT>
@@ -81,7 +93,7 @@ __device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, i3
     const int ni = n + i < a.n ? n + i : a.n - 1;
     float y = (float)c[i] * (sx * a.w_scale[ni]);
     if (a.bias) y += a.bias[ni];
-    v[i] = (O)activate(y, a.act);
+    v[i] = (O)activate<OT>(y, a.act);
   }
   if (n + 4 <= a.n) {
     store_as(out, v);
@@ -105,57 +117,165 @@ __device__ __forceinline__ u32x4 load_row16(const int8_t* row, int at, int k) {
   return v;
 }
 
-// 64 x 64 tiles, 64 bytes of k at a time, any size and alignment.
-constexpr int kPad = 80;   // bytes from one LDS row to the next
+// 64 x 64 tiles, 128 bytes of k a step, any size and alignment: through registers into LDS, the next step's loads in flight
+// during this one's matrix instructions.
+constexpr int kAnyStep = 128, kPad = kAnyStep + 16;   // bytes from one LDS row to the next
 template <int OT>
 __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t tiles_n, int64_t tiles) {
   __shared__ __align__(16) int8_t lw[64 * kPad], lx[64 * kPad];
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-  const int n0 = (int)(tile % tiles_n) * 64;
-  const int64_t m0 = tile / tiles_n * 64;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int row = t >> 2, col = (t & 3) * 16;
-  const int8_t* wr = a.w + (int64_t)(n0 + row < a.n ? n0 + row : a.n - 1) * a.ldw;
-  const int8_t* xr = a.x + (m0 + row < a.m ? m0 + row : a.m - 1) * a.ldx;
-  i32x4 acc[2][2] = {};
   const int wn = (wave & 1) * 32, wm = (wave >> 1) * 32;
-  for (int k0 = 0; k0 < a.k; k0 += 64) {
-    const u32x4 vw = load_row16(wr, k0 + col, a.k), vx = load_row16(xr, k0 + col, a.k);
-    __syncthreads();
-    *reinterpret_cast<u32x4*>(lw + row * kPad + col) = vw;
-    *reinterpret_cast<u32x4*>(lx + row * kPad + col) = vx;
-    __syncthreads();
-    i32x4 fw[2], fx[2];
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int n0 = (int)(tile % tiles_n) * 64;
+    const int64_t m0 = tile / tiles_n * 64;
+    const int8_t* wr = a.w + (int64_t)(n0 + row < a.n ? n0 + row : a.n - 1) * a.ldw;
+    const int8_t* xr = a.x + (m0 + row < a.m ? m0 + row : a.m - 1) * a.ldx;
+    u32x4 vw[2], vx[2];
+    auto fetch = [&](int k0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      fw[i] = *reinterpret_cast<const i32x4*>(lw + (wn + 16 * i + (lane & 15)) * kPad + (lane >> 4) * 16);
-      fx[i] = *reinterpret_cast<const i32x4*>(lx + (wm + 16 * i + (lane & 15)) * kPad + (lane >> 4) * 16);
+      for (int h = 0; h < 2; ++h) {
+        vw[h] = load_row16(wr, k0 + 64 * h + col, a.k);
+        vx[h] = load_row16(xr, k0 + 64 * h + col, a.k);
+      }
+    };
+    i32x4 acc[2][2] = {};
+    fetch(0);
+    for (int k0 = 0; k0 < a.k; k0 += kAnyStep) {
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<u32x4*>(lw + row * kPad + 64 * h + col) = vw[h];
+        *reinterpret_cast<u32x4*>(lx + row * kPad + 64 * h + col) = vx[h];
+      }
+      __syncthreads();
+      if (k0 + kAnyStep < a.k) fetch(k0 + kAnyStep);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        i32x4 fw[2], fx[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          fw[i] = *reinterpret_cast<const i32x4*>(lw + (wn + 16 * i + (lane & 15)) * kPad + 64 * kk + (lane >> 4) * 16);
+          fx[i] = *reinterpret_cast<const i32x4*>(lx + (wm + 16 * i + (lane & 15)) * kPad + 64 * kk + (lane >> 4) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t m = m0 + wm + 16 * j + (lane & 15);
-      const int n = n0 + wn + 16 * i + 4 * (lane >> 4);
-      if (m < a.m && n < a.n) store4<OT>(a, m, n, acc[i][j]);
-    }
+      for (int j = 0; j < 2; ++j) {
+        const int64_t m = m0 + wm + 16 * j + (lane & 15);
+        const int n = n0 + wn + 16 * i + 4 * (lane >> 4);
+        if (m < a.m && n < a.n) store4<OT>(a, m, n, acc[i][j]);
+      }
   }
 }
 
+// ---- few rows ------------------------------------------------------------------------------------------------------
+// Up to 16 R rows of x: the weights' bytes are all there is. A workgroup holds 16 channels; its eight waves take every eighth
+// 64 bytes of k, straight from memory into the matrix instruction's operands, and their integer sums, exact in any order, meet
+// in LDS. FUSED: x is floating point and every workgroup makes its own 8-bit rows in LDS while its first weights arrive: one
+// launch, where a short row would wait for two.
+constexpr int kFewWaves = 8, kFewRows = 64;
+constexpr int kFusedMost = 16384;   // values of x that every workgroup may convert for itself
+
+template <int OT, int R, int XT>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a) {
+  constexpr bool kFused = XT != T_I8;
+  constexpr int kAhead = R <= 2 ? 8 : 4;   // steps of 64 bytes of weights loaded together
+  __shared__ __align__(16) i32x4 sums[kFewWaves][R][64];
+  __shared__ __align__(16) int8_t x8[kFused ? kFusedMost + 16 * 64 : 16];
+  __shared__ float sc[16];
+  __shared__ float red[2 * kFewWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, kp = (a.k + 63) / 64 * 64;
+  const int8_t* wr = a.w + (int64_t)(n0 + i < a.n ? n0 + i : a.n - 1) * a.ldw;
+  i32x4 acc[R] = {};
+  for (int k0 = wave * 64; k0 < kp || (kFused && k0 == wave * 64); k0 += kAhead * kFewWaves * 64) {
+    u32x4 w[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) w[s] = load_row16(wr, k0 + s * kFewWaves * 64 + 16 * g, a.k);
+    if constexpr (kFused) {
+      if (k0 == wave * 64) {   // (every wave comes here once, with or without weights to multiply)
+        using E = typename Elem<XT>::type;
+        RowReduce<kFewWaves> over{red};
+        for (int r = 0; r < a.m; ++r) {
+          const E* x = reinterpret_cast<const E*>(a.x) + r * a.ldx;
+          constexpr int N = Chunk<E>::N, S = (kFusedMost + 64 * kFewWaves * N - 1) / (64 * kFewWaves * N);
+          const int chunks = (kp + N - 1) / N;
+          Chunk<E> c[S];
+          unsigned top = 0;
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            const int at = s * 64 * kFewWaves + threadIdx.x;
+            if (s * 64 * kFewWaves < chunks) {
+              c[s].load(x + at * N, a.k - at * N);
+#pragma unroll
+              for (int e = 0; e < N; ++e) top = mag(c[s][e]) > top ? mag(c[s][e]) : top;
+            }
+          }
+          const float scale = row_scale(over.max(top));
+          const float div = row_divisor(scale);
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            const int at = s * 64 * kFewWaves + threadIdx.x;
+            if (at < chunks) {
+              float v[N];
+#pragma unroll
+              for (int e = 0; e < N; ++e) v[e] = scale == scale ? c[s][e] : 0.f;
+              store_i8<N>(x8 + r * kp + at * N, v, div, N);
+            }
+          }
+          if (threadIdx.x == 0) sc[r] = scale;
+        }
+        __syncthreads();
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const int at = k0 + s * kFewWaves * 64 + 16 * g;
+      if (k0 + s * kFewWaves * 64 < kp) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          u32x4 x = {0, 0, 0, 0};
+          if (16 * r + i < a.m) {
+            if constexpr (kFused) x = *reinterpret_cast<const u32x4*>(x8 + (16 * r + i) * kp + at);
+            else x = load_row16(a.x + (16 * r + i) * a.ldx, at, a.k);
+          }
+          acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w[s]), __builtin_bit_cast(i32x4, x), acc[r], 0, 0, 0);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) sums[wave][r][lane] = acc[r];
+  __syncthreads();
+  if constexpr (kFused) a.x_scale = sc;
+  for (int r = wave; r < R; r += kFewWaves) {
+    i32x4 c = sums[0][r][lane];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) c += sums[w][r][lane];
+    const int m = 16 * r + i, n = n0 + 4 * g;
+    if (m < a.m && n < a.n) store4<OT>(a, m, n, c);
+  }
+}
 
 // ---- the tiled product -----------------------------------------------------------------------------------------------
-// Workgroup tile: TN channels x TM rows, 128 bytes of k a step, both operands brought into LDS by the loads' LDS form (no
-// registers, no ds_write), two buffers in turn: one barrier a step, the next step's loads in flight during this step's matrix
-// instructions. Waves: WN x WM, each (TN / WN) x (TM / WM) in 32 x 32 x 32 instructions. LDS: rows of 128 bytes, the
-// 16-byte column c of row r at column c ^ (r / 2 % 8): the 16 lanes that read a column of 16 rows at once meet all 64 banks.
+// Workgroup tile: TN channels x TM rows, STEP bytes of k a step, both operands brought into LDS by the loads' LDS form (no
+// registers, no ds_write) into BUFS buffers in turn: BUFS - 1 steps are in flight while one is multiplied, one barrier a step.
+// Waves: WN x WM, each (TN / WN) x (TM / WM) in 32 x 32 x 32 instructions. LDS rows hold a step; the 16-byte column c of row r
+// lies at column c ^ swizzle(r), so that the 16 lanes that read a column of 16 rows at once meet all 64 banks.
 // Wants rows at 16-byte addresses and k a multiple of 16 (the loads' unit); columns behind k and rows behind the end are out
 // of the buffer's range and read as zeros.
-constexpr int kStep = 128;
+template <int STEP>
+__device__ __forceinline__ int swizzle(int r) {
+  static_assert(STEP == 128 || STEP == 64, "a row's share of the 256-byte bank cycle");
+  return STEP == 128 ? r / 2 % 8 : r / 4 % 4;
+}
 
 __device__ __forceinline__ i32x4 buffer_of(const void* p, unsigned bytes) {
   const uint64_t at = (uint64_t)p;
@@ -172,16 +292,19 @@ __device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned at, unsigned 
       : "v"(at), "s"(buffer), "s"(to)
       : "memory");
 }
-// every load of this wave has landed, its LDS reads are done, and so are the other waves'
-__device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// all but this wave's last N loads have landed, its LDS reads are done, and so are the other waves'
+template <int N>
+__device__ __forceinline__ void step_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
+}
 
-template <int OT, int ACT, int TN, int TM, int WN, int WM>
-__global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearArgs a, int tiles_n, int64_t tiles) {
-  constexpr int kWaves = WN * WM, kN = TN / WN / 32, kM = TM / WM / 32;
-  constexpr int kBuf = (TN + TM) * kStep, kLoadsN = TN * kStep / (1024 * kWaves), kLoadsM = TM * kStep / (1024 * kWaves);
+template <int OT, int ACT, int TN, int TM, int WN, int WM, int STEP, int BUFS>
+__global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs a, int tiles_n, int64_t tiles) {
+  constexpr int kWaves = WN * WM, kN = TN / WN / 32, kM = TM / WM / 32, kCols = STEP / 16;
+  constexpr int kBuf = (TN + TM) * STEP, kLoadsN = TN * STEP / (1024 * kWaves), kLoadsM = TM * STEP / (1024 * kWaves);
   using O = typename Elem<OT>::type;
   constexpr int kOutLd = kN * 32 * sizeof(O) + 16;   // bytes of an output row in LDS
-  constexpr int kLds = 2 * kBuf > kWaves * 32 * kOutLd ? 2 * kBuf : kWaves * 32 * kOutLd;
+  constexpr int kLds = BUFS * kBuf > kWaves * 32 * kOutLd ? BUFS * kBuf : kWaves * 32 * kOutLd;
   __shared__ __align__(1024) char lds[kLds];
   __shared__ __align__(16) float chan[2][TN];   // the tile's channel scales and biases
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -196,20 +319,25 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearArgs
   const int rows_n = a.n - n0 < TN ? a.n - n0 : TN, rows_m = a.m - m0 < TM ? (int)(a.m - m0) : TM;
   const i32x4 bw = buffer_of(a.w + (int64_t)n0 * a.ldw, (unsigned)((rows_n - 1) * a.ldw + a.k));
   const i32x4 bx = buffer_of(a.x + m0 * a.ldx, (unsigned)((rows_m - 1) * a.ldx + a.k));
+  for (int c = threadIdx.x; c < TN; c += 64 * kWaves) {
+    const int n = n0 + c < a.n ? n0 + c : a.n - 1;
+    chan[0][c] = a.w_scale[n];
+    chan[1][c] = a.bias ? a.bias[n] : 0.f;
+  }
 
-  // this lane's 16 bytes of load j: row 8 (j waves + wave) + lane / 8, LDS column lane % 8
+  // this lane's 16 bytes of load j: row (64 / kCols) (j waves + wave) + lane / kCols, LDS column lane % kCols
   unsigned from_w[kLoadsN], from_x[kLoadsM];
   int col_w[kLoadsN], col_x[kLoadsM];
 #pragma unroll
   for (int j = 0; j < kLoadsN; ++j) {
-    const int r = 8 * (j * kWaves + wave) + lane / 8;
-    col_w[j] = 16 * (lane % 8 ^ (r / 2 % 8));
+    const int r = 64 / kCols * (j * kWaves + wave) + lane / kCols;
+    col_w[j] = 16 * (lane % kCols ^ swizzle<STEP>(r));
     from_w[j] = (unsigned)(r * a.ldw + col_w[j]);
   }
 #pragma unroll
   for (int j = 0; j < kLoadsM; ++j) {
-    const int r = 8 * (j * kWaves + wave) + lane / 8;
-    col_x[j] = 16 * (lane % 8 ^ (r / 2 % 8));
+    const int r = 64 / kCols * (j * kWaves + wave) + lane / kCols;
+    col_x[j] = 16 * (lane % kCols ^ swizzle<STEP>(r));
     from_x[j] = (unsigned)(r * a.ldx + col_x[j]);
   }
   auto fetch = [&](int k0, int buf) {
@@ -219,37 +347,38 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearArgs
       load_to_lds(bw, k0 + col_w[j] < a.k ? from_w[j] + k0 : ~15u, to + j * kWaves * 1024);
 #pragma unroll
     for (int j = 0; j < kLoadsM; ++j)
-      load_to_lds(bx, k0 + col_x[j] < a.k ? from_x[j] + k0 : ~15u, to + TN * kStep + j * kWaves * 1024);
+      load_to_lds(bx, k0 + col_x[j] < a.k ? from_x[j] + k0 : ~15u, to + TN * STEP + j * kWaves * 1024);
   };
   i32x16 acc[kN][kM] = {};
-  const int row = lane % 32, half = lane / 32, swz = row / 2 % 8;
-  fetch(0, 0);
-  for (int c = threadIdx.x; c < TN; c += 64 * kWaves) {
-    const int n = n0 + c < a.n ? n0 + c : a.n - 1;
-    chan[0][c] = a.w_scale[n];
-    chan[1][c] = a.bias ? a.bias[n] : 0.f;
-  }
-  int buf = 0;
-  for (int k0 = 0; k0 < a.k; k0 += kStep, buf ^= 1) {
-    step_barrier();
-    if (k0 + kStep < a.k) fetch(k0 + kStep, buf ^ 1);
-    const char* lw = lds + buf * kBuf + (wn * kN * 32 + row) * kStep;
-    const char* lx = lds + buf * kBuf + TN * kStep + (wm * kM * 32 + row) * kStep;
+  const int row = lane % 32, half = lane / 32, swz = swizzle<STEP>(row);
+  const int steps = (a.k + STEP - 1) / STEP;
 #pragma unroll
-    for (int kk = 0; kk < kStep / 32; ++kk) {
+  for (int s = 0; s < BUFS - 1; ++s)
+    if (s < steps) fetch(s * STEP, s);
+  int buf = 0, next = BUFS - 1;
+  for (int s = 0; s < steps; ++s) {
+    if (s + BUFS - 2 < steps) step_barrier<(BUFS - 2) * (kLoadsN + kLoadsM)>();
+    else step_barrier<0>();
+    if (s + BUFS - 1 < steps) fetch((s + BUFS - 1) * STEP, next);   // (its buffer was last read before this barrier)
+    const char* lw = lds + buf * kBuf + (wn * kN * 32 + row) * STEP;
+    const char* lx = lds + buf * kBuf + TN * STEP + (wm * kM * 32 + row) * STEP;
+#pragma unroll
+    for (int kk = 0; kk < STEP / 32; ++kk) {
       const int c = 16 * ((2 * kk + half) ^ swz);
       i32x4 fw[kN], fx[kM];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) fw[i] = *reinterpret_cast<const i32x4*>(lw + i * 32 * kStep + c);
+      for (int i = 0; i < kN; ++i) fw[i] = *reinterpret_cast<const i32x4*>(lw + i * 32 * STEP + c);
 #pragma unroll
-      for (int j = 0; j < kM; ++j) fx[j] = *reinterpret_cast<const i32x4*>(lx + j * 32 * kStep + c);
+      for (int j = 0; j < kM; ++j) fx[j] = *reinterpret_cast<const i32x4*>(lx + j * 32 * STEP + c);
 #pragma unroll
       for (int i = 0; i < kN; ++i)
 #pragma unroll
         for (int j = 0; j < kM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
     }
+    buf = buf + 1 == BUFS ? 0 : buf + 1;
+    next = next + 1 == BUFS ? 0 : next + 1;
   }
-  step_barrier();   // the buffers are free: each wave turns its results into rows there, 32 rows of x at a time
+  step_barrier<0>();   // the buffers are free: each wave turns its results into rows there, 32 rows of x at a time
   char* out = lds + wave * 32 * kOutLd;
 #pragma unroll
   for (int j = 0; j < kM; ++j) {
@@ -265,7 +394,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tile_kernel(LinearArgs
         typedef O o4 __attribute__((ext_vector_type(4)));
         o4 v;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = (O)activate((float)acc[i][j][4 * g + x] * (sx * sw[x]) + bias[x], ACT);
+        for (int x = 0; x < 4; ++x) v[x] = (O)activate<OT>((float)acc[i][j][4 * g + x] * (sx * sw[x]) + bias[x], ACT);
         *reinterpret_cast<o4*>(out + row * kOutLd + nl * sizeof(O)) = v;
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wave's own LDS: no barrier)
@@ -324,30 +453,53 @@ hipError_t launch_quantize_rows(int type, const void* x, int64_t ldx, int64_t ro
 }
 
 namespace {
-template <int OT>
+template <int OT, int ACT, int TN, int TM, int WN, int WM, int STEP, int BUFS>
+hipError_t tiled(const LinearArgs& a, hipStream_t s) {
+  const int tiles_n = (a.n + TN - 1) / TN;
+  const int64_t tiles = (int64_t)tiles_n * ((a.m + TM - 1) / TM);
+  linear_tile_kernel<OT, ACT, TN, TM, WN, WM, STEP, BUFS><<<dim3((unsigned)tiles), 64 * WN * WM, 0, s>>>(a, tiles_n, tiles);
+  return hipGetLastError();
+}
+template <int OT, int ACT>
 hipError_t linear(const LinearArgs& a, hipStream_t s) {
-  auto tiles_of = [&](int tn, int tm) { return (((int64_t)a.n + tn - 1) / tn) * (((int64_t)a.m + tm - 1) / tm); };
+  auto tiles_of = [&](int64_t t) { return ((a.n + t - 1) / t) * ((a.m + t - 1) / t); };
+  if (a.m <= kFewRows) {
+    const dim3 grid((a.n + 15) / 16);
+    if (a.m <= 16) linear_few_kernel<OT, 1, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
+    else if (a.m <= 32) linear_few_kernel<OT, 2, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
+    else linear_few_kernel<OT, 4, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
+    return hipGetLastError();
+  }
   const bool rows16 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw | a.k) & 15) == 0 &&
                       a.ldx < (1 << 22) && a.ldw < (1 << 22);
-  auto tile = [&](auto kernel, int tn, int tm, int threads) {
-    const int64_t tiles = tiles_of(tn, tm);
-    kernel<<<dim3((unsigned)tiles), threads, 0, s>>>(a, (a.n + tn - 1) / tn, tiles);
-    return hipGetLastError();
-  };
-  if (rows16 && tiles_of(256, 256) < (1 << 22)) {
-    if (tiles_of(256, 256) >= 192)
-      return tile(a.act ? linear_tile_kernel<OT, 1, 256, 256, 2, 4> : linear_tile_kernel<OT, 0, 256, 256, 2, 4>, 256, 256, 512);
-    if (tiles_of(128, 128) >= 96)
-      return tile(a.act ? linear_tile_kernel<OT, 1, 128, 128, 2, 2> : linear_tile_kernel<OT, 0, 128, 128, 2, 2>, 128, 128, 256);
+  if (rows16 && tiles_of(64) < (1 << 22)) {
+    if (tiles_of(256) >= 192) return tiled<OT, ACT, 256, 256, 2, 4, 128, 2>(a, s);
+    if (tiles_of(128) >= 512) return tiled<OT, ACT, 128, 128, 2, 2, 128, 2>(a, s);
+    return tiled<OT, ACT, 64, 64, 2, 2, 128, 3>(a, s);
   }
-  const int64_t tiles = tiles_of(64, 64);
+  const int64_t tiles = tiles_of(64);
   linear_any_kernel<OT><<<grid_of(tiles), 256, 0, s>>>(a, (a.n + 63) / 64, tiles);
+  return hipGetLastError();
+}
+template <int OT>
+hipError_t fused(int x_type, const LinearArgs& a, hipStream_t s) {
+  const dim3 grid((a.n + 15) / 16);
+  if (x_type == T_F32) linear_few_kernel<OT, 1, T_F32><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  else if (x_type == T_BF16) linear_few_kernel<OT, 1, T_BF16><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  else linear_few_kernel<OT, 1, T_F16><<<grid, 64 * kFewWaves, 0, s>>>(a);
   return hipGetLastError();
 }
 }  // namespace
 
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
-  return a.out_type == T_F32 ? linear<T_F32>(a, s) : a.out_type == T_BF16 ? linear<T_BF16>(a, s) : linear<T_F16>(a, s);
+  if (a.act) return a.out_type == T_F32 ? linear<T_F32, 1>(a, s) : a.out_type == T_BF16 ? linear<T_BF16, 1>(a, s) : linear<T_F16, 1>(a, s);
+  return a.out_type == T_F32 ? linear<T_F32, 0>(a, s) : a.out_type == T_BF16 ? linear<T_BF16, 0>(a, s) : linear<T_F16, 0>(a, s);
+}
+
+bool linear_fuses_rows(int64_t m, int k) { return m <= 16 && m * round_up(k, 64) <= kFusedMost; }
+
+hipError_t launch_linear_fused(int x_type, const LinearArgs& a, hipStream_t s) {
+  return a.out_type == T_F32 ? fused<T_F32>(x_type, a, s) : a.out_type == T_BF16 ? fused<T_BF16>(x_type, a, s) : fused<T_F16>(x_type, a, s);
 }
 
 }  // namespace enc

@@ -44,7 +44,7 @@ def test_nothing_to_do_is_fine(lib):
 
 
 def linear(lib, device=0, x_type=0, x=P, ldx=64, x_scale=NULL, w=P, ldw=64, w_scale=P, bias=NULL, act=0, out_type=0, out=P,
-           ldo=16, m=4, n=16, k=64, ws=P, ws_bytes=1 << 20):
+           ldo=16, m=40, n=16, k=64, ws=P, ws_bytes=1 << 20):
     return lib.rr_linear_i8(device, None, x_type, x, ldx, x_scale, w, ldw, w_scale, bias, act, out_type, out, ldo, m, n, k,
                             ws, ws_bytes)
 
@@ -54,7 +54,7 @@ def linear(lib, device=0, x_type=0, x=P, ldx=64, x_scale=NULL, w=P, ldw=64, w_sc
     ({"n": 0}, "n=0"), ({"k": 0}, "k=0"), ({"act": 2}, "act"), ({"out_type": 3}, "out_type"), ({"x": NULL}, "x is null"),
     ({"ldx": 63}, "stride"), ({"w": NULL}, "w is null"), ({"ldw": 63}, "stride"), ({"w_scale": NULL}, "w_scale is null"),
     ({"bias": ODD}, "bias"), ({"out": NULL}, "out is null"), ({"out": ODD}, "aligned"), ({"ldo": 15}, "stride"),
-    ({"x_scale": P}, "x_scale"), ({"x_type": 3}, "x_scale"), ({"ws": NULL}, "workspace"), ({"ws_bytes": 511}, "workspace"),
+    ({"x_scale": P}, "x_scale"), ({"x_type": 3}, "x_scale"), ({"ws": NULL}, "workspace"), ({"ws_bytes": 40 * 64}, "workspace"),
     ({"ws": ctypes.c_void_p((1 << 20) + 8)}, "16-byte")])
 def test_linear_refuses(lib, change, word):
     refused(lib, linear(lib, **change), _lib.RR_E_INVALID, word)
@@ -67,7 +67,8 @@ def test_linear_unsupported(lib):
     assert lib.rr_linear_i8_workspace(0, 4, 16, big) == _lib.RR_E_UNSUPPORTED
     assert lib.rr_linear_i8_workspace(7, 4, 16, 64) == _lib.RR_E_INVALID
     assert lib.rr_linear_i8_workspace(3, 4, 16, 64) == 0
-    assert lib.rr_linear_i8_workspace(1, 4, 16, 64) >= 4 * (64 + 4)
+    refused(lib, linear(lib, n=(1 << 26) + 1, ldo=1 << 27), _lib.RR_E_UNSUPPORTED, "2^26")
+    assert lib.rr_linear_i8_workspace(1, 40, 16, 64) >= 40 * (64 + 4)
 
 
 def norm(lib, device=0, type=0, rows=4, cols=8, y=P, ldy=8, x=P, ldx=8, rs=1.0, gate=NULL, ldg=8, gate_rows=1,
