@@ -180,58 +180,65 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t t
 // 64 bytes of k, straight from memory into the matrix instruction's operands, and their integer sums, exact in any order, meet
 // in LDS. FUSED: x is floating point and every workgroup makes its own 8-bit rows in LDS while its first weights arrive: one
 // launch, where a short row would wait for two.
-constexpr int kFewWaves = 8, kFewRows = 64;
-constexpr int kFusedMost = 16384;   // values of x that every workgroup may convert for itself
+constexpr int kFewWaves = 8, kFewRows = 48;
+constexpr int kFusedRow = 8192;    // columns of a single row that every workgroup converts for itself, all waves at it,
+constexpr int kFusedWave = 1024;   // and of up to eight rows, a wave each
 
-template <int OT, int R, int XT>
+// A row's 8-bit row by W waves, of which this is lane t: the row's values are asked for first, then the rest is done.
+template <int XT, int W>
+struct Row8 {
+  using E = typename Elem<XT>::type;
+  static constexpr int N = Chunk<E>::N, S = (W == 1 ? kFusedWave : kFusedRow) / (64 * W * N);
+  Chunk<E> c[S];
+  __device__ __forceinline__ void load(const E* x, int k, int t) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) c[s].load(x + (s * 64 * W + t) * N, k - (s * 64 * W + t) * N);
+  }
+  __device__ __forceinline__ void put(int8_t* to, int kp, float* scale, int t, float* red) {
+    unsigned top = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int e = 0; e < N; ++e) top = mag(c[s][e]) > top ? mag(c[s][e]) : top;
+    RowReduce<W> over{red};
+    const float s8 = row_scale(over.max(top));
+    const float div = row_divisor(s8);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int at = (s * 64 * W + t) * N;
+      float v[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = s8 == s8 ? c[s][e] : 0.f;
+      if (at < kp) store_i8<N>(to + at, v, div, N);
+    }
+    if (t == 0) *scale = s8;
+  }
+};
+
+// SINGLE: of a fused kernel, that x is one row.
+template <int OT, int R, int XT, bool SINGLE = false>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a) {
   constexpr bool kFused = XT != T_I8;
   constexpr int kAhead = R <= 2 ? 8 : 4;   // steps of 64 bytes of weights loaded together
   __shared__ __align__(16) i32x4 sums[kFewWaves][R][64];
-  __shared__ __align__(16) int8_t x8[kFused ? kFusedMost + 16 * 64 : 16];
+  __shared__ __align__(16) int8_t x8[kFused ? kFusedRow : 16];   // (eight rows of kFusedWave columns are as many)
   __shared__ float sc[16];
   __shared__ float red[2 * kFewWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16, kp = (a.k + 63) / 64 * 64;
   const int8_t* wr = a.w + (int64_t)(n0 + i < a.n ? n0 + i : a.n - 1) * a.ldw;
   i32x4 acc[R] = {};
+  Row8<kFused ? XT : T_F32, SINGLE ? kFewWaves : 1> rows;
+  const int t = SINGLE ? threadIdx.x : lane, mine = SINGLE ? 0 : wave;
+  if constexpr (kFused)
+    if (mine < a.m) rows.load(reinterpret_cast<const typename Elem<XT>::type*>(a.x) + mine * a.ldx, a.k, t);
   for (int k0 = wave * 64; k0 < kp || (kFused && k0 == wave * 64); k0 += kAhead * kFewWaves * 64) {
     u32x4 w[kAhead];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) w[s] = load_row16(wr, k0 + s * kFewWaves * 64 + 16 * g, a.k);
     if constexpr (kFused) {
       if (k0 == wave * 64) {   // (every wave comes here once, with or without weights to multiply)
-        using E = typename Elem<XT>::type;
-        RowReduce<kFewWaves> over{red};
-        for (int r = 0; r < a.m; ++r) {
-          const E* x = reinterpret_cast<const E*>(a.x) + r * a.ldx;
-          constexpr int N = Chunk<E>::N, S = (kFusedMost + 64 * kFewWaves * N - 1) / (64 * kFewWaves * N);
-          const int chunks = (kp + N - 1) / N;
-          Chunk<E> c[S];
-          unsigned top = 0;
-#pragma unroll
-          for (int s = 0; s < S; ++s) {
-            const int at = s * 64 * kFewWaves + threadIdx.x;
-            if (s * 64 * kFewWaves < chunks) {
-              c[s].load(x + at * N, a.k - at * N);
-#pragma unroll
-              for (int e = 0; e < N; ++e) top = mag(c[s][e]) > top ? mag(c[s][e]) : top;
-            }
-          }
-          const float scale = row_scale(over.max(top));
-          const float div = row_divisor(scale);
-#pragma unroll
-          for (int s = 0; s < S; ++s) {
-            const int at = s * 64 * kFewWaves + threadIdx.x;
-            if (at < chunks) {
-              float v[N];
-#pragma unroll
-              for (int e = 0; e < N; ++e) v[e] = scale == scale ? c[s][e] : 0.f;
-              store_i8<N>(x8 + r * kp + at * N, v, div, N);
-            }
-          }
-          if (threadIdx.x == 0) sc[r] = scale;
-        }
+        if (mine < a.m) rows.put(x8 + mine * kp, kp, sc + mine, t, red);
         __syncthreads();
       }
     }
@@ -467,27 +474,30 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
     const dim3 grid((a.n + 15) / 16);
     if (a.m <= 16) linear_few_kernel<OT, 1, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     else if (a.m <= 32) linear_few_kernel<OT, 2, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
-    else linear_few_kernel<OT, 4, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
+    else linear_few_kernel<OT, 3, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     return hipGetLastError();
   }
   const bool rows16 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw | a.k) & 15) == 0 &&
                       a.ldx < (1 << 22) && a.ldw < (1 << 22);
   if (rows16 && tiles_of(64) < (1 << 22)) {
     if (tiles_of(256) >= 192) return tiled<OT, ACT, 256, 256, 2, 4, 128, 2>(a, s);
-    if (tiles_of(128) >= 512) return tiled<OT, ACT, 128, 128, 2, 2, 128, 2>(a, s);
+    if (tiles_of(128) >= 224) return tiled<OT, ACT, 128, 128, 2, 2, 128, 2>(a, s);
     return tiled<OT, ACT, 64, 64, 2, 2, 128, 3>(a, s);
   }
   const int64_t tiles = tiles_of(64);
   linear_any_kernel<OT><<<grid_of(tiles), 256, 0, s>>>(a, (a.n + 63) / 64, tiles);
   return hipGetLastError();
 }
+template <int OT, int XT>
+hipError_t fused(const LinearArgs& a, hipStream_t s) {
+  const dim3 grid((a.n + 15) / 16);
+  if (a.m == 1) linear_few_kernel<OT, 1, XT, true><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  else linear_few_kernel<OT, 1, XT, false><<<grid, 64 * kFewWaves, 0, s>>>(a);
+  return hipGetLastError();
+}
 template <int OT>
 hipError_t fused(int x_type, const LinearArgs& a, hipStream_t s) {
-  const dim3 grid((a.n + 15) / 16);
-  if (x_type == T_F32) linear_few_kernel<OT, 1, T_F32><<<grid, 64 * kFewWaves, 0, s>>>(a);
-  else if (x_type == T_BF16) linear_few_kernel<OT, 1, T_BF16><<<grid, 64 * kFewWaves, 0, s>>>(a);
-  else linear_few_kernel<OT, 1, T_F16><<<grid, 64 * kFewWaves, 0, s>>>(a);
-  return hipGetLastError();
+  return x_type == T_F32 ? fused<OT, T_F32>(a, s) : x_type == T_BF16 ? fused<OT, T_BF16>(a, s) : fused<OT, T_F16>(a, s);
 }
 }  // namespace
 
@@ -496,7 +506,10 @@ hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
   return a.out_type == T_F32 ? linear<T_F32, 0>(a, s) : a.out_type == T_BF16 ? linear<T_BF16, 0>(a, s) : linear<T_F16, 0>(a, s);
 }
 
-bool linear_fuses_rows(int64_t m, int k) { return m <= 16 && m * round_up(k, 64) <= kFusedMost; }
+// One launch instead of two, as long as every workgroup's own conversion costs less than the second launch (bf16, GPU time
+// alone): one row 4096 -> 1024 4.7 us against 7.9, eight rows 1024 -> 4096 4.9 against 6.5; but sixteen rows, two a wave, 7.6
+// against 6.6 and two rows of 4096 8.9 against 7.9.
+bool linear_fuses_rows(int64_t m, int k) { return k <= (m == 1 ? kFusedRow : kFusedWave) && m <= kFewWaves; }
 
 hipError_t launch_linear_fused(int x_type, const LinearArgs& a, hipStream_t s) {
   return a.out_type == T_F32 ? fused<T_F32>(x_type, a, s) : a.out_type == T_BF16 ? fused<T_BF16>(x_type, a, s) : fused<T_F16>(x_type, a, s);
