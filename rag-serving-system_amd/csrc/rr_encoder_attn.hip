@@ -322,26 +322,225 @@ __global__ __launch_bounds__(64 * kWaves) void attn_rows_kernel(AttnParams p) {
   }
 }
 
-// joins the pieces of a tile
+// ---- many query rows -------------------------------------------------------------------------------------------------
+// 16-bit types. A workgroup takes 128 query rows, 32 a wave, and 64 keys a step: the keys' K and V rows go through registers
+// into LDS (two buffers: one barrier a step, the next step's rows are on their way during this one), where every wave reads
+// them for its own queries in 32 x 32 x 16 matrix instructions. Keys that do not take part become zeros on the way, whatever
+// they held. Lane (i = lane % 32, half = lane / 32) holds the scores of query i with keys 8 (r / 4) + 4 half + r % 4 of a
+// 32-key block, r < 16; eight of them in a row (r / 8 = t) are its slots of the second product's 16-key contraction t.
+// V lies in LDS as in memory; the transposing LDS read hands each lane four keys of one dimension.
+constexpr int kTileRows = 128, kTileKeys = 64;
+
+// LDS position of 16-byte column c of key row r: the 16 lanes that read a column of 16 K rows at once, and the 32 lanes that
+// read 64 bytes of four V rows at once, each meet all 64 banks.
+template <int DP>
+__device__ __forceinline__ unsigned k_at(unsigned r, unsigned c) {
+  constexpr unsigned kCols = DP / 8, kPerCycle = 16 / kCols;
+  return (r * kCols + (c ^ (r / kPerCycle % kCols))) * 16;
+}
+template <int DP>
+__device__ __forceinline__ unsigned v_at(unsigned r, unsigned c) {
+  constexpr unsigned kCols = DP / 8;
+  if constexpr (DP == 128) return (r * kCols + (c ^ 4 * (r % 4))) * 16;
+  if constexpr (DP == 64) return (r * kCols + (c ^ 4 * (r / 2 % 2))) * 16;
+  return (r * kCols + c) * 16;
+}
+
+template <int TY>
+__device__ __forceinline__ f32x16 mma32(u32x4 x, u32x4 y, f32x16 c) {
+  if constexpr (TY == T_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+__device__ __forceinline__ u32x2 read_transposed(const char* lds) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lds));
+}
+
 template <int TY, int DP>
+__global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
+  using E = typename Elem<TY>::type;
+  typedef E e8 __attribute__((ext_vector_type(8)));
+  constexpr int kCols = DP / 8, kLoads = kTileKeys * kCols / 256, kBuf = kTileKeys * DP * 2;
+  __shared__ __align__(1024) char lds[2][2][kBuf];
+  const AttnArgs& a = p.a;
+  const int b = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x % p.splits, tile0 = blockIdx.x / p.splits;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, half = lane >> 5;
+  const Span sq = queries_of(a, b), sk = keys_of(a, b);
+  const int64_t rows = (int64_t)sq.n * p.group;
+  const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
+  const E* vbase = static_cast<const E*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
+  const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+  auto takes_part = [&](int k) { return k < sk.n && (!mask || mask[k]); };
+
+  for (int64_t tile = tile0; tile * kTileRows < rows; tile += p.tiles) {
+    const bool whole = p.splits == 1 || tile >= p.tiles;
+    if (whole && split) break;
+    const int pieces = whole ? 1 : p.splits;
+    const int64_t row = tile * kTileRows + wave * 32 + i;
+    const bool busy = tile * kTileRows + wave * 32 < rows;   // (of this wave)
+    u32x4 q[DP / 16];
+    {
+      const int64_t qi = row / p.group;
+      const int h = kvh * p.group + (int)(row % p.group);
+      const E* at = static_cast<const E*>(a.q) + (a.q_offsets ? sq.first * a.q_ts : b * a.q_bs) + qi * a.q_ts + h * a.q_hs;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        q[s] = u32x4{0, 0, 0, 0};
+        if (qi < sq.n && 16 * s + 8 * half < a.d) q[s] = load_as<u32x4>(at + 16 * s + 8 * half);
+      }
+    }
+    u32x4 kr[kLoads], vr[kLoads];
+    auto fetch = [&](int kb) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int x = j * 256 + threadIdx.x, k = kb + x / kCols, c = 8 * (x % kCols);
+        kr[j] = vr[j] = u32x4{0, 0, 0, 0};
+        if (c < a.d && takes_part(k)) {
+          kr[j] = load_as<u32x4>(kbase + k * a.k_ts + c);
+          vr[j] = load_as<u32x4>(vbase + k * a.v_ts + c);
+        }
+      }
+    };
+    auto keep = [&](int buf) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int x = j * 256 + threadIdx.x;
+        *reinterpret_cast<u32x4*>(lds[buf][0] + k_at<DP>(x / kCols, x % kCols)) = kr[j];
+        *reinterpret_cast<u32x4*>(lds[buf][1] + v_at<DP>(x / kCols, x % kCols)) = vr[j];
+      }
+    };
+    f32x16 acc[DP / 32] = {};
+    float m = -INFINITY, l = 0.f;
+    const int step = pieces * kTileKeys;
+    int kb = split * kTileKeys, buf = 0;
+    if (kb < sk.n) {
+      fetch(kb);
+      keep(0);
+    }
+    for (; kb < sk.n; kb += step, buf ^= 1) {
+      __syncthreads();
+      const bool more = kb + step < sk.n;
+      if (more) fetch(kb + step);
+      if (busy) {
+        const uint64_t valid = __ballot(takes_part(kb + lane));
+        f32x16 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          s[h] = f32x16{};
+#pragma unroll
+          for (int st = 0; st < DP / 16; ++st)
+            s[h] = mma32<TY>(*reinterpret_cast<const u32x4*>(lds[buf][0] + k_at<DP>(32 * h + i, 2 * st + half)), q[st], s[h]);
+        }
+        if (valid != ~0ull) {   // bits 8 (r / 4) + r % 4 of what is left after this half's shift
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned mine = (unsigned)(valid >> 32 * h) >> 4 * half;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[h][r] = (mine >> (8 * (r / 4) + r % 4) & 1) ? s[h][r] * p.c : -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[h][r] *= p.c;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, s[h][r]);
+        if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
+          top = fmaxf(top, __shfl_xor(top, 32));
+          const float to = fmaxf(m, top);
+          const float f = to == m ? 1.f : exp2_fast(m - to);
+          m = to;
+          l *= f;
+#pragma unroll
+          for (int t = 0; t < DP / 32; ++t) acc[t] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            e8 w;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const float e = exp2_fast(s[h][8 * t + x] - ref);
+              l += e;
+              w[x] = (E)e;
+            }
+            const int key = 32 * h + 16 * t + 4 * half + i % 16 / 4;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) {
+              const int c = 4 * dt + 2 * (i / 16) + i % 4 / 2;
+              const u32x2 lo = read_transposed(lds[buf][1] + v_at<DP>(key, c) + 8 * (i % 2));
+              const u32x2 hi = read_transposed(lds[buf][1] + v_at<DP>(key + 8, c) + 8 * (i % 2));
+              acc[dt] = mma32<TY>(u32x4{lo[0], lo[1], hi[0], hi[1]}, __builtin_bit_cast(u32x4, w), acc[dt]);
+            }
+          }
+      }
+      if (more) keep(buf ^ 1);   // (last read before the barrier above)
+    }
+    __syncthreads();   // (a tile after this one writes the buffers again)
+    l += __shfl_xor(l, 32);
+    if (!busy) continue;
+    if (whole) {
+      E* to = out_row<E>(p, sq, b, kvh, row);
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      if (to) {
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            typedef E e4 __attribute__((ext_vector_type(4)));
+            const int d = 32 * dt + 8 * r + 4 * half;
+            e4 v;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = (E)(acc[dt][4 * r + x] * inv);
+            if (d < a.d) store_as(to + d, v);
+          }
+      }
+    } else {
+      float* ws = a.ws + ((((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits + split) * kTileRows * (DP + 2);
+      const int at = wave * 32 + i;
+      if (half == 0) {
+        ws[at] = m;
+        ws[kTileRows + at] = l;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          store_as(ws + 2 * kTileRows + at * DP + 32 * dt + 8 * r + 4 * half,
+                   f32x4{acc[dt][4 * r], acc[dt][4 * r + 1], acc[dt][4 * r + 2], acc[dt][4 * r + 3]});
+    }
+  }
+}
+
+// joins the pieces of a tile
+template <int TY, int DP, int ROWS>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   using E = typename Elem<TY>::type;
   const AttnArgs& a = p.a;
-  const int b = blockIdx.z, kvh = blockIdx.y, tile = blockIdx.x;
+  constexpr int kPiece = ROWS * (DP + 2);
+  const int b = blockIdx.z, kvh = blockIdx.y, tile = blockIdx.x / (ROWS / 16), row0 = blockIdx.x % (ROWS / 16) * 16;
   const Span sq = queries_of(a, b);
-  const float* ws = a.ws + (((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits * kRows * (DP + 2);
-  for (int x = threadIdx.x; x < kRows * DP; x += 256) {
-    const int row = x / DP, d = x % DP;
-    E* to = out_row<E>(p, sq, b, kvh, (int64_t)tile * kRows + row);
+  const float* ws = a.ws + (((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits * kPiece;
+  for (int x = threadIdx.x; x < 16 * DP; x += 256) {
+    const int row = row0 + x / DP, d = x % DP;
+    E* to = out_row<E>(p, sq, b, kvh, (int64_t)tile * ROWS + row);
     if (!to || d >= a.d) continue;
     float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ws[s * kRows * (DP + 2) + row]);
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ws[s * kPiece + row]);
     float o = 0.f, sum = 0.f;
     for (int s = 0; s < p.splits; ++s) {
-      const float* w = ws + s * kRows * (DP + 2);
+      const float* w = ws + s * kPiece;
       const float f = w[row] == top ? 1.f : exp2_fast(w[row] - top);
-      o += f * w[2 * kRows + x];
-      sum += f * w[kRows + row];
+      o += f * w[2 * ROWS + row * DP + d];
+      sum += f * w[ROWS + row];
     }
     to[d] = (E)(sum == 0.f ? 0.f : o / sum);
   }
@@ -349,49 +548,66 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
 
 int padded_d(int type, int d) { return d > 64 ? 128 : d > 32 || type == T_F32 ? 64 : 32; }
 
-// Pieces of the keys: enough workgroups for four on each of 256 CUs, and at least 256 keys in each.
-int split_count(int64_t groups, int max_k) {
-  int64_t n = (1024 + groups - 1) / groups;
-  const int64_t most = (max_k + 255) / 256;
+// How a launch is cut up: 128-row tiles where a key head has more than 32 query rows and a 16-bit type (below that, the
+// 16-row kernel reads the keys no more than twice and spreads them over its waves), at most 2^20 tiles (a grid holds below 2^32
+// threads; workgroups loop over the rest), and pieces of the keys for four workgroups on each of 256 CUs (16 rows) or two
+// (128), each with at least 256 keys.
+struct Plan {
+  bool tiled;
+  int tiles, splits, rows;
+  int64_t groups;
+};
+Plan plan(int type, int batch, int heads, int kv_heads, int max_q, int max_k) {
+  Plan p;
+  const int64_t rows = (int64_t)max_q * (heads / kv_heads);
+  p.tiled = type != T_F32 && rows > 32;
+  p.rows = p.tiled ? kTileRows : kRows;
+  const int64_t tiles = (rows + p.rows - 1) / p.rows;
+  p.tiles = (int)(tiles < (1 << 20) ? tiles : 1 << 20);
+  p.groups = (int64_t)p.tiles * batch * kv_heads;
+  int64_t n = p.groups ? ((p.tiled ? 512 : 1024) + p.groups - 1) / p.groups : 1;
+  const int64_t most = ((int64_t)max_k + 255) / 256;
   n = n < most ? n : most;
-  return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  p.splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  return p;
 }
 
-template <int TY, int DP>
-hipError_t run(const AttnParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.tiles * p.splits), p.a.kv_heads, p.a.batch);
-  attn_rows_kernel<TY, DP><<<grid, 64 * kWaves, 0, s>>>(p);
+template <int TY, int DP, int ROWS>
+hipError_t join(const AttnParams& p, hipStream_t s) {
   if (hipError_t e = hipGetLastError()) return e;
-  if (p.splits > 1) {
-    attn_join_kernel<TY, DP><<<dim3(p.tiles, p.a.kv_heads, p.a.batch), 256, 0, s>>>(p);
-    return hipGetLastError();
-  }
-  return hipSuccess;
+  if (p.splits == 1) return hipSuccess;
+  attn_join_kernel<TY, DP, ROWS><<<dim3(p.tiles * (ROWS / 16), p.a.kv_heads, p.a.batch), 256, 0, s>>>(p);
+  return hipGetLastError();
 }
-
-// Row tiles a launch is sized for: at most 2^20 (a grid holds below 2^32 threads), workgroups loop over the rest.
-int64_t row_tiles(int heads, int kv_heads, int max_q) {
-  const int64_t n = ((int64_t)max_q * (heads / kv_heads) + kRows - 1) / kRows;
-  return n < (1 << 20) ? n : 1 << 20;
+template <int TY, int DP>
+hipError_t run(const AttnParams& p, bool tiled, hipStream_t s) {
+  const dim3 grid((unsigned)(p.tiles * p.splits), p.a.kv_heads, p.a.batch);
+  if constexpr (TY != T_F32)
+    if (tiled) {
+      attn_tile_kernel<TY, DP><<<grid, 256, 0, s>>>(p);
+      return join<TY, DP, kTileRows>(p, s);
+    }
+  attn_rows_kernel<TY, DP><<<grid, 64 * kWaves, 0, s>>>(p);
+  return join<TY, DP, kRows>(p, s);
 }
 
 }  // namespace
 
 int64_t attention_workspace(int type, int batch, int heads, int kv_heads, int d, int max_q, int max_k) {
-  const int64_t tiles = row_tiles(heads, kv_heads, max_q), groups = tiles * batch * kv_heads;
-  if (groups == 0) return 0;
-  const int n = split_count(groups, max_k);
-  return n == 1 ? 0 : groups * n * kRows * (padded_d(type, d) + 2) * 4;
+  const Plan p = plan(type, batch, heads, kv_heads, max_q, max_k);
+  return p.splits == 1 ? 0 : p.groups * p.splits * p.rows * (padded_d(type, d) + 2) * 4;
 }
 
 hipError_t launch_attention(int type, const AttnArgs& a, hipStream_t s) {
-  AttnParams p{a, (float)(a.scale * 1.4426950408889634), a.heads / a.kv_heads,
-               (int)row_tiles(a.heads, a.kv_heads, a.max_q), 1};
-  p.splits = split_count((int64_t)p.tiles * a.batch * a.kv_heads, a.max_k);
+  const Plan n = plan(type, a.batch, a.heads, a.kv_heads, a.max_q, a.max_k);
+  const AttnParams p{a, (float)(a.scale * 1.4426950408889634), a.heads / a.kv_heads, n.tiles, n.splits};
   const int dp = padded_d(type, a.d);
-  if (type == T_F32) return dp == 64 ? run<T_F32, 64>(p, s) : run<T_F32, 128>(p, s);
-  if (type == T_BF16) return dp == 32 ? run<T_BF16, 32>(p, s) : dp == 64 ? run<T_BF16, 64>(p, s) : run<T_BF16, 128>(p, s);
-  return dp == 32 ? run<T_F16, 32>(p, s) : dp == 64 ? run<T_F16, 64>(p, s) : run<T_F16, 128>(p, s);
+  if (type == T_F32) return dp == 64 ? run<T_F32, 64>(p, false, s) : run<T_F32, 128>(p, false, s);
+  if (type == T_BF16)
+    return dp == 32   ? run<T_BF16, 32>(p, n.tiled, s)
+           : dp == 64 ? run<T_BF16, 64>(p, n.tiled, s)
+                      : run<T_BF16, 128>(p, n.tiled, s);
+  return dp == 32 ? run<T_F16, 32>(p, n.tiled, s) : dp == 64 ? run<T_F16, 64>(p, n.tiled, s) : run<T_F16, 128>(p, n.tiled, s);
 }
 
 }  // namespace enc
