@@ -85,6 +85,8 @@ int attention_sizes(int type, int32_t batch, int32_t heads, int32_t kv_heads, in
     return fail(RR_E_UNSUPPORTED, "%s: head size %d (a multiple of 8 up to %d)", me, d, RR_ATTN_DMAX);
   if (batch > 65535 || kv_heads > 65535)
     return fail(RR_E_UNSUPPORTED, "%s: batch=%d kv_heads=%d above 65535", me, batch, kv_heads);
+  if ((int64_t)batch * kv_heads > 1 << 22)
+    return fail(RR_E_UNSUPPORTED, "%s: %d sequences of %d key heads above 2^22", me, batch, kv_heads);
   if (max_q > 1 << 30 || max_k > 1 << 30)
     return fail(RR_E_UNSUPPORTED, "%s: max_q=%d max_k=%d above 2^30", me, max_q, max_k);
   return RR_OK;

@@ -9,14 +9,15 @@ namespace rr {
 namespace enc {
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kRows = 16;   // query rows of a tile: (query, head of the key head's group) pairs
 
 struct AttnParams {
   AttnArgs a;
-  float c;          // scale * log2 e
+  float c;          // |scale| * log2 e
+  bool flip;        // scale below 0: the queries change sign instead, so that larger scores are larger here too
   int group;        // heads per key head
-  int tiles;        // row tiles the launch was sized for
+  int tiles;        // row tiles of a key head the launch was sized for
+  int64_t units;    // tiles * key heads * batch
   int splits;       // pieces of the keys, each a workgroup's; joined by attn_join_kernel when more than one
 };
 
@@ -58,9 +59,11 @@ struct Core16 {
   static constexpr int VW = DP / 16;   // values of a V row a lane loads: tile t's row i is dimension VW i + t
   using E = typename Elem<TY>::type;
   typedef E e8 __attribute__((ext_vector_type(8)));
+  struct Keys {   // a block's keys and values, on their way or there
+    u32x4 k[2][kSteps];
+    unsigned v[8][VW / 2];
+  };
   u32x4 q[kSteps];
-  u32x4 kf[2][kSteps];
-  unsigned vr[8][VW / 2];
 
   static __device__ __forceinline__ int key(int g, int j) { return (j < 4 ? 0 : 12) + 4 * g + j; }
   static __device__ __forceinline__ int dim(int t, int i) { return VW * i + t; }
@@ -70,14 +73,15 @@ struct Core16 {
     else
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
   }
-  __device__ __forceinline__ void load_q(const E* row, bool there, int d, int g) {
+  __device__ __forceinline__ void load_q(const E* row, bool there, bool flip, int d, int g) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       q[s] = u32x4{0, 0, 0, 0};
       if (there && 32 * s + 8 * g < d) q[s] = load_as<u32x4>(row + 32 * s + 8 * g);
+      if (flip) q[s] ^= 0x80008000u;
     }
   }
-  __device__ __forceinline__ void load_k(const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
+  static __device__ __forceinline__ void load_k(Keys& to, const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       int key = kb + 16 * h + i;
@@ -85,12 +89,12 @@ struct Core16 {
       const E* row = base + key * ts;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        kf[h][s] = u32x4{0, 0, 0, 0};
-        if (32 * s + 8 * g < d) kf[h][s] = load_as<u32x4>(row + 32 * s + 8 * g);
+        to.k[h][s] = u32x4{0, 0, 0, 0};
+        if (32 * s + 8 * g < d) to.k[h][s] = load_as<u32x4>(row + 32 * s + 8 * g);
       }
     }
   }
-  __device__ __forceinline__ void load_v(const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
+  static __device__ __forceinline__ void load_v(Keys& to, const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
     typedef unsigned vv __attribute__((ext_vector_type(VW / 2)));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -100,23 +104,23 @@ struct Core16 {
       if (VW * i < d) v = load_as<vv>(base + k * ts + VW * i);
 #pragma unroll
       for (int p = 0; p < VW / 2; ++p) {
-        if constexpr (VW == 2) vr[j][p] = v[0];
-        else vr[j][p] = v[p];
+        if constexpr (VW == 2) to.v[j][p] = v[0];
+        else to.v[j][p] = v[p];
       }
     }
   }
-  __device__ __forceinline__ void scores(float* s) const {
+  __device__ __forceinline__ void scores(const Keys& of, float* s) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       f32x4 c = {0, 0, 0, 0};
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) c = mma(kf[h][st], q[st], c);
+      for (int st = 0; st < kSteps; ++st) c = mma(of.k[h][st], q[st], c);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[4 * h + r] = c[r];
     }
   }
   // valid: bit j says whether key j of this lane takes part; the V rows of the others may hold anything and become zeros
-  __device__ __forceinline__ void accumulate(const float* p, unsigned valid, f32x4* acc) {
+  static __device__ __forceinline__ void accumulate(Keys& of, const float* p, unsigned valid, f32x4* acc) {
     e8 pe;
 #pragma unroll
     for (int j = 0; j < 8; ++j) pe[j] = (E)p[j];
@@ -125,15 +129,15 @@ struct Core16 {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int w = 0; w < VW / 2; ++w) vr[j][w] = (valid >> j & 1) ? vr[j][w] : 0u;
+        for (int w = 0; w < VW / 2; ++w) of.v[j][w] = (valid >> j & 1) ? of.v[j][w] : 0u;
     }
 #pragma unroll
     for (int w = 0; w < VW / 2; ++w) {
       u32x4 lo, hi;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        lo[x] = __builtin_amdgcn_perm(vr[2 * x + 1][w], vr[2 * x][w], 0x05040100u);
-        hi[x] = __builtin_amdgcn_perm(vr[2 * x + 1][w], vr[2 * x][w], 0x07060302u);
+        lo[x] = __builtin_amdgcn_perm(of.v[2 * x + 1][w], of.v[2 * x][w], 0x05040100u);
+        hi[x] = __builtin_amdgcn_perm(of.v[2 * x + 1][w], of.v[2 * x][w], 0x07060302u);
       }
       acc[2 * w] = mma(lo, pb, acc[2 * w]);
       acc[2 * w + 1] = mma(hi, pb, acc[2 * w + 1]);
@@ -148,56 +152,60 @@ template <int DP>
 struct Core<T_F32, DP> {
   static constexpr int kKeys = 16, kMine = 4, kTiles = DP / 16, kSteps = DP / 16, kWide = DP / 64;
   using E = float;
-  f32x4 q[kSteps], kf[kSteps], vr[4][kWide];
+  struct Keys {
+    f32x4 k[kSteps], v[4][kWide];
+  };
+  f32x4 q[kSteps];
 
   static __device__ __forceinline__ int key(int g, int j) { return 4 * g + j; }
   static __device__ __forceinline__ int dim(int t, int i) { return 64 * (t / 4) + 4 * i + t % 4; }
-  __device__ __forceinline__ void load_q(const float* row, bool there, int d, int g) {
+  __device__ __forceinline__ void load_q(const float* row, bool there, bool flip, int d, int g) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       q[s] = f32x4{0, 0, 0, 0};
       if (there && 16 * s + 4 * g < d) q[s] = load_as<f32x4>(row + 16 * s + 4 * g);
+      if (flip) q[s] = -q[s];
     }
   }
-  __device__ __forceinline__ void load_k(const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
+  static __device__ __forceinline__ void load_k(Keys& to, const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
     int key = kb + i;
     key = key < n ? key : n - 1;
     const float* row = base + key * ts;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      kf[s] = f32x4{0, 0, 0, 0};
-      if (16 * s + 4 * g < d) kf[s] = load_as<f32x4>(row + 16 * s + 4 * g);
+      to.k[s] = f32x4{0, 0, 0, 0};
+      if (16 * s + 4 * g < d) to.k[s] = load_as<f32x4>(row + 16 * s + 4 * g);
     }
   }
-  __device__ __forceinline__ void load_v(const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
+  static __device__ __forceinline__ void load_v(Keys& to, const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       int k = kb + key(g, j);
       k = k < n ? k : n - 1;
 #pragma unroll
       for (int w = 0; w < kWide; ++w) {
-        vr[j][w] = f32x4{0, 0, 0, 0};
-        if (64 * w + 4 * i < d) vr[j][w] = load_as<f32x4>(base + k * ts + 64 * w + 4 * i);
+        to.v[j][w] = f32x4{0, 0, 0, 0};
+        if (64 * w + 4 * i < d) to.v[j][w] = load_as<f32x4>(base + k * ts + 64 * w + 4 * i);
       }
     }
   }
-  __device__ __forceinline__ void scores(float* s) const {
+  __device__ __forceinline__ void scores(const Keys& of, float* s) const {
     f32x4 c = {0, 0, 0, 0};
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) c = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[st][x], q[st][x], c, 0, 0, 0);
+      for (int x = 0; x < 4; ++x) c = __builtin_amdgcn_mfma_f32_16x16x4f32(of.k[st][x], q[st][x], c, 0, 0, 0);
 #pragma unroll
     for (int r = 0; r < 4; ++r) s[r] = c[r];
   }
-  __device__ __forceinline__ void accumulate(const float* p, unsigned valid, f32x4* acc) {
+  static __device__ __forceinline__ void accumulate(Keys& of, const float* p, unsigned valid, f32x4* acc) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int w = 0; w < kWide; ++w)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const float v = (valid >> j & 1) ? vr[j][w][t] : 0.f;
+          const float v = (valid >> j & 1) ? of.v[j][w][t] : 0.f;
           acc[4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[j], acc[4 * w + t], 0, 0, 0);
         }
   }
@@ -215,18 +223,22 @@ __device__ __forceinline__ E* out_row(const AttnParams& p, const Span& sq, int b
   return static_cast<E*>(a.out) + (a.q_offsets ? sq.first * a.o_ts : b * a.o_bs) + qi * a.o_ts + h * a.o_hs;
 }
 
-// One workgroup: one tile of 16 query rows and one piece of the keys; each wave takes every fourth block of keys, the four
-// waves' sums are joined in LDS.
-template <int TY, int DP>
-__global__ __launch_bounds__(64 * kWaves) void attn_rows_kernel(AttnParams p) {
+// Tiles of 16 query rows. WK = 1: four tiles a workgroup, a wave each, which takes all keys of its own; nothing is shared. WK
+// waves: one tile and one piece of the keys a workgroup, each wave every WK-th block of keys, their sums joined in LDS. Either
+// way a wave has its next block of keys on the way while it works on one, straight from memory into registers.
+template <int TY, int DP, int WK>
+__global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(AttnParams p) {
   using C = Core<TY, DP>;
   using E = typename C::E;
   constexpr int kLd = DP + 4;
-  __shared__ float so[kWaves][kRows][kLd];
-  __shared__ float sm[kWaves][kRows], sl[kWaves][kRows];
+  __shared__ float so[WK == 1 ? 1 : WK][kRows][kLd];
+  __shared__ float sm[WK][kRows], sl[WK][kRows];
   const AttnArgs& a = p.a;
-  const int b = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x % p.splits, tile0 = blockIdx.x / p.splits;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = WK == 1 ? 0 : threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int64_t unit = WK == 1 ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x / p.splits;
+  const int split = WK == 1 ? 0 : blockIdx.x % p.splits;
+  if (unit >= p.units) return;
+  const int tile0 = (int)(unit % p.tiles), kvh = (int)(unit / p.tiles % a.kv_heads), b = (int)(unit / p.tiles / a.kv_heads);
   const Span sq = queries_of(a, b), sk = keys_of(a, b);
   const int64_t rows = (int64_t)sq.n * p.group;
   const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
@@ -244,21 +256,27 @@ __global__ __launch_bounds__(64 * kWaves) void attn_rows_kernel(AttnParams p) {
       const int64_t qi = row / p.group;
       const int h = kvh * p.group + (int)(row % p.group);
       const E* q = static_cast<const E*>(a.q) + (a.q_offsets ? sq.first * a.q_ts : b * a.q_bs) + qi * a.q_ts + h * a.q_hs;
-      core.load_q(q, qi < sq.n, a.d, g);
+      core.load_q(q, qi < sq.n, p.flip, a.d, g);
     }
     f32x4 acc[C::kTiles] = {};
     float m = -INFINITY, l = 0.f;
-    for (int kb = (split * kWaves + wave) * C::kKeys; kb < sk.n; kb += pieces * kWaves * C::kKeys) {
-      core.load_k(kbase, a.k_ts, kb, sk.n, a.d, i, g);
-      core.load_v(vbase, a.v_ts, kb, sk.n, a.d, i, g);
+    struct Block {
+      typename C::Keys keys;
+      unsigned char there;   // of key `lane`, if there is a mask
+    } one, two;
+    auto load = [&](Block& to, int kb) {
+      to.there = 1;
+      if (mask) to.there = mask[kb + lane < sk.n ? kb + lane : sk.n - 1];
+      C::load_k(to.keys, kbase, a.k_ts, kb, sk.n, a.d, i, g);
+      C::load_v(to.keys, vbase, a.v_ts, kb, sk.n, a.d, i, g);
+    };
+    auto take = [&](Block& of, int kb) {
+      const uint64_t all = __ballot(kb + lane < sk.n && of.there);
       unsigned valid = 0;
 #pragma unroll
-      for (int j = 0; j < C::kMine; ++j) {
-        const int k = kb + C::key(g, j);
-        valid |= (k < sk.n && (!mask || mask[k]) ? 1u : 0u) << j;
-      }
+      for (int j = 0; j < C::kMine; ++j) valid |= (unsigned)(all >> C::key(g, j) & 1) << j;
       float s[C::kMine];
-      core.scores(s);
+      core.scores(of.keys, s);
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < C::kMine; ++j) top = fmaxf(top, (valid >> j & 1) ? s[j] * p.c : -INFINITY);
@@ -280,42 +298,70 @@ __global__ __launch_bounds__(64 * kWaves) void attn_rows_kernel(AttnParams p) {
         w[j] = (valid >> j & 1) ? exp2_fast(fmaf(s[j], p.c, -ref)) : 0.f;
         l += w[j];
       }
-      core.accumulate(w, valid, acc);
+      C::accumulate(of.keys, w, valid, acc);
+    };
+    const int step = pieces * WK * C::kKeys;
+    int kb = (split * WK + wave) * C::kKeys;
+    if (kb < sk.n) load(one, kb);
+    for (; kb < sk.n; kb += 2 * step) {
+      const int next = kb + step, after = next + step;
+      if (next < sk.n) load(two, next);
+      take(one, kb);
+      if (next >= sk.n) break;
+      if (after < sk.n) load(one, after);
+      take(two, next);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    __syncthreads();   // (a tile before this one may still be read)
+    if constexpr (WK == 1) {
+      E* to = out_row<E>(p, sq, b, kvh, tile * kRows + i);
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      constexpr int kRun = TY == T_F32 ? 4 : C::kTiles;   // tiles whose rows are neighbouring dimensions
+      typedef E run __attribute__((ext_vector_type(kRun)));
+      if (to)
 #pragma unroll
-    for (int t = 0; t < C::kTiles; ++t)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) so[wave][i][C::dim(t, 4 * g + r)] = acc[t][r];
-    if (g == 0) {
-      sm[wave][i] = m;
-      sl[wave][i] = l;
-    }
-    __syncthreads();
-    float* ws = whole ? nullptr
-                      : a.ws + ((((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits + split) * kRows * (DP + 2);
-    for (int x = threadIdx.x; x < kRows * DP; x += 64 * kWaves) {
-      const int row = x / DP, d = x % DP;
-      float top = sm[0][row];
+          for (int t = 0; t < C::kTiles; t += kRun) {
+            run v;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][row]);
-      float o = 0.f, sum = 0.f;
+            for (int x = 0; x < kRun; ++x) v[x] = (E)(acc[t + x][r] * inv);
+            const int d = C::dim(t, 4 * g + r);
+            if (d < a.d) store_as(to + d, v);
+          }
+    } else {
+      __syncthreads();   // (a tile before this one may still be read)
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = sm[w][row] == top ? 1.f : exp2_fast(sm[w][row] - top);
-        o += f * so[w][row][d];
-        sum += f * sl[w][row];
+      for (int t = 0; t < C::kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) so[wave][i][C::dim(t, 4 * g + r)] = acc[t][r];
+      if (g == 0) {
+        sm[wave][i] = m;
+        sl[wave][i] = l;
       }
-      if (whole) {
-        E* to = out_row<E>(p, sq, b, kvh, tile * kRows + row);
-        if (to && d < a.d) to[d] = (E)(sum == 0.f ? 0.f : o / sum);
-      } else {
-        ws[2 * kRows + x] = o;
-        if (d == 0) {
-          ws[row] = top;
-          ws[kRows + row] = sum;
+      __syncthreads();
+      float* ws = whole ? nullptr : a.ws + (unit / p.tiles * p.tiles + tile) * p.splits * kRows * (DP + 2) + split * kRows * (DP + 2);
+      for (int x = threadIdx.x; x < kRows * DP; x += 64 * WK) {
+        const int row = x / DP, d = x % DP;
+        float top = sm[0][row];
+#pragma unroll
+        for (int w = 1; w < WK; ++w) top = fmaxf(top, sm[w][row]);
+        float o = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float f = sm[w][row] == top ? 1.f : exp2_fast(sm[w][row] - top);
+          o += f * so[w][row][d];
+          sum += f * sl[w][row];
+        }
+        if (whole) {
+          E* to = out_row<E>(p, sq, b, kvh, tile * kRows + row);
+          if (to && d < a.d) to[d] = (E)(sum == 0.f ? 0.f : o / sum);
+        } else {
+          ws[2 * kRows + x] = o;
+          if (d == 0) {
+            ws[row] = top;
+            ws[kRows + row] = sum;
+          }
         }
       }
     }
@@ -365,14 +411,22 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
   constexpr int kCols = DP / 8, kLoads = kTileKeys * kCols / 256, kBuf = kTileKeys * DP * 2;
   __shared__ __align__(1024) char lds[2][2][kBuf];
   const AttnArgs& a = p.a;
-  const int b = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x % p.splits, tile0 = blockIdx.x / p.splits;
+  // Workgroups go to the 8 XCDs in turn: those of one key head, which read the same keys, stay in one XCD's cache
+  // (where the heads divide evenly).
+  const int64_t each = (int64_t)p.tiles * p.splits, heads = p.units / p.tiles;
+  const int64_t at = heads % 8 ? blockIdx.x : (blockIdx.x / 8 / each * 8 + blockIdx.x % 8) * each + blockIdx.x / 8 % each;
+  const int split = (int)(at % p.splits), tile0 = (int)(at / p.splits % p.tiles);
+  const int kvh = (int)(at / each % a.kv_heads), b = (int)(at / each / a.kv_heads);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, half = lane >> 5;
   const Span sq = queries_of(a, b), sk = keys_of(a, b);
   const int64_t rows = (int64_t)sq.n * p.group;
   const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
   const E* vbase = static_cast<const E*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
   const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
-  auto takes_part = [&](int k) { return k < sk.n && (!mask || mask[k]); };
+  // A step's keys as bits. The mask's bytes are asked for two steps ahead, before that step's rows, so that nothing waits
+  // for more than the bytes themselves.
+  auto byte_of = [&](int kb) -> unsigned char { return mask && kb + lane < sk.n ? mask[kb + lane] : 1; };
+  auto bits_of = [&](int kb, unsigned char there) -> uint64_t { return __ballot(kb + lane < sk.n && there); };
 
   for (int64_t tile = tile0; tile * kTileRows < rows; tile += p.tiles) {
     const bool whole = p.splits == 1 || tile >= p.tiles;
@@ -389,15 +443,16 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
       for (int s = 0; s < DP / 16; ++s) {
         q[s] = u32x4{0, 0, 0, 0};
         if (qi < sq.n && 16 * s + 8 * half < a.d) q[s] = load_as<u32x4>(at + 16 * s + 8 * half);
+        if (p.flip) q[s] ^= 0x80008000u;
       }
     }
     u32x4 kr[kLoads], vr[kLoads];
-    auto fetch = [&](int kb) {
+    auto fetch = [&](int kb, uint64_t bits) {
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int x = j * 256 + threadIdx.x, k = kb + x / kCols, c = 8 * (x % kCols);
         kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-        if (c < a.d && takes_part(k)) {
+        if (c < a.d && (bits >> x / kCols & 1)) {
           kr[j] = load_as<u32x4>(kbase + k * a.k_ts + c);
           vr[j] = load_as<u32x4>(vbase + k * a.v_ts + c);
         }
@@ -415,16 +470,21 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
     float m = -INFINITY, l = 0.f;
     const int step = pieces * kTileKeys;
     int kb = split * kTileKeys, buf = 0;
+    unsigned char ahead = byte_of(kb + step);
+    uint64_t valid = bits_of(kb, byte_of(kb));
     if (kb < sk.n) {
-      fetch(kb);
+      fetch(kb, valid);
       keep(0);
     }
     for (; kb < sk.n; kb += step, buf ^= 1) {
       __syncthreads();
       const bool more = kb + step < sk.n;
-      if (more) fetch(kb + step);
+      const uint64_t next = bits_of(kb + step, ahead);
+      if (more) {
+        ahead = byte_of(kb + 2 * step);
+        fetch(kb + step, next);
+      }
       if (busy) {
-        const uint64_t valid = __ballot(takes_part(kb + lane));
         f32x16 s[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -438,19 +498,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
           for (int h = 0; h < 2; ++h) {
             const unsigned mine = (unsigned)(valid >> 32 * h) >> 4 * half;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[h][r] = (mine >> (8 * (r / 4) + r % 4) & 1) ? s[h][r] * p.c : -INFINITY;
+            for (int r = 0; r < 16; ++r) s[h][r] = (mine >> (8 * (r / 4) + r % 4) & 1) ? s[h][r] : -INFINITY;
           }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[h][r] *= p.c;
         }
         float top = -INFINITY;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 16; ++r) top = fmaxf(top, s[h][r]);
+        top = top == -INFINITY ? top : top * p.c;   // (a scale of 0)
         if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
           top = fmaxf(top, __shfl_xor(top, 32));
           const float to = fmaxf(m, top);
@@ -468,7 +524,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
             e8 w;
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-              const float e = exp2_fast(s[h][8 * t + x] - ref);
+              const float e = exp2_fast(fmaf(s[h][8 * t + x], p.c, -ref));
               l += e;
               w[x] = (E)e;
             }
@@ -483,6 +539,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
           }
       }
       if (more) keep(buf ^ 1);   // (last read before the barrier above)
+      valid = next;
     }
     __syncthreads();   // (a tile after this one writes the buffers again)
     l += __shfl_xor(l, 32);
@@ -505,69 +562,98 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
       }
     } else {
       float* ws = a.ws + ((((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits + split) * kTileRows * (DP + 2);
-      const int at = wave * 32 + i;
+      const int mine = wave * 32 + i;
       if (half == 0) {
-        ws[at] = m;
-        ws[kTileRows + at] = l;
+        ws[mine] = m;
+        ws[kTileRows + mine] = l;
       }
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          store_as(ws + 2 * kTileRows + at * DP + 32 * dt + 8 * r + 4 * half,
+          store_as(ws + 2 * kTileRows + mine * DP + 32 * dt + 8 * r + 4 * half,
                    f32x4{acc[dt][4 * r], acc[dt][4 * r + 1], acc[dt][4 * r + 2], acc[dt][4 * r + 3]});
     }
   }
 }
 
-// joins the pieces of a tile
+// Joins the pieces of the tiles: a wave each row, the pieces' weights first (a lane each piece), then the pieces' sums, eight on
+// the way at a time.
 template <int TY, int DP, int ROWS>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   using E = typename Elem<TY>::type;
   const AttnArgs& a = p.a;
-  constexpr int kPiece = ROWS * (DP + 2);
-  const int b = blockIdx.z, kvh = blockIdx.y, tile = blockIdx.x / (ROWS / 16), row0 = blockIdx.x % (ROWS / 16) * 16;
-  const Span sq = queries_of(a, b);
-  const float* ws = a.ws + (((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits * kPiece;
-  for (int x = threadIdx.x; x < 16 * DP; x += 256) {
-    const int row = row0 + x / DP, d = x % DP;
-    E* to = out_row<E>(p, sq, b, kvh, (int64_t)tile * ROWS + row);
-    if (!to || d >= a.d) continue;
-    float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ws[s * kPiece + row]);
-    float o = 0.f, sum = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float* w = ws + s * kPiece;
-      const float f = w[row] == top ? 1.f : exp2_fast(w[row] - top);
-      o += f * w[2 * ROWS + row * DP + d];
-      sum += f * w[ROWS + row];
-    }
-    to[d] = (E)(sum == 0.f ? 0.f : o / sum);
+  constexpr int kPiece = ROWS * (DP + 2), kPer = DP < 64 ? 1 : DP / 64;
+  const int lane = threadIdx.x & 63, row = blockIdx.x % (ROWS / 4) * 4 + threadIdx.x / 64;
+  const int64_t unit = blockIdx.x / (ROWS / 4);
+  const int tile = (int)(unit % p.tiles), kvh = (int)(unit / p.tiles % a.kv_heads), b = (int)(unit / p.tiles / a.kv_heads);
+  E* to = out_row<E>(p, queries_of(a, b), b, kvh, (int64_t)tile * ROWS + row);
+  if (!to) return;
+  const float* ws = a.ws + unit * p.splits * kPiece;
+  float m[4], l = 0.f, top = -INFINITY;   // (at most 256 pieces)
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int s = 64 * x + lane;
+    m[x] = s < p.splits ? ws[(int64_t)s * kPiece + row] : -INFINITY;
+    top = fmaxf(top, m[x]);
   }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int s = 64 * x + lane;
+    m[x] = s >= p.splits ? 0.f : m[x] == top ? 1.f : exp2_fast(m[x] - top);
+    if (s < p.splits) l += m[x] * ws[(int64_t)s * kPiece + ROWS + row];
+  }
+  const float sum = wave_sum_f32(l);
+  typedef float vec __attribute__((ext_vector_type(kPer)));
+  vec o = 0.f;
+  const int d = lane * kPer;
+  const float* at = ws + 2 * ROWS + row * DP + (d < DP ? d : 0);
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    for (int s0 = 64 * x; s0 < p.splits && s0 < 64 * x + 64; s0 += 8) {
+      vec v[8];
+#pragma unroll
+      for (int y = 0; y < 8; ++y) v[y] = load_as<vec>(at + (int64_t)(s0 + y < p.splits ? s0 + y : s0) * kPiece);
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const float f = __shfl(m[x], s0 + y - 64 * x);
+        o += s0 + y < p.splits ? f * v[y] : vec(0.f);
+      }
+    }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+  for (int x = 0; x < kPer; ++x)
+    if (d + x < a.d) to[d + x] = (E)(o[x] * inv);
 }
 
 int padded_d(int type, int d) { return d > 64 ? 128 : d > 32 || type == T_F32 ? 64 : 32; }
 
-// How a launch is cut up: 128-row tiles where a key head has more than 32 query rows and a 16-bit type (below that, the
-// 16-row kernel reads the keys no more than twice and spreads them over its waves), at most 2^20 tiles (a grid holds below 2^32
-// threads; workgroups loop over the rest), and pieces of the keys for four workgroups on each of 256 CUs (16 rows) or two
-// (128), each with at least 256 keys.
+// How a launch is cut up.
+//   tiled  128-row tiles, where a key head has more than 32 query rows of a 16-bit type (with fewer, the 16-row kernel reads
+//          the keys no more than twice)
+//   alone  16-row tiles a wave each: tiles enough for two waves on each of 1024 SIMDs, or so few keys that a wave is done
+//          with them before a join would be
+//   else   16-row tiles, eight waves each
+// and, where those leave CUs idle, pieces of the keys, each at least 512 long, up to two workgroups a CU.
 struct Plan {
-  bool tiled;
+  bool tiled, alone;
   int tiles, splits, rows;
-  int64_t groups;
+  int64_t units;
 };
 Plan plan(int type, int batch, int heads, int kv_heads, int max_q, int max_k) {
   Plan p;
   const int64_t rows = (int64_t)max_q * (heads / kv_heads);
   p.tiled = type != T_F32 && rows > 32;
   p.rows = p.tiled ? kTileRows : kRows;
-  const int64_t tiles = (rows + p.rows - 1) / p.rows;
-  p.tiles = (int)(tiles < (1 << 20) ? tiles : 1 << 20);
-  p.groups = (int64_t)p.tiles * batch * kv_heads;
-  int64_t n = p.groups ? ((p.tiled ? 512 : 1024) + p.groups - 1) / p.groups : 1;
-  const int64_t most = ((int64_t)max_k + 255) / 256;
-  n = n < most ? n : most;
+  const int64_t tiles = (rows + p.rows - 1) / p.rows, most = ((int64_t)1 << 22) / ((int64_t)batch * kv_heads) + 1;
+  p.tiles = (int)(tiles < most ? tiles : most);   // (a grid holds below 2^32 threads; workgroups loop over the rest)
+  p.units = (int64_t)p.tiles * batch * kv_heads;
+  p.alone = !p.tiled && (max_k <= 128 || p.units >= 2048);
+  int64_t n = p.units && !p.alone ? (512 + p.units - 1) / p.units : 1;
+  const int64_t pieces = (int64_t)max_k / 512;
+  n = n < pieces ? n : pieces;
   p.splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
   return p;
 }
@@ -576,38 +662,39 @@ template <int TY, int DP, int ROWS>
 hipError_t join(const AttnParams& p, hipStream_t s) {
   if (hipError_t e = hipGetLastError()) return e;
   if (p.splits == 1) return hipSuccess;
-  attn_join_kernel<TY, DP, ROWS><<<dim3(p.tiles * (ROWS / 16), p.a.kv_heads, p.a.batch), 256, 0, s>>>(p);
+  attn_join_kernel<TY, DP, ROWS><<<dim3((unsigned)(p.units * (ROWS / 4))), 256, 0, s>>>(p);
   return hipGetLastError();
 }
 template <int TY, int DP>
-hipError_t run(const AttnParams& p, bool tiled, hipStream_t s) {
-  const dim3 grid((unsigned)(p.tiles * p.splits), p.a.kv_heads, p.a.batch);
+hipError_t run(const AttnParams& p, const Plan& n, hipStream_t s) {
+  const dim3 grid((unsigned)(p.units * p.splits));
   if constexpr (TY != T_F32)
-    if (tiled) {
+    if (n.tiled) {
       attn_tile_kernel<TY, DP><<<grid, 256, 0, s>>>(p);
       return join<TY, DP, kTileRows>(p, s);
     }
-  attn_rows_kernel<TY, DP><<<grid, 64 * kWaves, 0, s>>>(p);
+  if (n.alone) attn_rows_kernel<TY, DP, 1><<<dim3((unsigned)((p.units + 3) / 4)), 256, 0, s>>>(p);
+  else attn_rows_kernel<TY, DP, 8><<<grid, 512, 0, s>>>(p);
   return join<TY, DP, kRows>(p, s);
 }
 
 }  // namespace
 
 int64_t attention_workspace(int type, int batch, int heads, int kv_heads, int d, int max_q, int max_k) {
+  if (batch == 0) return 0;
   const Plan p = plan(type, batch, heads, kv_heads, max_q, max_k);
-  return p.splits == 1 ? 0 : p.groups * p.splits * p.rows * (padded_d(type, d) + 2) * 4;
+  return p.splits == 1 ? 0 : p.units * p.splits * p.rows * (padded_d(type, d) + 2) * 4;
 }
 
 hipError_t launch_attention(int type, const AttnArgs& a, hipStream_t s) {
   const Plan n = plan(type, a.batch, a.heads, a.kv_heads, a.max_q, a.max_k);
-  const AttnParams p{a, (float)(a.scale * 1.4426950408889634), a.heads / a.kv_heads, n.tiles, n.splits};
+  // (never 0: a masked score of -inf stays one)
+  const float c = fmaxf((float)(fabs((double)a.scale) * 1.4426950408889634), __FLT_DENORM_MIN__);
+  const AttnParams p{a, c, a.scale < 0, a.heads / a.kv_heads, n.tiles, n.units, n.splits};
   const int dp = padded_d(type, a.d);
-  if (type == T_F32) return dp == 64 ? run<T_F32, 64>(p, false, s) : run<T_F32, 128>(p, false, s);
-  if (type == T_BF16)
-    return dp == 32   ? run<T_BF16, 32>(p, n.tiled, s)
-           : dp == 64 ? run<T_BF16, 64>(p, n.tiled, s)
-                      : run<T_BF16, 128>(p, n.tiled, s);
-  return dp == 32 ? run<T_F16, 32>(p, n.tiled, s) : dp == 64 ? run<T_F16, 64>(p, n.tiled, s) : run<T_F16, 128>(p, n.tiled, s);
+  if (type == T_F32) return dp == 64 ? run<T_F32, 64>(p, n, s) : run<T_F32, 128>(p, n, s);
+  if (type == T_BF16) return dp == 32 ? run<T_BF16, 32>(p, n, s) : dp == 64 ? run<T_BF16, 64>(p, n, s) : run<T_BF16, 128>(p, n, s);
+  return dp == 32 ? run<T_F16, 32>(p, n, s) : dp == 64 ? run<T_F16, 64>(p, n, s) : run<T_F16, 128>(p, n, s);
 }
 
 }  // namespace enc

@@ -118,7 +118,7 @@ def test_attention_refuses(lib, change, word):
 
 @pytest.mark.parametrize("change,word", [
     ({"d": 12}, "head size"), ({"d": 136}, "head size"), ({"d": 0}, "head size"), ({"batch": 65536}, "65535"),
-    ({"heads": 65536, "kv_heads": 65536}, "65535"), ({"max_q": (1 << 30) + 1}, "2^30"), ({"max_k": (1 << 30) + 1}, "2^30")])
+    ({"heads": 65536, "kv_heads": 65536}, "65535"), ({"batch": 4096, "heads": 2048, "kv_heads": 2048}, "2^22"), ({"max_q": (1 << 30) + 1}, "2^30"), ({"max_k": (1 << 30) + 1}, "2^30")])
 def test_attention_unsupported(lib, change, word):
     refused(lib, attention(lib, **change), _lib.RR_E_UNSUPPORTED, word)
     if "max_q" not in change:

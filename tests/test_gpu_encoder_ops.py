@@ -396,6 +396,23 @@ def test_attention_large_scores(ops):
             check_attention(got, q, k, v, torch.ones(2, 400, dtype=torch.bool), scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq,lk,h,hkv,d", [(40, 70, 8, 8, 64), (1, 70, 8, 8, 64), (50, 3000, 2, 2, 128), (2, 3000, 4, 2, 32),
+                                           (70, 200, 16, 8, 64), (600, 90, 40, 40, 32)])
+def test_attention_scales_signs_and_holes(ops, dtype, lq, lk, h, hkv, d):
+    """Scales of 0 and below, a mask with holes of whole blocks, few and many rows, keys in pieces or not."""
+    g = gen(lq + lk)
+    q, k, v = qkv(g, 2, lq, lk, h, hkv, d, dtype)
+    there = torch.rand(2, lk, generator=g) < 0.7
+    there[0, : lk // 2] = False
+    there[1, lk // 3: 2 * lk // 3] = False
+    k2, v2 = k.clone(), v.clone()
+    k2[~there], v2[~there] = float("nan"), float("nan")
+    for scale in (0.0, -0.25, 0.1):
+        got = ops.cross_attention(q.cuda(), k2.cuda(), v2.cuda(), key_mask=there.cuda(), scale=scale)
+        check_attention(got, q, k, v, there, scale)
+
+
 def test_attention_no_keys_no_queries(ops):
     q = torch.ones(2, 3, 2, 16).cuda()
     kv = torch.ones(2, 0, 2, 16).cuda()
