@@ -75,6 +75,8 @@ int linear_sizes(int x_type, int64_t m, int32_t n, int32_t k) {
   return RR_OK;
 }
 
+constexpr int64_t kTsMost = (1 << 23) - 1;   // 64 rows of up to 4-byte elements within 32-bit byte offsets
+
 int attention_sizes(int type, int32_t batch, int32_t heads, int32_t kv_heads, int32_t d, int32_t max_q, int32_t max_k) {
   const char* me = "rr_cross_attention";
   if (!float_type(type)) return fail(RR_E_INVALID, "%s: bad type %d", me, type);
@@ -89,6 +91,8 @@ int attention_sizes(int type, int32_t batch, int32_t heads, int32_t kv_heads, in
     return fail(RR_E_UNSUPPORTED, "%s: %d sequences of %d key heads above 2^22", me, batch, kv_heads);
   if (max_q > 1 << 30 || max_k > 1 << 30)
     return fail(RR_E_UNSUPPORTED, "%s: max_q=%d max_k=%d above 2^30", me, max_q, max_k);
+  if ((int64_t)max_q * (heads / kv_heads) > 1 << 30)
+    return fail(RR_E_UNSUPPORTED, "%s: %d queries of %d heads a key head above 2^30 rows", me, max_q, heads / kv_heads);
   return RR_OK;
 }
 
@@ -217,6 +221,12 @@ int rr_cross_attention(int device, void* stream, int type, const void* q, int64_
     return fail(RR_E_INVALID, "%s: mask row stride %lld below max_k=%d", me, (long long)mask_stride, max_k);
   if (q_offsets && (total_q < 0 || total_q > 1 << 30)) return fail(RR_E_INVALID, "%s: total_q=%lld", me, (long long)total_q);
   if (k_offsets && (total_k < 0 || total_k > 1 << 30)) return fail(RR_E_INVALID, "%s: total_k=%lld", me, (long long)total_k);
+  if (q_offsets && total_q * (heads / kv_heads) > 1 << 30)
+    return fail(RR_E_UNSUPPORTED, "%s: %lld queries of %d heads a key head above 2^30 rows", me, (long long)total_q,
+                heads / kv_heads);
+  if (k_ts > kTsMost || v_ts > kTsMost)
+    return fail(RR_E_UNSUPPORTED, "%s: keys %lld and values %lld elements apart, above %lld", me, (long long)k_ts,
+                (long long)v_ts, (long long)kTsMost);
   const int eb = bytes_of(type);
   for (int64_t st : {q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, q_offsets ? 0 : q_bs, q_offsets ? 0 : o_bs,
                      k_offsets ? 0 : k_bs, k_offsets ? 0 : v_bs})

@@ -15,37 +15,53 @@ struct AttnParams {
   AttnArgs a;
   float c;          // |scale| * log2 e
   bool flip;        // scale below 0: the queries change sign instead, so that larger scores are larger here too
-  int group;        // heads per key head
-  int tiles;        // row tiles of a key head the launch was sized for
-  int64_t units;    // tiles * key heads * batch
-  int splits;       // pieces of the keys, each a workgroup's; joined by attn_join_kernel when more than one
+  unsigned group;   // heads per key head
+  unsigned tiles;   // row tiles of a key head the launch was sized for
+  unsigned units;   // tiles * key heads * batch
+  unsigned splits;       // pieces of the keys, each a workgroup's; joined by attn_join_kernel when more than one
 };
 
 struct Span {
   int64_t first;    // packed row, 0 for dense
   int n;
 };
-__device__ __forceinline__ Span queries_of(const AttnArgs& a, int b) {
-  if (!a.q_offsets) return {0, a.max_q};
-  int64_t lo = a.q_offsets[b], hi = a.q_offsets[b + 1];
-  lo = lo < 0 ? 0 : lo > a.total_q ? a.total_q : lo;
-  hi = hi < lo ? lo : hi > a.total_q ? a.total_q : hi;
+// (the same for a whole wave, and known to the compiler as such: what follows from them stays in scalar registers)
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Span span_of(const int32_t* offsets, int64_t total, int b) {
+  int64_t lo = uniform(offsets[b]), hi = uniform(offsets[b + 1]);
+  lo = lo < 0 ? 0 : lo > total ? total : lo;
+  hi = hi < lo ? lo : hi > total ? total : hi;
   return {lo, (int)(hi - lo)};
 }
+__device__ __forceinline__ Span queries_of(const AttnArgs& a, int b) {
+  return a.q_offsets ? span_of(a.q_offsets, a.total_q, b) : Span{0, a.max_q};
+}
 __device__ __forceinline__ Span keys_of(const AttnArgs& a, int b) {
-  Span s{0, a.max_k};
-  if (a.k_offsets) {
-    int64_t lo = a.k_offsets[b], hi = a.k_offsets[b + 1];
-    lo = lo < 0 ? 0 : lo > a.total_k ? a.total_k : lo;
-    hi = hi < lo ? lo : hi > a.total_k ? a.total_k : hi;
-    s = {lo, (int)(hi - lo)};
-  }
+  Span s = a.k_offsets ? span_of(a.k_offsets, a.total_k, b) : Span{0, a.max_k};
   if (a.key_lengths) {
-    const int len = a.key_lengths[b];
+    const int len = uniform(a.key_lengths[b]);
     s.n = len < 0 ? 0 : len < s.n ? len : s.n;
   }
   return s;
 }
+
+// Rows [first, first + count) of a tensor whose rows lie `ts` elements apart, as a buffer: reads behind the last row's end give
+// zeros, so that no lane has to ask whether its key is there, and 32-bit offsets reach every row of a block of keys (the
+// caller keeps ts below 2^23).
+template <class E>
+struct RowBuffer {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ RowBuffer(const E* base, int64_t ts, int first, int count, int d)
+      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(base + first * ts), 0,
+                                            count > 0 ? (int)(((count - 1) * (int)ts + d) * (int)sizeof(E)) : 0, 0x00020000)) {}
+  template <int BYTES>
+  __device__ __forceinline__ auto load(unsigned at) const {
+    if constexpr (BYTES == 16) return __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
+    else if constexpr (BYTES == 8) return __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+  }
+};
+constexpr unsigned kNowhere = 0xfffffff0u;   // an offset behind every buffer
 
 // ---- the two products of one wave over a block of keys ------------------------------------------------------------
 // Lane (i = lane % 16, g = lane / 16). DP: the head size rounded up to a whole tile.
@@ -81,31 +97,27 @@ struct Core16 {
       if (flip) q[s] ^= 0x80008000u;
     }
   }
-  static __device__ __forceinline__ void load_k(Keys& to, const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      int key = kb + 16 * h + i;
-      key = key < n ? key : n - 1;
-      const E* row = base + key * ts;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        to.k[h][s] = u32x4{0, 0, 0, 0};
-        if (32 * s + 8 * g < d) to.k[h][s] = load_as<u32x4>(row + 32 * s + 8 * g);
-      }
-    }
+  // byte offsets in a block: of this lane's part of K rows 0 .. 15 (+ 32 bytes a step) and of V rows 4g (+ a row each)
+  static __device__ __forceinline__ unsigned k_offset(unsigned ts, int i, int g) { return 2 * (i * ts + 8 * g); }
+  static __device__ __forceinline__ unsigned v_offset(unsigned ts, int i, int g, int d) {
+    return VW * i < d ? 2 * (4 * g * ts + VW * i) : kNowhere;
   }
-  static __device__ __forceinline__ void load_v(Keys& to, const E* base, int64_t ts, int kb, int n, int d, int i, int g) {
-    typedef unsigned vv __attribute__((ext_vector_type(VW / 2)));
+  static __device__ __forceinline__ void load_k(Keys& to, const RowBuffer<E>& k, unsigned at, unsigned ts, int d, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        to.k[h][s] = k.template load<16>(32 * s + 32 <= d || 32 * s + 8 * g < d ? at + 32 * h * ts + 64 * s : kNowhere);
+  }
+  static __device__ __forceinline__ void load_v(Keys& to, const RowBuffer<E>& v, unsigned at, unsigned ts) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      int k = kb + key(g, j);
-      k = k < n ? k : n - 1;
-      vv v = 0;
-      if (VW * i < d) v = load_as<vv>(base + k * ts + VW * i);
+      const unsigned row = at == kNowhere ? kNowhere : at + 2 * key(0, j) * ts;
+      const auto x = v.template load<2 * VW>(row);
 #pragma unroll
       for (int p = 0; p < VW / 2; ++p) {
-        if constexpr (VW == 2) to.v[j][p] = v[0];
-        else to.v[j][p] = v[p];
+        if constexpr (VW == 2) to.v[j][p] = x;
+        else to.v[j][p] = x[p];
       }
     }
   }
@@ -167,27 +179,19 @@ struct Core<T_F32, DP> {
       if (flip) q[s] = -q[s];
     }
   }
-  static __device__ __forceinline__ void load_k(Keys& to, const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
-    int key = kb + i;
-    key = key < n ? key : n - 1;
-    const float* row = base + key * ts;
+  static __device__ __forceinline__ unsigned k_offset(unsigned ts, int i, int g) { return 4 * (i * ts + 4 * g); }
+  static __device__ __forceinline__ unsigned v_offset(unsigned ts, int i, int g, int d) { return 4 * (4 * g * ts + 4 * i); }
+  static __device__ __forceinline__ void load_k(Keys& to, const RowBuffer<float>& k, unsigned at, unsigned ts, int d, int g) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      to.k[s] = f32x4{0, 0, 0, 0};
-      if (16 * s + 4 * g < d) to.k[s] = load_as<f32x4>(row + 16 * s + 4 * g);
-    }
+    for (int s = 0; s < kSteps; ++s)
+      to.k[s] = __builtin_bit_cast(f32x4, k.load<16>(16 * s + 16 <= d || 16 * s + 4 * g < d ? at + 64 * s : kNowhere));
   }
-  static __device__ __forceinline__ void load_v(Keys& to, const float* base, int64_t ts, int kb, int n, int d, int i, int g) {
+  // (columns behind d are the next head's: they end up in columns of the result that are not stored)
+  static __device__ __forceinline__ void load_v(Keys& to, const RowBuffer<float>& v, unsigned at, unsigned ts) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int k = kb + key(g, j);
-      k = k < n ? k : n - 1;
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int w = 0; w < kWide; ++w) {
-        to.v[j][w] = f32x4{0, 0, 0, 0};
-        if (64 * w + 4 * i < d) to.v[j][w] = load_as<f32x4>(base + k * ts + 64 * w + 4 * i);
-      }
-    }
+      for (int w = 0; w < kWide; ++w) to.v[j][w] = __builtin_bit_cast(f32x4, v.load<16>(at + 4 * j * ts + 256 * w));
   }
   __device__ __forceinline__ void scores(const Keys& of, float* s) const {
     f32x4 c = {0, 0, 0, 0};
@@ -215,11 +219,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 // where the row's results go, null if the row is not there
 template <class E>
-__device__ __forceinline__ E* out_row(const AttnParams& p, const Span& sq, int b, int kvh, int64_t row) {
+__device__ __forceinline__ E* out_row(const AttnParams& p, const Span& sq, int b, int kvh, unsigned row) {
   const AttnArgs& a = p.a;
-  const int64_t qi = row / p.group;
-  const int h = kvh * p.group + (int)(row % p.group);
-  if (qi >= sq.n) return nullptr;
+  const unsigned qi = row / p.group, h = kvh * p.group + row % p.group;
+  if ((int)qi >= sq.n) return nullptr;
   return static_cast<E*>(a.out) + (a.q_offsets ? sq.first * a.o_ts : b * a.o_bs) + qi * a.o_ts + h * a.o_hs;
 }
 
@@ -234,29 +237,29 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
   __shared__ float so[WK == 1 ? 1 : WK][kRows][kLd];
   __shared__ float sm[WK][kRows], sl[WK][kRows];
   const AttnArgs& a = p.a;
-  const int lane = threadIdx.x & 63, wave = WK == 1 ? 0 : threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int64_t unit = WK == 1 ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x / p.splits;
+  const int lane = threadIdx.x & 63, first = uniform(threadIdx.x >> 6), wave = WK == 1 ? 0 : first, i = lane & 15, g = lane >> 4;
+  const unsigned unit = WK == 1 ? blockIdx.x * 4 + first : blockIdx.x / p.splits;
   const int split = WK == 1 ? 0 : blockIdx.x % p.splits;
   if (unit >= p.units) return;
-  const int tile0 = (int)(unit % p.tiles), kvh = (int)(unit / p.tiles % a.kv_heads), b = (int)(unit / p.tiles / a.kv_heads);
+  const int tile0 = unit % p.tiles, kvh = unit / p.tiles % a.kv_heads, b = unit / p.tiles / a.kv_heads;
   const Span sq = queries_of(a, b), sk = keys_of(a, b);
-  const int64_t rows = (int64_t)sq.n * p.group;
+  const int rows = sq.n * p.group;
   const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
   const E* vbase = static_cast<const E*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
   const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
 
   // tiles behind the ones the launch was sized for (a sequence longer than max_q) take all keys in one piece
-  for (int64_t tile = tile0; tile * kRows < rows; tile += p.tiles) {
-    const bool whole = p.splits == 1 || tile >= p.tiles;
+  const unsigned k_ts = (unsigned)a.k_ts, v_ts = (unsigned)a.v_ts;
+  const unsigned k_at = C::k_offset(k_ts, i, g), v_at = C::v_offset(v_ts, i, g, a.d);
+  for (int tile = tile0; tile < (rows + kRows - 1) / kRows; tile += p.tiles) {
+    const bool whole = p.splits == 1 || tile >= (int)p.tiles;
     if (whole && split) break;
     const int pieces = whole ? 1 : p.splits;
     C core;
     {
-      const int64_t row = tile * kRows + i;
-      const int64_t qi = row / p.group;
-      const int h = kvh * p.group + (int)(row % p.group);
+      const unsigned row = tile * kRows + i, qi = row / p.group, h = kvh * p.group + row % p.group;
       const E* q = static_cast<const E*>(a.q) + (a.q_offsets ? sq.first * a.q_ts : b * a.q_bs) + qi * a.q_ts + h * a.q_hs;
-      core.load_q(q, qi < sq.n, p.flip, a.d, g);
+      core.load_q(q, (int)qi < sq.n, p.flip, a.d, g);
     }
     f32x4 acc[C::kTiles] = {};
     float m = -INFINITY, l = 0.f;
@@ -267,8 +270,9 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
     auto load = [&](Block& to, int kb) {
       to.there = 1;
       if (mask) to.there = mask[kb + lane < sk.n ? kb + lane : sk.n - 1];
-      C::load_k(to.keys, kbase, a.k_ts, kb, sk.n, a.d, i, g);
-      C::load_v(to.keys, vbase, a.v_ts, kb, sk.n, a.d, i, g);
+      const int n = sk.n - kb < C::kKeys ? sk.n - kb : C::kKeys;
+      C::load_k(to.keys, RowBuffer<E>(kbase, a.k_ts, kb, n, a.d), k_at, k_ts, a.d, g);
+      C::load_v(to.keys, RowBuffer<E>(vbase, a.v_ts, kb, n, a.d), v_at, v_ts);
     };
     auto take = [&](Block& of, int kb) {
       const uint64_t all = __ballot(kb + lane < sk.n && of.there);
@@ -340,7 +344,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
         sl[wave][i] = l;
       }
       __syncthreads();
-      float* ws = whole ? nullptr : a.ws + (unit / p.tiles * p.tiles + tile) * p.splits * kRows * (DP + 2) + split * kRows * (DP + 2);
+      float* ws = whole ? nullptr : a.ws + ((int64_t)unit * p.splits + split) * kRows * (DP + 2);
       for (int x = threadIdx.x; x < kRows * DP; x += 64 * WK) {
         const int row = x / DP, d = x % DP;
         float top = sm[0][row];
@@ -405,7 +409,7 @@ __device__ __forceinline__ u32x2 read_transposed(const char* lds) {
 }
 
 template <int TY, int DP>
-__global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnParams p) {
   using E = typename Elem<TY>::type;
   typedef E e8 __attribute__((ext_vector_type(8)));
   constexpr int kCols = DP / 8, kLoads = kTileKeys * kCols / 256, kBuf = kTileKeys * DP * 2;
@@ -413,13 +417,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
   const AttnArgs& a = p.a;
   // Workgroups go to the 8 XCDs in turn: those of one key head, which read the same keys, stay in one XCD's cache
   // (where the heads divide evenly).
-  const int64_t each = (int64_t)p.tiles * p.splits, heads = p.units / p.tiles;
-  const int64_t at = heads % 8 ? blockIdx.x : (blockIdx.x / 8 / each * 8 + blockIdx.x % 8) * each + blockIdx.x / 8 % each;
-  const int split = (int)(at % p.splits), tile0 = (int)(at / p.splits % p.tiles);
-  const int kvh = (int)(at / each % a.kv_heads), b = (int)(at / each / a.kv_heads);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, half = lane >> 5;
+  const unsigned each = p.tiles * p.splits, heads = p.units / p.tiles;
+  const unsigned at = heads % 8 ? blockIdx.x : (blockIdx.x / 8 / each * 8 + blockIdx.x % 8) * each + blockIdx.x / 8 % each;
+  const int split = at % p.splits, tile0 = at / p.splits % p.tiles;
+  const int kvh = at / each % a.kv_heads, b = at / each / a.kv_heads;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), i = lane & 31, half = lane >> 5;
   const Span sq = queries_of(a, b), sk = keys_of(a, b);
-  const int64_t rows = (int64_t)sq.n * p.group;
+  const int rows = sq.n * p.group;
   const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
   const E* vbase = static_cast<const E*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
   const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
@@ -427,43 +431,45 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
   // for more than the bytes themselves.
   auto byte_of = [&](int kb) -> unsigned char { return mask && kb + lane < sk.n ? mask[kb + lane] : 1; };
   auto bits_of = [&](int kb, unsigned char there) -> uint64_t { return __ballot(kb + lane < sk.n && there); };
+  // this thread's 16 bytes of load j: key row 256 j / kCols + threadIdx.x / kCols, column threadIdx.x % kCols
+  const int r0 = threadIdx.x / kCols, c0 = threadIdx.x % kCols;
+  const unsigned from_k = 2 * (r0 * (unsigned)a.k_ts + 8 * c0), from_v = 2 * (r0 * (unsigned)a.v_ts + 8 * c0);
 
-  for (int64_t tile = tile0; tile * kTileRows < rows; tile += p.tiles) {
-    const bool whole = p.splits == 1 || tile >= p.tiles;
+  for (int tile = tile0; tile < (rows + kTileRows - 1) / kTileRows; tile += p.tiles) {
+    const bool whole = p.splits == 1 || tile >= (int)p.tiles;
     if (whole && split) break;
     const int pieces = whole ? 1 : p.splits;
-    const int64_t row = tile * kTileRows + wave * 32 + i;
+    const unsigned row = tile * kTileRows + wave * 32 + i;
     const bool busy = tile * kTileRows + wave * 32 < rows;   // (of this wave)
     u32x4 q[DP / 16];
     {
-      const int64_t qi = row / p.group;
-      const int h = kvh * p.group + (int)(row % p.group);
-      const E* at = static_cast<const E*>(a.q) + (a.q_offsets ? sq.first * a.q_ts : b * a.q_bs) + qi * a.q_ts + h * a.q_hs;
+      const unsigned qi = row / p.group, h = kvh * p.group + row % p.group;
+      const E* from = static_cast<const E*>(a.q) + (a.q_offsets ? sq.first * a.q_ts : b * a.q_bs) + qi * a.q_ts + h * a.q_hs;
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
         q[s] = u32x4{0, 0, 0, 0};
-        if (qi < sq.n && 16 * s + 8 * half < a.d) q[s] = load_as<u32x4>(at + 16 * s + 8 * half);
+        if ((int)qi < sq.n && 16 * s + 8 * half < a.d) q[s] = load_as<u32x4>(from + 16 * s + 8 * half);
         if (p.flip) q[s] ^= 0x80008000u;
       }
     }
     u32x4 kr[kLoads], vr[kLoads];
     auto fetch = [&](int kb, uint64_t bits) {
+      const int n = sk.n - kb < kTileKeys ? sk.n - kb : kTileKeys;
+      const RowBuffer<E> k(kbase, a.k_ts, kb, n, a.d), v(vbase, a.v_ts, kb, n, a.d);
+      const bool in = 8 * c0 < a.d;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int x = j * 256 + threadIdx.x, k = kb + x / kCols, c = 8 * (x % kCols);
-        kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-        if (c < a.d && (bits >> x / kCols & 1)) {
-          kr[j] = load_as<u32x4>(kbase + k * a.k_ts + c);
-          vr[j] = load_as<u32x4>(vbase + k * a.v_ts + c);
-        }
+        constexpr int kApart = 256 / kCols;
+        const bool there = in && (bits >> (r0 + kApart * j) & 1);
+        kr[j] = k.template load<16>(there ? from_k + 2 * kApart * j * (unsigned)a.k_ts : kNowhere);
+        vr[j] = v.template load<16>(there ? from_v + 2 * kApart * j * (unsigned)a.v_ts : kNowhere);
       }
     };
     auto keep = [&](int buf) {
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int x = j * 256 + threadIdx.x;
-        *reinterpret_cast<u32x4*>(lds[buf][0] + k_at<DP>(x / kCols, x % kCols)) = kr[j];
-        *reinterpret_cast<u32x4*>(lds[buf][1] + v_at<DP>(x / kCols, x % kCols)) = vr[j];
+        *reinterpret_cast<u32x4*>(lds[buf][0] + k_at<DP>(r0 + 256 / kCols * j, c0)) = kr[j];
+        *reinterpret_cast<u32x4*>(lds[buf][1] + v_at<DP>(r0 + 256 / kCols * j, c0)) = vr[j];
       }
     };
     f32x16 acc[DP / 32] = {};
@@ -485,46 +491,39 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
         fetch(kb + step, next);
       }
       if (busy) {
-        f32x16 s[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          s[h] = f32x16{};
+        for (int h = 0; h < 2; ++h) {   // 32 keys at a time: the registers of more would cost a workgroup per CU
+          const unsigned here = (unsigned)(valid >> 32 * h);
+          if (here == 0) continue;
+          f32x16 s = {};
 #pragma unroll
           for (int st = 0; st < DP / 16; ++st)
-            s[h] = mma32<TY>(*reinterpret_cast<const u32x4*>(lds[buf][0] + k_at<DP>(32 * h + i, 2 * st + half)), q[st], s[h]);
-        }
-        if (valid != ~0ull) {   // bits 8 (r / 4) + r % 4 of what is left after this half's shift
+            s = mma32<TY>(*reinterpret_cast<const u32x4*>(lds[buf][0] + k_at<DP>(32 * h + i, 2 * st + half)), q[st], s);
+          if (here != ~0u) {
+            const unsigned mine = here >> 4 * half;   // bits 8 (r / 4) + r % 4
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const unsigned mine = (unsigned)(valid >> 32 * h) >> 4 * half;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[h][r] = (mine >> (8 * (r / 4) + r % 4) & 1) ? s[h][r] : -INFINITY;
+            for (int r = 0; r < 16; ++r) s[r] = (mine >> (8 * (r / 4) + r % 4) & 1) ? s[r] : -INFINITY;
           }
-        }
-        float top = -INFINITY;
+          float top = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+          top = top == -INFINITY ? top : top * p.c;
+          if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float to = fmaxf(m, top);
+            const float f = to == m ? 1.f : exp2_fast(m - to);
+            m = to;
+            l *= f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, s[h][r]);
-        top = top == -INFINITY ? top : top * p.c;   // (a scale of 0)
-        if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const float to = fmaxf(m, top);
-          const float f = to == m ? 1.f : exp2_fast(m - to);
-          m = to;
-          l *= f;
-#pragma unroll
-          for (int t = 0; t < DP / 32; ++t) acc[t] *= f;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int t = 0; t < DP / 32; ++t) acc[t] *= f;
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             e8 w;
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-              const float e = exp2_fast(fmaf(s[h][8 * t + x], p.c, -ref));
+              const float e = exp2_fast(fmaf(s[8 * t + x], p.c, -ref));
               l += e;
               w[x] = (E)e;
             }
@@ -537,6 +536,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
               acc[dt] = mma32<TY>(u32x4{lo[0], lo[1], hi[0], hi[1]}, __builtin_bit_cast(u32x4, w), acc[dt]);
             }
           }
+        }
       }
       if (more) keep(buf ^ 1);   // (last read before the barrier above)
       valid = next;
@@ -561,7 +561,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnParams p) {
           }
       }
     } else {
-      float* ws = a.ws + ((((int64_t)b * a.kv_heads + kvh) * p.tiles + tile) * p.splits + split) * kTileRows * (DP + 2);
+      const int64_t unit = ((int64_t)b * a.kv_heads + kvh) * p.tiles + tile;
+      float* ws = a.ws + (unit * p.splits + split) * kTileRows * (DP + 2);
       const int mine = wave * 32 + i;
       if (half == 0) {
         ws[mine] = m;
@@ -585,16 +586,17 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   const AttnArgs& a = p.a;
   constexpr int kPiece = ROWS * (DP + 2), kPer = DP < 64 ? 1 : DP / 64;
   const int lane = threadIdx.x & 63, row = blockIdx.x % (ROWS / 4) * 4 + threadIdx.x / 64;
-  const int64_t unit = blockIdx.x / (ROWS / 4);
-  const int tile = (int)(unit % p.tiles), kvh = (int)(unit / p.tiles % a.kv_heads), b = (int)(unit / p.tiles / a.kv_heads);
-  E* to = out_row<E>(p, queries_of(a, b), b, kvh, (int64_t)tile * ROWS + row);
+  const unsigned unit = blockIdx.x / (ROWS / 4);
+  const int tile = unit % p.tiles, kvh = unit / p.tiles % a.kv_heads, b = unit / p.tiles / a.kv_heads;
+  E* to = out_row<E>(p, queries_of(a, b), b, kvh, tile * ROWS + row);
   if (!to) return;
-  const float* ws = a.ws + unit * p.splits * kPiece;
+  const int splits = p.splits;
+  const float* ws = a.ws + (int64_t)unit * splits * kPiece;
   float m[4], l = 0.f, top = -INFINITY;   // (at most 256 pieces)
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int s = 64 * x + lane;
-    m[x] = s < p.splits ? ws[(int64_t)s * kPiece + row] : -INFINITY;
+    m[x] = s < splits ? ws[(int64_t)s * kPiece + row] : -INFINITY;
     top = fmaxf(top, m[x]);
   }
 #pragma unroll
@@ -602,8 +604,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int s = 64 * x + lane;
-    m[x] = s >= p.splits ? 0.f : m[x] == top ? 1.f : exp2_fast(m[x] - top);
-    if (s < p.splits) l += m[x] * ws[(int64_t)s * kPiece + ROWS + row];
+    m[x] = s >= splits ? 0.f : m[x] == top ? 1.f : exp2_fast(m[x] - top);
+    if (s < splits) l += m[x] * ws[(int64_t)s * kPiece + ROWS + row];
   }
   const float sum = wave_sum_f32(l);
   typedef float vec __attribute__((ext_vector_type(kPer)));
@@ -612,14 +614,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   const float* at = ws + 2 * ROWS + row * DP + (d < DP ? d : 0);
 #pragma unroll
   for (int x = 0; x < 4; ++x)
-    for (int s0 = 64 * x; s0 < p.splits && s0 < 64 * x + 64; s0 += 8) {
+    for (int s0 = 64 * x; s0 < splits && s0 < 64 * x + 64; s0 += 8) {
       vec v[8];
 #pragma unroll
-      for (int y = 0; y < 8; ++y) v[y] = load_as<vec>(at + (int64_t)(s0 + y < p.splits ? s0 + y : s0) * kPiece);
+      for (int y = 0; y < 8; ++y) v[y] = load_as<vec>(at + (int64_t)(s0 + y < splits ? s0 + y : s0) * kPiece);
 #pragma unroll
       for (int y = 0; y < 8; ++y) {
         const float f = __shfl(m[x], s0 + y - 64 * x);
-        o += s0 + y < p.splits ? f * v[y] : vec(0.f);
+        o += s0 + y < splits ? f * v[y] : vec(0.f);
       }
     }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -690,7 +692,7 @@ hipError_t launch_attention(int type, const AttnArgs& a, hipStream_t s) {
   const Plan n = plan(type, a.batch, a.heads, a.kv_heads, a.max_q, a.max_k);
   // (never 0: a masked score of -inf stays one)
   const float c = fmaxf((float)(fabs((double)a.scale) * 1.4426950408889634), __FLT_DENORM_MIN__);
-  const AttnParams p{a, c, a.scale < 0, a.heads / a.kv_heads, n.tiles, n.units, n.splits};
+  const AttnParams p{a, c, a.scale < 0, (unsigned)(a.heads / a.kv_heads), (unsigned)n.tiles, (unsigned)n.units, (unsigned)n.splits};
   const int dp = padded_d(type, a.d);
   if (type == T_F32) return dp == 64 ? run<T_F32, 64>(p, n, s) : run<T_F32, 128>(p, n, s);
   if (type == T_BF16) return dp == 32 ? run<T_BF16, 32>(p, n, s) : dp == 64 ? run<T_BF16, 64>(p, n, s) : run<T_BF16, 128>(p, n, s);

@@ -118,10 +118,12 @@ def test_attention_refuses(lib, change, word):
 
 @pytest.mark.parametrize("change,word", [
     ({"d": 12}, "head size"), ({"d": 136}, "head size"), ({"d": 0}, "head size"), ({"batch": 65536}, "65535"),
-    ({"heads": 65536, "kv_heads": 65536}, "65535"), ({"batch": 4096, "heads": 2048, "kv_heads": 2048}, "2^22"), ({"max_q": (1 << 30) + 1}, "2^30"), ({"max_k": (1 << 30) + 1}, "2^30")])
+    ({"heads": 65536, "kv_heads": 65536}, "65535"), ({"batch": 4096, "heads": 2048, "kv_heads": 2048}, "2^22"),
+    ({"ks": (1 << 24, 1 << 23, 16)}, "apart"), ({"vs": (1 << 24, 1 << 23, 16)}, "apart"),
+    ({"max_q": 1 << 29, "heads": 8}, "2^30 rows"), ({"qo": P, "total_q": 1 << 29, "heads": 8}, "2^30 rows"), ({"max_q": (1 << 30) + 1}, "2^30"), ({"max_k": (1 << 30) + 1}, "2^30")])
 def test_attention_unsupported(lib, change, word):
     refused(lib, attention(lib, **change), _lib.RR_E_UNSUPPORTED, word)
-    if "max_q" not in change:
+    if not {"max_q", "ks", "vs", "qo"} & set(change):
         assert lib.rr_cross_attention_workspace(1, change.get("batch", 2), change.get("heads", 2), change.get("kv_heads", 2),
                                                 change.get("d", 16), 2, change.get("max_k", 2)) == _lib.RR_E_UNSUPPORTED
 

@@ -382,6 +382,26 @@ def test_attention_mixed_forms_and_strides(ops, dtype):
         plain.within(got[i], want, err, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq,h,hkv,d", [(1, 4, 2, 64), (50, 2, 2, 64), (3, 2, 1, 128), (90, 2, 1, 24), (40, 1, 1, 128)])
+def test_attention_unaligned_and_broadcast_keys(ops, dtype, lq, h, hkv, d):
+    """Keys and values that start at odd elements, rows of odd spacing, heads in front of tokens; keys shared by the batch, and
+    one row shared by every key (strides of 0)."""
+    g = gen(lq + d)
+    lk = 75
+    q = rand(g, 2, lq, h, d).to(dtype).cuda()
+    k = rand(g, 2, hkv, lk, d + 5).to(dtype).cuda()[..., 1:1 + d].transpose(1, 2)
+    v = rand(g, 2, hkv, lk, d + 3).to(dtype).cuda()[..., 3:3 + d].transpose(1, 2)
+    all_ = torch.ones(2, lk, dtype=torch.bool)
+    check_attention(ops.cross_attention(q, k, v), q, k, v, all_, d ** -0.5)
+    k1, v1 = k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1)
+    check_attention(ops.cross_attention(q, k1, v1), q, k1, v1, all_, d ** -0.5)
+    k1, v1 = k[:, :1].expand(-1, lk, -1, -1), v[:, :1].expand(-1, lk, -1, -1)
+    lens = torch.tensor([lk, 7], dtype=torch.int32)
+    check_attention(ops.cross_attention(q, k1, v1, key_lengths=lens.cuda()), q, k1, v1, torch.arange(lk) < lens[:, None],
+                    d ** -0.5)
+
+
 def test_attention_large_scores(ops):
     """Scores of thousands: the maximum is found before anything overflows; a first key far below the others."""
     g = gen(6)
