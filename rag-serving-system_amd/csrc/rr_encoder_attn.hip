@@ -60,6 +60,16 @@ struct RowBuffer {
     else if constexpr (BYTES == 8) return __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
     else return __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
   }
+  // 16 bytes a lane to LDS address `to` + 16 * lane
+  __device__ __forceinline__ void to_lds(unsigned at, unsigned to) const {
+    unsigned keep;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(at), "s"(r), "s"(to)
+        : "memory");
+  }
 };
 constexpr unsigned kNowhere = 0xfffffff0u;   // an offset behind every buffer
 
@@ -109,11 +119,11 @@ struct Core16 {
       for (int s = 0; s < kSteps; ++s)
         to.k[h][s] = k.template load<16>(32 * s + 32 <= d || 32 * s + 8 * g < d ? at + 32 * h * ts + 64 * s : kNowhere);
   }
+  // (ts: 0 in lanes that have no part of a row, which stay at kNowhere)
   static __device__ __forceinline__ void load_v(Keys& to, const RowBuffer<E>& v, unsigned at, unsigned ts) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const unsigned row = at == kNowhere ? kNowhere : at + 2 * key(0, j) * ts;
-      const auto x = v.template load<2 * VW>(row);
+      const auto x = v.template load<2 * VW>(at + 2 * key(0, j) * ts);
 #pragma unroll
       for (int p = 0; p < VW / 2; ++p) {
         if constexpr (VW == 2) to.v[j][p] = x;
@@ -250,7 +260,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
 
   // tiles behind the ones the launch was sized for (a sequence longer than max_q) take all keys in one piece
   const unsigned k_ts = (unsigned)a.k_ts, v_ts = (unsigned)a.v_ts;
-  const unsigned k_at = C::k_offset(k_ts, i, g), v_at = C::v_offset(v_ts, i, g, a.d);
+  const unsigned k_at = C::k_offset(k_ts, i, g), v_at = C::v_offset(v_ts, i, g, a.d), v_step = v_at == kNowhere ? 0 : v_ts;
   for (int tile = tile0; tile < (rows + kRows - 1) / kRows; tile += p.tiles) {
     const bool whole = p.splits == 1 || tile >= (int)p.tiles;
     if (whole && split) break;
@@ -272,7 +282,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
       if (mask) to.there = mask[kb + lane < sk.n ? kb + lane : sk.n - 1];
       const int n = sk.n - kb < C::kKeys ? sk.n - kb : C::kKeys;
       C::load_k(to.keys, RowBuffer<E>(kbase, a.k_ts, kb, n, a.d), k_at, k_ts, a.d, g);
-      C::load_v(to.keys, RowBuffer<E>(vbase, a.v_ts, kb, n, a.d), v_at, v_ts);
+      C::load_v(to.keys, RowBuffer<E>(vbase, a.v_ts, kb, n, a.d), v_at, v_step);
     };
     auto take = [&](Block& of, int kb) {
       const uint64_t all = __ballot(kb + lane < sk.n && of.there);
@@ -372,28 +382,28 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
   }
 }
 
-// ---- many query rows -------------------------------------------------------------------------------------------------
-// 16-bit types. A workgroup takes 128 query rows, 32 a wave, and 64 keys a step: the keys' K and V rows go through registers
-// into LDS (two buffers: one barrier a step, the next step's rows are on their way during this one), where every wave reads
-// them for its own queries in 32 x 32 x 16 matrix instructions. Keys that do not take part become zeros on the way, whatever
-// they held. Lane (i = lane % 32, half = lane / 32) holds the scores of query i with keys 8 (r / 4) + 4 half + r % 4 of a
-// 32-key block, r < 16; eight of them in a row (r / 8 = t) are its slots of the second product's 16-key contraction t.
-// V lies in LDS as in memory; the transposing LDS read hands each lane four keys of one dimension.
-constexpr int kTileRows = 128, kTileKeys = 64;
+// ---- 16-bit types, keys through LDS -----------------------------------------------------------------------------------
+// A workgroup of four waves brings a step's K and V rows into LDS (whole rows at a time, two buffers: one barrier a step, the
+// next step's rows are on their way during this one) and multiplies them in 32 x 32 x 16 instructions, 32 query rows and 32
+// keys at a time. WK = 1: 128 query rows, 32 a wave; every wave takes every key, 64 a step. WK = 4: 32 query rows, of which
+// every wave takes another 32 of 128 keys a step, and their sums are joined in LDS: for few rows, where bandwidth counts.
+// Keys that do not take part are read as zeros, whatever they held. Lane (i = lane % 32, half = lane / 32) holds the scores
+// of query i with keys 8 (r / 4) + 4 half + r % 4 of a 32-key block, r < 16; eight of them in a row (r / 8 = t) are its slots
+// of the second product's 16-key contraction t. V lies in LDS as in memory; the transposing LDS read hands each lane four keys
+// of one dimension.
+// DMA: rows at 16-byte addresses go to LDS by the loads themselves; others through registers.
+constexpr int kTileRows = 128, kFewRows = 32;
 
-// LDS position of 16-byte column c of key row r: the 16 lanes that read a column of 16 K rows at once, and the 32 lanes that
-// read 64 bytes of four V rows at once, each meet all 64 banks.
+// The 16-byte column of key row r that lies at column c of its LDS row (and the other way round): the 16 lanes that read a
+// column of 16 K rows at once, and the 32 lanes that read 64 bytes of four V rows at once, each meet all 64 banks.
 template <int DP>
-__device__ __forceinline__ unsigned k_at(unsigned r, unsigned c) {
+__device__ __forceinline__ unsigned k_column(unsigned r, unsigned c) {
   constexpr unsigned kCols = DP / 8, kPerCycle = 16 / kCols;
-  return (r * kCols + (c ^ (r / kPerCycle % kCols))) * 16;
+  return c ^ (r / kPerCycle % kCols);
 }
 template <int DP>
-__device__ __forceinline__ unsigned v_at(unsigned r, unsigned c) {
-  constexpr unsigned kCols = DP / 8;
-  if constexpr (DP == 128) return (r * kCols + (c ^ 4 * (r % 4))) * 16;
-  if constexpr (DP == 64) return (r * kCols + (c ^ 4 * (r / 2 % 2))) * 16;
-  return (r * kCols + c) * 16;
+__device__ __forceinline__ unsigned v_column(unsigned r, unsigned c) {
+  return DP == 128 ? c ^ 4 * (r % 4) : DP == 64 ? c ^ 4 * (r / 2 % 2) : c;
 }
 
 template <int TY>
@@ -408,12 +418,15 @@ __device__ __forceinline__ u32x2 read_transposed(const char* lds) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lds));
 }
 
-template <int TY, int DP>
+template <int TY, int DP, int WK, bool DMA>
 __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnParams p) {
   using E = typename Elem<TY>::type;
   typedef E e8 __attribute__((ext_vector_type(8)));
-  constexpr int kCols = DP / 8, kLoads = kTileKeys * kCols / 256, kBuf = kTileKeys * DP * 2;
-  __shared__ __align__(1024) char lds[2][2][kBuf];
+  constexpr int kRowsHere = WK == 1 ? kTileRows : kFewRows, kKeys = WK == 1 ? 64 : 128, kWords = kKeys / 64;
+  constexpr int kCols = DP / 8, kLoads = kKeys * kCols / 256, kHalf = kKeys * DP * 2, kBuf = 2 * kHalf;
+  constexpr int kLd = DP + 4;
+  constexpr int kJoin = WK == 1 ? 0 : WK * kFewRows * (kLd + 2) * 4;
+  __shared__ __align__(1024) char lds[2 * kBuf > kJoin ? 2 * kBuf : kJoin];
   const AttnArgs& a = p.a;
   // Workgroups go to the 8 XCDs in turn: those of one key head, which read the same keys, stay in one XCD's cache
   // (where the heads divide evenly).
@@ -429,18 +442,71 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
   const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
   // A step's keys as bits. The mask's bytes are asked for two steps ahead, before that step's rows, so that nothing waits
   // for more than the bytes themselves.
-  auto byte_of = [&](int kb) -> unsigned char { return mask && kb + lane < sk.n ? mask[kb + lane] : 1; };
-  auto bits_of = [&](int kb, unsigned char there) -> uint64_t { return __ballot(kb + lane < sk.n && there); };
-  // this thread's 16 bytes of load j: key row 256 j / kCols + threadIdx.x / kCols, column threadIdx.x % kCols
-  const int r0 = threadIdx.x / kCols, c0 = threadIdx.x % kCols;
-  const unsigned from_k = 2 * (r0 * (unsigned)a.k_ts + 8 * c0), from_v = 2 * (r0 * (unsigned)a.v_ts + 8 * c0);
+  struct Bytes {
+    unsigned char there[kWords];
+  };
+  struct Bits {
+    uint64_t word[kWords];
+  };
+  auto bytes_of = [&](int kb) {
+    Bytes r;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) r.there[w] = mask && kb + 64 * w + lane < sk.n ? mask[kb + 64 * w + lane] : 1;
+    return r;
+  };
+  auto bits_of = [&](int kb, const Bytes& of) {
+    Bits r;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) r.word[w] = __ballot(kb + 64 * w + lane < sk.n && of.there[w]);
+    return r;
+  };
+  // this lane's 16 bytes of load j: key row (4 j + wave) 64 / kCols + lane / kCols, at LDS column lane % kCols
+  const unsigned r0 = wave * (64 / kCols) + lane / kCols, c0 = lane % kCols;
+  constexpr unsigned kApart = 256 / kCols;   // (a multiple of the swizzles' periods: the columns are the same for every j)
+  const unsigned ck = k_column<DP>(r0, c0), cv = v_column<DP>(r0, c0);
+  const unsigned from_k = 2 * (r0 * (unsigned)a.k_ts + 8 * ck), from_v = 2 * (r0 * (unsigned)a.v_ts + 8 * cv);
+  const bool in_k = (int)(8 * ck) < a.d, in_v = (int)(8 * cv) < a.d;
+  const unsigned lds0 = (unsigned)(uintptr_t)lds;
 
-  for (int tile = tile0; tile < (rows + kTileRows - 1) / kTileRows; tile += p.tiles) {
+  for (int tile = tile0; tile < (rows + kRowsHere - 1) / kRowsHere; tile += p.tiles) {
     const bool whole = p.splits == 1 || tile >= (int)p.tiles;
     if (whole && split) break;
     const int pieces = whole ? 1 : p.splits;
-    const unsigned row = tile * kTileRows + wave * 32 + i;
-    const bool busy = tile * kTileRows + wave * 32 < rows;   // (of this wave)
+    const unsigned row = tile * kRowsHere + (WK == 1 ? wave * 32 : 0) + i;
+    const bool busy = WK > 1 || tile * kRowsHere + wave * 32 < rows;   // (of this wave)
+    u32x4 kr[DMA ? 1 : kLoads], vr[DMA ? 1 : kLoads];
+    auto fetch = [&](int kb, const Bits& bits, int buf) {
+      const int n = sk.n - kb < kKeys ? sk.n - kb : kKeys;
+      const RowBuffer<E> k(kbase, a.k_ts, kb, n, a.d), v(vbase, a.v_ts, kb, n, a.d);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const unsigned r = r0 + kApart * j;
+        const bool there = (kWords == 1 || 64 / kCols * (4 * j + wave) < 64 ? bits.word[0] : bits.word[kWords - 1]) >> (r % 64) & 1;
+        const unsigned at_k = there && in_k ? from_k + 2 * kApart * j * (unsigned)a.k_ts : kNowhere;
+        const unsigned at_v = there && in_v ? from_v + 2 * kApart * j * (unsigned)a.v_ts : kNowhere;
+        if constexpr (DMA) {
+          const unsigned to = lds0 + buf * kBuf + (4 * j + wave) * 1024;
+          k.to_lds(at_k, to);
+          v.to_lds(at_v, to + kHalf);
+        } else {
+          kr[j] = k.template load<16>(at_k);
+          vr[j] = v.template load<16>(at_v);
+        }
+      }
+    };
+    auto keep = [&](int buf) {
+      if constexpr (!DMA)
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          char* to = lds + buf * kBuf + (4 * j + wave) * 1024 + lane * 16;
+          *reinterpret_cast<u32x4*>(to) = kr[j];
+          *reinterpret_cast<u32x4*>(to + kHalf) = vr[j];
+        }
+    };
+    const int step = pieces * kKeys;
+    int kb = split * kKeys, buf = 0;
+    Bytes ahead = bytes_of(kb + step);
+    Bits valid = bits_of(kb, bytes_of(kb));
     u32x4 q[DP / 16];
     {
       const unsigned qi = row / p.group, h = kvh * p.group + row % p.group;
@@ -449,131 +515,167 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
       for (int s = 0; s < DP / 16; ++s) {
         q[s] = u32x4{0, 0, 0, 0};
         if ((int)qi < sq.n && 16 * s + 8 * half < a.d) q[s] = load_as<u32x4>(from + 16 * s + 8 * half);
-        if (p.flip) q[s] ^= 0x80008000u;
       }
     }
-    u32x4 kr[kLoads], vr[kLoads];
-    auto fetch = [&](int kb, uint64_t bits) {
-      const int n = sk.n - kb < kTileKeys ? sk.n - kb : kTileKeys;
-      const RowBuffer<E> k(kbase, a.k_ts, kb, n, a.d), v(vbase, a.v_ts, kb, n, a.d);
-      const bool in = 8 * c0 < a.d;
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        constexpr int kApart = 256 / kCols;
-        const bool there = in && (bits >> (r0 + kApart * j) & 1);
-        kr[j] = k.template load<16>(there ? from_k + 2 * kApart * j * (unsigned)a.k_ts : kNowhere);
-        vr[j] = v.template load<16>(there ? from_v + 2 * kApart * j * (unsigned)a.v_ts : kNowhere);
-      }
-    };
-    auto keep = [&](int buf) {
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        *reinterpret_cast<u32x4*>(lds[buf][0] + k_at<DP>(r0 + 256 / kCols * j, c0)) = kr[j];
-        *reinterpret_cast<u32x4*>(lds[buf][1] + v_at<DP>(r0 + 256 / kCols * j, c0)) = vr[j];
-      }
-    };
-    f32x16 acc[DP / 32] = {};
-    float m = -INFINITY, l = 0.f;
-    const int step = pieces * kTileKeys;
-    int kb = split * kTileKeys, buf = 0;
-    unsigned char ahead = byte_of(kb + step);
-    uint64_t valid = bits_of(kb, byte_of(kb));
     if (kb < sk.n) {
-      fetch(kb, valid);
+      fetch(kb, valid, 0);
       keep(0);
     }
-    for (; kb < sk.n; kb += step, buf ^= 1) {
-      __syncthreads();
-      const bool more = kb + step < sk.n;
-      const uint64_t next = bits_of(kb + step, ahead);
-      if (more) {
-        ahead = byte_of(kb + 2 * step);
-        fetch(kb + step, next);
+    if (p.flip)
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) q[s] ^= 0x80008000u;
+    f32x16 acc[DP / 32] = {};
+    float m = -INFINITY, l = 0.f;
+    // 32 keys of the buffer, rows key0 and on, `here` those that take part
+    auto take = [&](const char* k_rows, int key0, unsigned here) {
+      f32x16 s = {};
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st) {
+        const unsigned r = key0 + i;
+        s = mma32<TY>(*reinterpret_cast<const u32x4*>(k_rows + (r * kCols + k_column<DP>(r, 2 * st + half)) * 16), q[st], s);
       }
-      if (busy) {
+      if (here != ~0u) {
+        const unsigned mine = here >> 4 * half;   // bits 8 (r / 4) + r % 4
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {   // 32 keys at a time: the registers of more would cost a workgroup per CU
-          const unsigned here = (unsigned)(valid >> 32 * h);
-          if (here == 0) continue;
-          f32x16 s = {};
+        for (int r = 0; r < 16; ++r) s[r] = (mine >> (8 * (r / 4) + r % 4) & 1) ? s[r] : -INFINITY;
+      }
+      float top = -INFINITY;
 #pragma unroll
-          for (int st = 0; st < DP / 16; ++st)
-            s = mma32<TY>(*reinterpret_cast<const u32x4*>(lds[buf][0] + k_at<DP>(32 * h + i, 2 * st + half)), q[st], s);
-          if (here != ~0u) {
-            const unsigned mine = here >> 4 * half;   // bits 8 (r / 4) + r % 4
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+      top = top == -INFINITY ? top : top * p.c;
+      if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float to = fmaxf(m, top);
+        const float f = to == m ? 1.f : exp2_fast(m - to);
+        m = to;
+        l *= f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = (mine >> (8 * (r / 4) + r % 4) & 1) ? s[r] : -INFINITY;
-          }
-          float top = -INFINITY;
+        for (int t = 0; t < DP / 32; ++t) acc[t] *= f;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-          top = top == -INFINITY ? top : top * p.c;
-          if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float to = fmaxf(m, top);
-            const float f = to == m ? 1.f : exp2_fast(m - to);
-            m = to;
-            l *= f;
+      for (int t = 0; t < 2; ++t) {
+        e8 w;
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t) acc[t] *= f;
-          }
-          const float ref = m == -INFINITY ? 0.f : m;
+        for (int x = 0; x < 8; ++x) {
+          const float e = exp2_fast(fmaf(s[8 * t + x], p.c, -ref));
+          l += e;
+          w[x] = (E)e;
+        }
+        const unsigned r = key0 + 16 * t + 4 * half + i % 16 / 4;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            e8 w;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const float e = exp2_fast(fmaf(s[8 * t + x], p.c, -ref));
-              l += e;
-              w[x] = (E)e;
-            }
-            const int key = 32 * h + 16 * t + 4 * half + i % 16 / 4;
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) {
-              const int c = 4 * dt + 2 * (i / 16) + i % 4 / 2;
-              const u32x2 lo = read_transposed(lds[buf][1] + v_at<DP>(key, c) + 8 * (i % 2));
-              const u32x2 hi = read_transposed(lds[buf][1] + v_at<DP>(key + 8, c) + 8 * (i % 2));
-              acc[dt] = mma32<TY>(u32x4{lo[0], lo[1], hi[0], hi[1]}, __builtin_bit_cast(u32x4, w), acc[dt]);
-            }
-          }
+        for (int dt = 0; dt < DP / 32; ++dt) {
+          const unsigned c = 4 * dt + 2 * (i / 16) + i % 4 / 2;
+          const char* v_rows = k_rows + kHalf + 8 * (i % 2);
+          const u32x2 lo = read_transposed(v_rows + (r * kCols + v_column<DP>(r, c)) * 16);
+          const u32x2 hi = read_transposed(v_rows + ((r + 8) * kCols + v_column<DP>(r + 8, c)) * 16);
+          acc[dt] = mma32<TY>(u32x4{lo[0], lo[1], hi[0], hi[1]}, __builtin_bit_cast(u32x4, w), acc[dt]);
         }
       }
-      if (more) keep(buf ^ 1);   // (last read before the barrier above)
+    };
+    for (; kb < sk.n; kb += step, buf ^= 1) {
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (this step's rows are in LDS)
+      else __syncthreads();
+      const bool more = kb + step < sk.n;
+      const Bits next = bits_of(kb + step, ahead);
+      if (more) {
+        ahead = bytes_of(kb + 2 * step);
+        fetch(kb + step, next, buf ^ 1);   // (last read before the barrier above)
+      }
+      const char* k_rows = lds + buf * kBuf;
+      if constexpr (WK == 1) {
+        if (busy)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (const unsigned here = (unsigned)(valid.word[0] >> 32 * h)) take(k_rows, 32 * h, here);
+      } else {
+        const unsigned here = (unsigned)((wave < 2 ? valid.word[0] : valid.word[kWords - 1]) >> 32 * (wave % 2));
+        if (here) take(k_rows, 32 * wave, here);
+      }
+      if (more) keep(buf ^ 1);
       valid = next;
     }
-    __syncthreads();   // (a tile after this one writes the buffers again)
+    __syncthreads();   // (the buffers are written again: by the join, or by a tile after this one)
     l += __shfl_xor(l, 32);
-    if (!busy) continue;
-    if (whole) {
-      E* to = out_row<E>(p, sq, b, kvh, row);
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      if (to) {
+    const int64_t unit = ((int64_t)b * a.kv_heads + kvh) * p.tiles + tile;
+    float* ws = whole ? nullptr : a.ws + (unit * p.splits + split) * kRowsHere * (DP + 2);
+    if constexpr (WK == 1) {
+      if (!busy) continue;
+      if (whole) {
+        E* to = out_row<E>(p, sq, b, kvh, row);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (to) {
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              typedef E e4 __attribute__((ext_vector_type(4)));
+              const int d = 32 * dt + 8 * r + 4 * half;
+              e4 v;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) v[x] = (E)(acc[dt][4 * r + x] * inv);
+              if (d < a.d) store_as(to + d, v);
+            }
+        }
+      } else {
+        const int mine = wave * 32 + i;
+        if (half == 0) {
+          ws[mine] = m;
+          ws[kRowsHere + mine] = l;
+        }
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            typedef E e4 __attribute__((ext_vector_type(4)));
-            const int d = 32 * dt + 8 * r + 4 * half;
-            e4 v;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] = (E)(acc[dt][4 * r + x] * inv);
-            if (d < a.d) store_as(to + d, v);
-          }
+          for (int r = 0; r < 4; ++r)
+            store_as(ws + 2 * kRowsHere + mine * DP + 32 * dt + 8 * r + 4 * half,
+                     f32x4{acc[dt][4 * r], acc[dt][4 * r + 1], acc[dt][4 * r + 2], acc[dt][4 * r + 3]});
       }
     } else {
-      const int64_t unit = ((int64_t)b * a.kv_heads + kvh) * p.tiles + tile;
-      float* ws = a.ws + (unit * p.splits + split) * kTileRows * (DP + 2);
-      const int mine = wave * 32 + i;
-      if (half == 0) {
-        ws[mine] = m;
-        ws[kTileRows + mine] = l;
-      }
+      float* so = reinterpret_cast<float*>(lds);             // [WK][kFewRows][kLd]
+      float* sm = so + WK * kFewRows * kLd;                  // [WK][kFewRows]
+      float* sl = sm + WK * kFewRows;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          store_as(ws + 2 * kTileRows + mine * DP + 32 * dt + 8 * r + 4 * half,
-                   f32x4{acc[dt][4 * r], acc[dt][4 * r + 1], acc[dt][4 * r + 2], acc[dt][4 * r + 3]});
+          *reinterpret_cast<f32x4*>(so + (wave * kFewRows + i) * kLd + 32 * dt + 8 * r + 4 * half) =
+              f32x4{acc[dt][4 * r], acc[dt][4 * r + 1], acc[dt][4 * r + 2], acc[dt][4 * r + 3]};
+      if (half == 0) {
+        sm[wave * kFewRows + i] = m;
+        sl[wave * kFewRows + i] = l;
+      }
+      __syncthreads();
+      const int last = rows - tile * kRowsHere < kRowsHere ? rows - tile * kRowsHere : kRowsHere;
+      for (int x = threadIdx.x; x < last * DP / 4; x += 256) {   // four dimensions of a row
+        const int r = x / (DP / 4), d = x % (DP / 4) * 4;
+        float top = sm[r];
+#pragma unroll
+        for (int w = 1; w < WK; ++w) top = fmaxf(top, sm[w * kFewRows + r]);
+        f32x4 o = {0, 0, 0, 0};
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float mw = sm[w * kFewRows + r], f = mw == top ? 1.f : exp2_fast(mw - top);
+          o += f * *reinterpret_cast<const f32x4*>(so + (w * kFewRows + r) * kLd + d);
+          sum += f * sl[w * kFewRows + r];
+        }
+        if (whole) {
+          typedef E e4 __attribute__((ext_vector_type(4)));
+          E* to = out_row<E>(p, sq, b, kvh, tile * kRowsHere + r);
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          e4 v;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) v[y] = (E)(o[y] * inv);
+          if (to && d < a.d) store_as(to + d, v);
+        } else {
+          store_as(ws + 2 * kRowsHere + r * DP + d, o);
+          if (d == 0) {
+            ws[r] = top;
+            ws[kRowsHere + r] = sum;
+          }
+        }
+      }
+      __syncthreads();   // (a tile after this one writes the buffers again)
     }
   }
 }
@@ -633,27 +735,28 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
 int padded_d(int type, int d) { return d > 64 ? 128 : d > 32 || type == T_F32 ? 64 : 32; }
 
 // How a launch is cut up.
-//   tiled  128-row tiles, where a key head has more than 32 query rows of a 16-bit type (with fewer, the 16-row kernel reads
-//          the keys no more than twice)
-//   alone  16-row tiles a wave each: tiles enough for two waves on each of 1024 SIMDs, or so few keys that a wave is done
-//          with them before a join would be
-//   else   16-row tiles, eight waves each
+//   16-bit types  128-row tiles where a key head has more than 32 query rows, else 32-row tiles
+//   fp32          16-row tiles, eight waves each
+//   alone         16-row tiles, a wave each: with so few keys that a wave is done with them before a join would be (a 16-bit
+//                 type's key heads of at most 32 query rows, or fp32), or, fp32, tiles enough for two waves on each of 1024 SIMDs
 // and, where those leave CUs idle, pieces of the keys, each at least 512 long, up to two workgroups a CU.
+enum class Way { kAlone, kRows, kFew, kTile };
 struct Plan {
-  bool tiled, alone;
+  Way way;
   int tiles, splits, rows;
   int64_t units;
 };
 Plan plan(int type, int batch, int heads, int kv_heads, int max_q, int max_k) {
   Plan p;
   const int64_t rows = (int64_t)max_q * (heads / kv_heads);
-  p.tiled = type != T_F32 && rows > 32;
-  p.rows = p.tiled ? kTileRows : kRows;
+  const int64_t sixteens = (rows + kRows - 1) / kRows * batch * kv_heads;
+  if (type == T_F32) p.way = max_k <= 128 || sixteens >= 2048 ? Way::kAlone : Way::kRows;
+  else p.way = rows > kFewRows ? Way::kTile : max_k <= 128 ? Way::kAlone : Way::kFew;
+  p.rows = p.way == Way::kTile ? kTileRows : p.way == Way::kFew ? kFewRows : kRows;
   const int64_t tiles = (rows + p.rows - 1) / p.rows, most = ((int64_t)1 << 22) / ((int64_t)batch * kv_heads) + 1;
   p.tiles = (int)(tiles < most ? tiles : most);   // (a grid holds below 2^32 threads; workgroups loop over the rest)
   p.units = (int64_t)p.tiles * batch * kv_heads;
-  p.alone = !p.tiled && (max_k <= 128 || p.units >= 2048);
-  int64_t n = p.units && !p.alone ? (512 + p.units - 1) / p.units : 1;
+  int64_t n = p.units && p.way != Way::kAlone ? (512 + p.units - 1) / p.units : 1;
   const int64_t pieces = (int64_t)max_k / 512;
   n = n < pieces ? n : pieces;
   p.splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
@@ -670,14 +773,26 @@ hipError_t join(const AttnParams& p, hipStream_t s) {
 template <int TY, int DP>
 hipError_t run(const AttnParams& p, const Plan& n, hipStream_t s) {
   const dim3 grid((unsigned)(p.units * p.splits));
-  if constexpr (TY != T_F32)
-    if (n.tiled) {
-      attn_tile_kernel<TY, DP><<<grid, 256, 0, s>>>(p);
+  if (n.way == Way::kAlone) {
+    attn_rows_kernel<TY, DP, 1><<<dim3((unsigned)((p.units + 3) / 4)), 256, 0, s>>>(p);
+    return hipGetLastError();
+  }
+  if constexpr (TY == T_F32) {
+    attn_rows_kernel<TY, DP, 8><<<grid, 512, 0, s>>>(p);
+    return join<TY, DP, kRows>(p, s);
+  } else {
+    const AttnArgs& a = p.a;
+    const bool dma = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | 2 * (a.k_ts | a.k_hs | a.v_ts | a.v_hs) |
+                       (a.k_offsets ? 0 : 2 * (a.k_bs | a.v_bs))) & 15) == 0;
+    if (n.way == Way::kTile) {
+      if (dma) attn_tile_kernel<TY, DP, 1, true><<<grid, 256, 0, s>>>(p);
+      else attn_tile_kernel<TY, DP, 1, false><<<grid, 256, 0, s>>>(p);
       return join<TY, DP, kTileRows>(p, s);
     }
-  if (n.alone) attn_rows_kernel<TY, DP, 1><<<dim3((unsigned)((p.units + 3) / 4)), 256, 0, s>>>(p);
-  else attn_rows_kernel<TY, DP, 8><<<grid, 512, 0, s>>>(p);
-  return join<TY, DP, kRows>(p, s);
+    if (dma) attn_tile_kernel<TY, DP, 4, true><<<grid, 256, 0, s>>>(p);
+    else attn_tile_kernel<TY, DP, 4, false><<<grid, 256, 0, s>>>(p);
+    return join<TY, DP, kFewRows>(p, s);
+  }
 }
 
 }  // namespace
