@@ -8,10 +8,12 @@ SURVEY.md §8a row a8), same result/error conventions. Differences, all on the r
   retrievers do) the (B, 1024) fp32 tensor's device pointer is handed to the C-ABI
   (``rr_set_queries_device``) instead of the reference's ``.cpu().numpy()`` round trip (:92);
   ``device_handoff=False`` restores the host path;
+* ``encoder="hip"`` runs the embedding model's forward pass on the HIP operators in 8 bits (``core.encoder.HipEncoder``, an
+  approximation of the fp32 model) instead of PyTorch's; the default leaves the model as it is;
 * the LLM prompt list is passed directly (the reference wraps it in ``datasets.Dataset`` only to read
   the same list back, :104-105).
 
-The embedding half (e5 forward) is PyTorch-ROCm, as BASELINE config 4 specifies; its semantics are kept
+The embedding half (e5 forward) is PyTorch-ROCm by default, as BASELINE config 4 specifies; its semantics are kept
 exactly: "query: " prefix, tokenizer(padding=True, truncation=True), ``last_hidden_state.mean(dim=1)``
 over ALL positions (pad tokens included, no attention-mask weighting) and no L2 normalisation
 (:83-91).
@@ -41,10 +43,17 @@ class BatchProcessor(threading.Thread):
     """Background thread that processes batches of RAG requests (batch_processor.py:15-125)."""
 
     def __init__(self, request_queue, embedding_model: dict, llm_model, retriever, device: str = "cuda",
-                 polling_interval: float = 0.1, device_handoff: bool = True):
+                 polling_interval: float = 0.1, device_handoff: bool = True, encoder: str = "torch"):
         super().__init__(daemon=True)
         import torch
+        if encoder not in ("torch", "hip"):
+            raise ValueError(f"encoder must be 'torch' or 'hip', not {encoder!r}")
+        if encoder == "hip" and torch.device(device).type != "cuda":
+            raise ValueError(f"encoder='hip' runs on the GPU only, not on {device}")
         self.request_queue = request_queue
+        if encoder == "hip":
+            from .encoder import HipEncoder
+            embedding_model = {**embedding_model, "model": HipEncoder(embedding_model["model"])}
         self.embedding_model = embedding_model
         self.llm_model = llm_model
         self.retriever = retriever

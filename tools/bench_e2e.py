@@ -2,7 +2,10 @@
 """BASELINE config 4 — SQuAD end to end on one GPU: e5-large-shaped query encoder (PyTorch-ROCm) + the HIP
 retriever, batch 32. Reports the latency split embed / retrieve.
 
-    python tools/bench_e2e.py [--batches 30] [--warmup 3] [--batch 32] [--dtype fp32]
+    python tools/bench_e2e.py [--batches 30] [--warmup 3] [--batch 32] [--dtype fp32] [--encoder torch|hip]
+
+--encoder hip: the same encoder's forward pass on the HIP operators in 8 bits (rag_service_amd.core.encoder.HipEncoder)
+instead of PyTorch's fp32; the result then also says how near its embeddings are to PyTorch's.
 
 What runs is the reference's embedding half (batch_processor.py:81-92, restated in
 rag_service_amd.core.batch_processor.embed_queries: "query: " prefix, padding + truncation, encoder forward,
@@ -61,6 +64,7 @@ def main():
     ap.add_argument("--batch", type=int, default=32)
     ap.add_argument("--k", type=int, default=2, help="the HTTP default k (api/models.py:6)")
     ap.add_argument("--dtype", default="fp32", choices=["fp32", "bf16", "fp32-split"])
+    ap.add_argument("--encoder", default="torch", choices=["torch", "hip"])
     args = ap.parse_args()
 
     import torch
@@ -75,10 +79,19 @@ def main():
                            pad_token_id=1, bos_token_id=0, eos_token_id=2, layer_norm_eps=1e-5)
     model = XLMRobertaModel(cfg, add_pooling_layer=False).eval().to(dev)
     emb_model = {"tokenizer": WordHashTokenizer(), "model": model}
+    nearness = {}
+    if args.encoder == "hip":
+        from rag_service_amd.core.encoder import HipEncoder
+        hip_model = {"tokenizer": WordHashTokenizer(), "model": HipEncoder(model).to(dev)}
 
     corpus = np.load(os.path.join(REPO, "tests", "golden", "data", "squad_embeddings.npy"))
     queries = json.load(open(os.path.join(REPO, "tests", "golden", "data", "squad_queries.json")))
     retr = HipRetriever(corpus, list(range(corpus.shape[0])), dtype=args.dtype)
+    if args.encoder == "hip":
+        a, b = (embed_queries(m, queries[:args.batch], dev) for m in (emb_model, hip_model))
+        cos = torch.nn.functional.cosine_similarity(a, b, dim=1)
+        nearness = {"cosine_to_torch_min": round(float(cos.min()), 5), "cosine_to_torch_mean": round(float(cos.mean()), 5)}
+        emb_model = hip_model
 
     def one_batch(i, handoff):
         qs = [queries[(i * args.batch + j) % len(queries)] for j in range(args.batch)]
@@ -121,9 +134,10 @@ def main():
         same = all(one_batch(i, True)[2] == one_batch(i, False)[2] for i in range(3))
     print(json.dumps({"config": "squad-e2e (BASELINE configs[3])", "batch": args.batch, "k": args.k,
                       "batches": args.batches, "corpus": list(corpus.shape), "corpus_dtype": args.dtype,
-                      "encoder": "XLM-RoBERTa-large architecture (e5-large-instruct), random init, fp32",
+                      "encoder": "XLM-RoBERTa-large architecture (e5-large-instruct), random init, " +
+                                 ("fp32" if args.encoder == "torch" else "8-bit products, bf16 between them (HipEncoder)"),
                       "tokenizer": "word-hash stand-in (no sentencepiece model offline)",
-                      "handoff_results_identical": same, **res}), flush=True)
+                      "handoff_results_identical": same, **nearness, **res}), flush=True)
     retr.close()
 
 
