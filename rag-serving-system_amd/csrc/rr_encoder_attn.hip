@@ -528,12 +528,30 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
     float m = -INFINITY, l = 0.f;
     // 32 keys of the buffer, rows key0 and on, `here` those that take part
     auto take = [&](const char* k_rows, int key0, unsigned here) {
-      f32x16 s = {};
+      // K is read before the first product, V before the softmax that its product waits for: the reads' latency is hidden
+      // behind arithmetic, not met once for each instruction
+      u32x4 kf[DP / 16];
 #pragma unroll
       for (int st = 0; st < DP / 16; ++st) {
         const unsigned r = key0 + i;
-        s = mma32<TY>(*reinterpret_cast<const u32x4*>(k_rows + (r * kCols + k_column<DP>(r, 2 * st + half)) * 16), q[st], s);
+        kf[st] = *reinterpret_cast<const u32x4*>(k_rows + (r * kCols + k_column<DP>(r, 2 * st + half)) * 16);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 s = {};
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st) s = mma32<TY>(kf[st], q[st], s);
+      u32x4 vf[2][DP / 32];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) {
+          const unsigned r = key0 + 16 * t + 4 * half + i % 16 / 4, c = 4 * dt + 2 * (i / 16) + i % 4 / 2;
+          const char* v_rows = k_rows + kHalf + 8 * (i % 2);
+          const u32x2 lo = read_transposed(v_rows + (r * kCols + v_column<DP>(r, c)) * 16);
+          const u32x2 hi = read_transposed(v_rows + ((r + 8) * kCols + v_column<DP>(r + 8, c)) * 16);
+          vf[t][dt] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+      __builtin_amdgcn_sched_barrier(0);
       if (here != ~0u) {
         const unsigned mine = here >> 4 * half;   // bits 8 (r / 4) + r % 4
 #pragma unroll
@@ -562,15 +580,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
           l += e;
           w[x] = (E)e;
         }
-        const unsigned r = key0 + 16 * t + 4 * half + i % 16 / 4;
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) {
-          const unsigned c = 4 * dt + 2 * (i / 16) + i % 4 / 2;
-          const char* v_rows = k_rows + kHalf + 8 * (i % 2);
-          const u32x2 lo = read_transposed(v_rows + (r * kCols + v_column<DP>(r, c)) * 16);
-          const u32x2 hi = read_transposed(v_rows + ((r + 8) * kCols + v_column<DP>(r + 8, c)) * 16);
-          acc[dt] = mma32<TY>(u32x4{lo[0], lo[1], hi[0], hi[1]}, __builtin_bit_cast(u32x4, w), acc[dt]);
-        }
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = mma32<TY>(vf[t][dt], __builtin_bit_cast(u32x4, w), acc[dt]);
       }
     };
     for (; kb < sk.n; kb += step, buf ^= 1) {
