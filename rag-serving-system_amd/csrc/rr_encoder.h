@@ -51,6 +51,7 @@ struct NormArgs {
   int8_t* q;
   int64_t ldq;
   float* q_scale;
+  bool past;   // (set by the launcher) results are written past the caches
 };
 hipError_t launch_block_norm(int type, const NormArgs& a, hipStream_t s);
 

@@ -195,7 +195,7 @@ int rr_block_norm(int device, void* hip_stream, int type, int64_t rows, int32_t 
     TRY(bad_rows(me, "q_scale", q_scale, 1, 1, 4));
   }
   const NormArgs a{rows, cols, y, x, gate, ldy, ldx, ldg, gate ? rows_per_gate : 1, residual_scale, eps, post_norm,
-                   next_norm, post_weight, post_bias, next_weight, next_bias, stream, normed, lds, ldn, q, ldq, q_scale};
+                   next_norm, post_weight, post_bias, next_weight, next_bias, stream, normed, lds, ldn, q, ldq, q_scale, false};
   return enqueue(me, device, [&] { return launch_block_norm(type, a, static_cast<hipStream_t>(hip_stream)); });
 }
 

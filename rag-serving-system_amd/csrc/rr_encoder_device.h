@@ -37,6 +37,13 @@ template <class V>
 __device__ __forceinline__ void store_as(void* p, V v) {
   __builtin_memcpy(p, &v, sizeof(V));
 }
+// The same past the caches (non-temporal): for results that are too many to be found there when they are read.
+template <class V>
+__device__ __forceinline__ void store_past(void* p, V v) {
+  typedef V any __attribute__((aligned(1)));
+  __builtin_nontemporal_store(v, static_cast<any*>(p));
+}
+constexpr int64_t kCacheBytes = 32 << 20;   // eight XCDs' L2 of 4 MiB
 
 // Sums and maxima over the W waves of a row, every lane gets them. `red`: LDS words, 2 W for each row of the workgroup, used
 // in turn (the first half, the second, ...): one barrier a call, since a half is written again only after a barrier that
@@ -107,13 +114,16 @@ struct Chunk {
   }
 };
 template <class E>
-__device__ __forceinline__ void store_chunk(E* p, const float* v, int left) {
+__device__ __forceinline__ void store_chunk(E* p, const float* v, int left, bool past) {
   constexpr int N = 16 / sizeof(E);
   E o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = (E)v[i];
   if (left >= N) {
-    __builtin_memcpy(p, o, 16);
+    u32x4 raw;
+    __builtin_memcpy(&raw, o, 16);
+    if (past) store_past(p, raw);
+    else store_as(p, raw);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)

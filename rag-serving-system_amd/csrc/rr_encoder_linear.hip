@@ -81,20 +81,16 @@ __device__ __forceinline__ float activate(float y, int act) {
   return act == 1 ? gelu<OT>(y) : y;
 }
 
+// Four channels of one row: sums to results.
 template <int OT>
-__device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, i32x4 c) {
+__device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, i32x4 c, float sx, const float* sw,
+                                       const float* bias) {
   using O = typename Elem<OT>::type;
-  const float sx = a.x_scale[m];
   O* out = static_cast<O*>(a.out) + m * a.ldo + n;
   typedef O o4 __attribute__((ext_vector_type(4)));
   o4 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int ni = n + i < a.n ? n + i : a.n - 1;
-    float y = (float)c[i] * (sx * a.w_scale[ni]);
-    if (a.bias) y += a.bias[ni];
-    v[i] = (O)activate<OT>(y, a.act);
-  }
+  for (int i = 0; i < 4; ++i) v[i] = (O)activate<OT>((float)c[i] * (sx * sw[i]) + bias[i], a.act);
   if (n + 4 <= a.n) {
     store_as(out, v);
   } else {
@@ -104,52 +100,57 @@ __device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, i3
   }
 }
 
-// 16 bytes of a row of `k`, zeros behind its end
+// 16 bytes of a row of `k`, zeros behind its end: there the row's last 16 bytes, moved down.
 __device__ __forceinline__ u32x4 load_row16(const int8_t* row, int at, int k) {
-  u32x4 v = {0, 0, 0, 0};
   if (at + 16 <= k) return load_as<u32x4>(row + at);
-  if (at < k) {
-    int8_t b[16];
+  if (at >= k) return u32x4{0, 0, 0, 0};
+  if (k >= 16)
+    return __builtin_bit_cast(u32x4, load_as<unsigned __int128>(row + k - 16) >> 8 * (at + 16 - k));
+  u32x4 v;
+  int8_t b[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = at + i < k ? row[at + i] : 0;
-    __builtin_memcpy(&v, b, 16);
-  }
+  for (int i = 0; i < 16; ++i) b[i] = at + i < k ? row[at + i] : 0;
+  __builtin_memcpy(&v, b, 16);
   return v;
 }
 
-// 64 x 64 tiles, 128 bytes of k a step, any size and alignment: through registers into LDS, the next step's loads in flight
-// during this one's matrix instructions.
-constexpr int kAnyStep = 128, kPad = kAnyStep + 16;   // bytes from one LDS row to the next
+// 64 x 64 tiles, any size and alignment: through registers into LDS, the next two steps' loads in flight during a step's matrix
+// instructions. Two groups of four waves take every other 128 bytes of k, since such calls have few tiles and wait for their
+// chain of steps; each group then finishes half of the tile, with scales that it asked for before the first step
+// (1031 x 1000 -> 777, GPU time: 10.3 us with one group and scales read at the end, 8.1 so).
+constexpr int kAnyStep = 128, kAnyGroups = 2, kPad = kAnyStep + 16;   // kPad: bytes from one LDS row to the next
 template <int OT>
-__global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t tiles_n, int64_t tiles) {
-  __shared__ __align__(16) int8_t lw[64 * kPad], lx[64 * kPad];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+__global__ __launch_bounds__(256 * kAnyGroups) void linear_any_kernel(LinearArgs a, int64_t tiles_n, int64_t tiles) {
+  __shared__ __align__(16) int8_t lds[kAnyGroups][2][64 * kPad];
+  const int t = threadIdx.x & 255, lane = t & 63, wave = t >> 6, group = threadIdx.x >> 8;
   const int row = t >> 2, col = (t & 3) * 16;
   const int wn = (wave & 1) * 32, wm = (wave >> 1) * 32;
+  int8_t *lw = lds[group][0], *lx = lds[group][1];
+  struct Step {
+    u32x4 w[2], x[2];
+  };
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int n0 = (int)(tile % tiles_n) * 64;
     const int64_t m0 = tile / tiles_n * 64;
     const int8_t* wr = a.w + (int64_t)(n0 + row < a.n ? n0 + row : a.n - 1) * a.ldw;
     const int8_t* xr = a.x + (m0 + row < a.m ? m0 + row : a.m - 1) * a.ldx;
-    u32x4 vw[2], vx[2];
-    auto fetch = [&](int k0) {
+    auto fetch = [&](Step& s, int k0) {   // (zeros behind k)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        vw[h] = load_row16(wr, k0 + 64 * h + col, a.k);
-        vx[h] = load_row16(xr, k0 + 64 * h + col, a.k);
+        s.w[h] = load_row16(wr, k0 + 64 * h + col, a.k);
+        s.x[h] = load_row16(xr, k0 + 64 * h + col, a.k);
       }
     };
     i32x4 acc[2][2] = {};
-    fetch(0);
-    for (int k0 = 0; k0 < a.k; k0 += kAnyStep) {
+    auto take = [&](Step& s, int next) {   // and asks for the step at `next`
       __syncthreads();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        *reinterpret_cast<u32x4*>(lw + row * kPad + 64 * h + col) = vw[h];
-        *reinterpret_cast<u32x4*>(lx + row * kPad + 64 * h + col) = vx[h];
+        *reinterpret_cast<u32x4*>(lw + row * kPad + 64 * h + col) = s.w[h];
+        *reinterpret_cast<u32x4*>(lx + row * kPad + 64 * h + col) = s.x[h];
       }
       __syncthreads();
-      if (k0 + kAnyStep < a.k) fetch(k0 + kAnyStep);
+      fetch(s, next);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         i32x4 fw[2], fx[2];
@@ -163,15 +164,41 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t t
 #pragma unroll
           for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
       }
+    };
+    constexpr int kRound = kAnyGroups * kAnyStep;   // what all groups take in a step; both go through the same steps
+    Step one, two;
+    const int first = group * kAnyStep;
+    fetch(one, first);
+    fetch(two, first + kRound);
+    // group g finishes channels 16 g .. 16 g + 15 of every wave's 32; what that takes is asked for now
+    const int n = n0 + wn + 16 * group + 4 * (lane >> 4);
+    float scale[4], bias[4], row_scales[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ni = n + i < a.n ? n + i : a.n - 1;
+      scale[i] = a.w_scale[ni];
+      bias[i] = a.bias ? a.bias[ni] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j) {
+      const int64_t m = m0 + wm + 16 * j + (lane & 15);
+      row_scales[j] = a.x_scale[m < a.m ? m : a.m - 1];
+    }
+    for (int k0 = 0; k0 < a.k; k0 += 2 * kRound) {
+      take(one, first + k0 + 2 * kRound);
+      if (k0 + kRound < a.k) take(two, first + k0 + 3 * kRound);
+    }
+    __syncthreads();
+    i32x4* other = reinterpret_cast<i32x4*>(lds[0][0]);   // [group][wave][j][lane]
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int64_t m = m0 + wm + 16 * j + (lane & 15);
-        const int n = n0 + wn + 16 * i + 4 * (lane >> 4);
-        if (m < a.m && n < a.n) store4<OT>(a, m, n, acc[i][j]);
-      }
+    for (int j = 0; j < 2; ++j) other[(((1 - group) * 4 + wave) * 2 + j) * 64 + lane] = group ? acc[0][j] : acc[1][j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const i32x4 c = (group ? acc[1][j] : acc[0][j]) + other[((group * 4 + wave) * 2 + j) * 64 + lane];
+      const int64_t m = m0 + wm + 16 * j + (lane & 15);
+      if (m < a.m && n < a.n) store4<OT>(a, m, n, c, row_scales[j], scale, bias);
+    }
   }
 }
 
@@ -219,7 +246,7 @@ struct Row8 {
 template <int OT, int R, int XT, bool SINGLE = false>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a) {
   constexpr bool kFused = XT != T_I8;
-  constexpr int kAhead = R <= 2 ? 8 : 4;   // steps of 64 bytes of weights loaded together
+  constexpr int kAhead = R == 1 ? 8 : 4;   // steps of 64 bytes, of weights and rows, loaded together
   __shared__ __align__(16) i32x4 sums[kFewWaves][R][64];
   __shared__ __align__(16) int8_t x8[kFused ? kFusedRow : 16];   // (eight rows of kFusedWave columns are as many)
   __shared__ float sc[16];
@@ -228,6 +255,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
   const int n0 = blockIdx.x * 16, kp = (a.k + 63) / 64 * 64;
   const int8_t* wr = a.w + (int64_t)(n0 + i < a.n ? n0 + i : a.n - 1) * a.ldw;
   i32x4 acc[R] = {};
+  float scale[4], bias[4];   // of the four channels that this lane finishes
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int n = n0 + 4 * g + x < a.n ? n0 + 4 * g + x : a.n - 1;
+    scale[x] = a.w_scale[n];
+    bias[x] = a.bias ? a.bias[n] : 0.f;
+  }
   Row8<kFused ? XT : T_F32, SINGLE ? kFewWaves : 1> rows;
   const int t = SINGLE ? threadIdx.x : lane, mine = SINGLE ? 0 : wave;
   if constexpr (kFused)
@@ -236,6 +270,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
     u32x4 w[kAhead];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) w[s] = load_row16(wr, k0 + s * kFewWaves * 64 + 16 * g, a.k);
+    u32x4 x[kFused ? 1 : kAhead][R];
+    if constexpr (!kFused)
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          x[s][r] = load_row16(a.x + (16 * r + i < a.m ? 16 * r + i : a.m - 1) * a.ldx, k0 + s * kFewWaves * 64 + 16 * g, a.k);
     if constexpr (kFused) {
       if (k0 == wave * 64) {   // (every wave comes here once, with or without weights to multiply)
         if (mine < a.m) rows.put(x8 + mine * kp, kp, sc + mine, t, red);
@@ -243,31 +284,29 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
       }
     }
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
-      const int at = k0 + s * kFewWaves * 64 + 16 * g;
-      if (k0 + s * kFewWaves * 64 < kp) {
+    for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          u32x4 x = {0, 0, 0, 0};
-          if (16 * r + i < a.m) {
-            if constexpr (kFused) x = *reinterpret_cast<const u32x4*>(x8 + (16 * r + i) * kp + at);
-            else x = load_row16(a.x + (16 * r + i) * a.ldx, at, a.k);
-          }
-          acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w[s]), __builtin_bit_cast(i32x4, x), acc[r], 0, 0, 0);
+      for (int r = 0; r < R; ++r) {
+        u32x4 v;
+        if constexpr (kFused) {
+          const int at = k0 + s * kFewWaves * 64 + 16 * g;
+          v = u32x4{0, 0, 0, 0};
+          if (i < a.m && at < kp) v = *reinterpret_cast<const u32x4*>(x8 + i * kp + at);
+        } else {
+          v = x[s][r];
         }
+        acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w[s]), __builtin_bit_cast(i32x4, v), acc[r], 0, 0, 0);
       }
-    }
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) sums[wave][r][lane] = acc[r];
   __syncthreads();
-  if constexpr (kFused) a.x_scale = sc;
   for (int r = wave; r < R; r += kFewWaves) {
     i32x4 c = sums[0][r][lane];
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) c += sums[w][r][lane];
     const int m = 16 * r + i, n = n0 + 4 * g;
-    if (m < a.m && n < a.n) store4<OT>(a, m, n, c);
+    if (m < a.m && n < a.n) store4<OT>(a, m, n, c, kFused ? sc[m] : a.x_scale[m], scale, bias);
   }
 }
 
@@ -485,7 +524,7 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
     return tiled<OT, ACT, 64, 64, 2, 2, 128, 3>(a, s);
   }
   const int64_t tiles = tiles_of(64);
-  linear_any_kernel<OT><<<grid_of(tiles), 256, 0, s>>>(a, (a.n + 63) / 64, tiles);
+  linear_any_kernel<OT><<<grid_of(tiles), 256 * kAnyGroups, 0, s>>>(a, (a.n + 63) / 64, tiles);
   return hipGetLastError();
 }
 template <int OT, int XT>
@@ -507,8 +546,8 @@ hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
 }
 
 // One launch instead of two, as long as every workgroup's own conversion costs less than the second launch (bf16, GPU time
-// alone): one row 4096 -> 1024 4.7 us against 7.9, eight rows 1024 -> 4096 4.9 against 6.5; but sixteen rows, two a wave, 7.6
-// against 6.6 and two rows of 4096 8.9 against 7.9.
+// alone): one row 4096 -> 1024 4.5 us against 7.1, eight rows 1024 -> 4096 4.8 against 6.2; but sixteen rows, two a wave, 7.6
+// against 6.3 and two rows of 4096 8.9 against 7.2.
 bool linear_fuses_rows(int64_t m, int k) { return k <= (m == 1 ? kFusedRow : kFusedWave) && m <= kFewWaves; }
 
 hipError_t launch_linear_fused(int x_type, const LinearArgs& a, hipStream_t s) {

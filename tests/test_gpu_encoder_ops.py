@@ -118,6 +118,24 @@ def test_linear_int8_many_tiles(ops, out, m, n, k):
         assert ((got.double().cpu() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("k", [1, 15, 17, 127, 129, 250, 257, 300, 385, 399, 513, 600, 650, 777, 1027, 1300, 2049])
+def test_linear_int8_inner_sizes(ops, k):
+    """Inner sizes that end anywhere in a step, rows at any byte."""
+    g = gen(k)
+    for m, n in ((70, 65), (3, 20)):
+        q = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+        w, sw, _ = weights(g, n, k)
+        sx = 0.01 + torch.rand(m, generator=g)
+        got = ops.linear_int8(q.cuda(), w.cuda(), sw.cuda(), x_scale=sx.cuda())
+        want, tol = plain.linear(q, sx, w, sw, None, "none", torch.float32)
+        assert ((got.double().cpu() - want).abs() <= tol).all()
+        x = rand(g, m, k).to(torch.bfloat16)
+        got = ops.linear_int8(x.cuda(), w.cuda(), sw.cuda())
+        q8, s8 = plain.rows8(x)
+        want, tol = plain.linear(q8, s8, w, sw, None, "none", torch.bfloat16)
+        assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_linear_int8_extremes(ops, m):
     """The longest inner size with every product at its largest: the 32-bit sum must still be exact. -128 is a valid value."""
