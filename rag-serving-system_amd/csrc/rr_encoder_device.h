@@ -131,11 +131,12 @@ __device__ __forceinline__ void store_chunk(E* p, const float* v, int left, bool
   }
 }
 
-// The 8-bit row rule. The row's largest magnitude travels as its bit pattern: patterns of |x| order as their values do,
+// The 8-bit row rule: scale = max|x| times the fp32 neighbour of 1/127 (one multiplication: a row's scale is then the same
+// wherever it is made, also by code that divides by 127 through its reciprocal). The row's largest magnitude travels as its bit pattern: patterns of |x| order as their values do,
 // infinities above every finite value and NaNs above those.
 __device__ __forceinline__ unsigned mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ float row_scale(unsigned m) {
-  return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(m) / 127.0f;
+  return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(m) * (1.0f / 127.0f);
 }
 // the divisor that goes with it: rows of zeros, of non-finite values and of a scale that underflows give q = 0
 __device__ __forceinline__ float row_divisor(float scale) { return scale > 0.f ? scale : __uint_as_float(0x7f800000u); }

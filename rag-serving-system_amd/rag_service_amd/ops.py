@@ -44,7 +44,7 @@ def _load():
 
 def quantize_rows(x):
     """8-bit rows of x (..., cols): int8 values of the same shape and fp32 scales (...), with
-    scale = max|row| / 127 and value = rint(x / scale). A row that holds a NaN or an infinity gets scale NaN and zeros."""
+    scale = max|row| * (1 / 127) and value = rint(x / scale), all in fp32. A row that holds a NaN or an infinity gets scale NaN and zeros."""
     r = (_native or _load()).quantize_rows(x)
     if type(r) is int:
         _check(r)

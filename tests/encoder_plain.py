@@ -13,11 +13,12 @@ TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 
 
 
 def rows8(x):
-    """(q, scale) of fp32 rows: both quotients are IEEE fp32 divisions, so these are the operator's values bit for bit."""
+    """(q, scale) of fp32 rows: an fp32 product with the neighbour of 1/127 and an IEEE fp32 quotient, so these are the
+    operator's values bit for bit."""
     x = x.float().cpu()
     amax = x.abs().amax(dim=-1)
     bad = ~torch.isfinite(x).all(dim=-1)
-    scale = (amax / torch.tensor(127.0)).masked_fill(bad, float("nan"))
+    scale = (amax * torch.tensor(1 / 127, dtype=torch.float32)).masked_fill(bad, float("nan"))
     div = torch.where(scale > 0, scale, torch.tensor(float("inf")))
     q = torch.clamp(torch.round(x / div[..., None]), -127, 127)
     q = torch.where(bad[..., None], torch.zeros(()), q)
