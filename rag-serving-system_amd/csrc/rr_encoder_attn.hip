@@ -143,10 +143,13 @@ struct Core16 {
   }
   // valid: bit j says whether key j of this lane takes part; the V rows of the others may hold anything and become zeros
   static __device__ __forceinline__ void accumulate(Keys& of, const float* p, unsigned valid, f32x4* acc) {
-    e8 pe;
+    e8 pe, rest;   // the weights to twice the type's precision, as kFewRows' kernel takes them
 #pragma unroll
-    for (int j = 0; j < 8; ++j) pe[j] = (E)p[j];
-    const u32x4 pb = __builtin_bit_cast(u32x4, pe);
+    for (int j = 0; j < 8; ++j) {
+      pe[j] = (E)p[j];
+      rest[j] = (E)(p[j] - (float)pe[j]);
+    }
+    const u32x4 pb = __builtin_bit_cast(u32x4, pe), pr = __builtin_bit_cast(u32x4, rest);
     if (valid != 0xffu) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -161,8 +164,8 @@ struct Core16 {
         lo[x] = __builtin_amdgcn_perm(of.v[2 * x + 1][w], of.v[2 * x][w], 0x05040100u);
         hi[x] = __builtin_amdgcn_perm(of.v[2 * x + 1][w], of.v[2 * x][w], 0x07060302u);
       }
-      acc[2 * w] = mma(lo, pb, acc[2 * w]);
-      acc[2 * w + 1] = mma(hi, pb, acc[2 * w + 1]);
+      acc[2 * w] = mma(lo, pr, mma(lo, pb, acc[2 * w]));
+      acc[2 * w + 1] = mma(hi, pr, mma(hi, pb, acc[2 * w + 1]));
     }
   }
 };
@@ -390,7 +393,8 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
 // Keys that do not take part are read as zeros, whatever they held. Lane (i = lane % 32, half = lane / 32) holds the scores
 // of query i with keys 8 (r / 4) + 4 half + r % 4 of a 32-key block, r < 16; eight of them in a row (r / 8 = t) are its slots
 // of the second product's 16-key contraction t. V lies in LDS as in memory; the transposing LDS read hands each lane four keys
-// of one dimension.
+// of one dimension. The weights enter the second product rounded to the type, which is off by as much as the result's own
+// rounding; few rows, which wait for memory and not for arithmetic, add what the rounding left in a product of its own.
 // DMA: rows at 16-byte addresses go to LDS by the loads themselves; others through registers.
 constexpr int kTileRows = 128, kFewRows = 32;
 
@@ -573,15 +577,19 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        e8 w;
+        e8 w, rest;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const float e = exp2_fast(fmaf(s[8 * t + x], p.c, -ref));
           l += e;
           w[x] = (E)e;
+          if constexpr (WK > 1) rest[x] = (E)(e - (float)w[x]);
         }
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = mma32<TY>(vf[t][dt], __builtin_bit_cast(u32x4, w), acc[dt]);
+        for (int dt = 0; dt < DP / 32; ++dt) {
+          acc[dt] = mma32<TY>(vf[t][dt], __builtin_bit_cast(u32x4, w), acc[dt]);
+          if constexpr (WK > 1) acc[dt] = mma32<TY>(vf[t][dt], __builtin_bit_cast(u32x4, rest), acc[dt]);
+        }
       }
     };
     for (; kb < sk.n; kb += step, buf ^= 1) {
