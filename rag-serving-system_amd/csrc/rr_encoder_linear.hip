@@ -319,8 +319,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
 // of the buffer's range and read as zeros.
 template <int STEP>
 __device__ __forceinline__ int swizzle(int r) {
-  static_assert(STEP == 128 || STEP == 64, "a row's share of the 256-byte bank cycle");
-  return STEP == 128 ? r / 2 % 8 : r / 4 % 4;
+  static_assert(STEP == 256 || STEP == 128 || STEP == 64, "a row's share of the 256-byte bank cycle");
+  return STEP == 256 ? r % 16 : STEP == 128 ? r / 2 % 8 : r / 4 % 4;
 }
 
 __device__ __forceinline__ i32x4 buffer_of(const void* p, unsigned bytes) {
@@ -397,6 +397,12 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
   };
   i32x16 acc[kN][kM] = {};
   const int row = lane % 32, half = lane / 32, swz = swizzle<STEP>(row);
+  float sx[kM];
+#pragma unroll
+  for (int j = 0; j < kM; ++j) {
+    const int64_t m = m0 + (wm * kM + j) * 32 + row;
+    sx[j] = a.x_scale[m < a.m ? m : a.m - 1];
+  }
   const int steps = (a.k + STEP - 1) / STEP;
 #pragma unroll
   for (int s = 0; s < BUFS - 1; ++s)
@@ -428,8 +434,6 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
   char* out = lds + wave * 32 * kOutLd;
 #pragma unroll
   for (int j = 0; j < kM; ++j) {
-    const int64_t m = m0 + (wm * kM + j) * 32 + row;
-    const float sx = a.x_scale[m < a.m ? m : a.m - 1];
 #pragma unroll
     for (int i = 0; i < kN; ++i)
 #pragma unroll
@@ -440,7 +444,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
         typedef O o4 __attribute__((ext_vector_type(4)));
         o4 v;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = (O)activate<OT>((float)acc[i][j][4 * g + x] * (sx * sw[x]) + bias[x], ACT);
+        for (int x = 0; x < 4; ++x) v[x] = (O)activate<OT>((float)acc[i][j][4 * g + x] * (sx[j] * sw[x]) + bias[x], ACT);
         *reinterpret_cast<o4*>(out + row * kOutLd + nl * sizeof(O)) = v;
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wave's own LDS: no barrier)
@@ -508,7 +512,7 @@ hipError_t tiled(const LinearArgs& a, hipStream_t s) {
 }
 template <int OT, int ACT>
 hipError_t linear(const LinearArgs& a, hipStream_t s) {
-  auto tiles_of = [&](int64_t t) { return ((a.n + t - 1) / t) * ((a.m + t - 1) / t); };
+  auto tiles_of = [&](int64_t tn, int64_t tm) { return ((a.n + tn - 1) / tn) * ((a.m + tm - 1) / tm); };
   if (a.m <= kFewRows) {
     const dim3 grid((a.n + 15) / 16);
     if (a.m <= 16) linear_few_kernel<OT, 1, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
@@ -518,12 +522,20 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
   }
   const bool rows16 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw | a.k) & 15) == 0 &&
                       a.ldx < (1 << 22) && a.ldw < (1 << 22);
-  if (rows16 && tiles_of(64) < (1 << 22)) {
-    if (tiles_of(256) >= 192) return tiled<OT, ACT, 256, 256, 2, 4, 128, 2>(a, s);
-    if (tiles_of(128) >= 224) return tiled<OT, ACT, 128, 128, 2, 2, 128, 2>(a, s);
+  // The largest tile that still gives the 256 CUs one each, or nearly (int8 rows, GPU time; channels x rows, waves, buffers):
+  //   16384 x 4096 -> 1024   256 x 256  70 us    128 x 128  85    64 x 64  125
+  //    4096 x 4096 -> 1024   128 x 128, four buffers 24, two 27;  64 x 64  32
+  //    2048 x 1024 -> 4096   128 x 128, four buffers 19, two 15;  64 x 64  22   (two tiles a CU: they fill each other's waits)
+  //     613 x 1024 -> 4096   64 x 128  9.0         128 x 128  9.5  64 x 64  10.0
+  //     613 x 4096 -> 1024   64 x 64  11.5         128 x 128 19
+  if (rows16 && tiles_of(64, 64) < (1 << 22)) {
+    if (tiles_of(256, 256) >= 192) return tiled<OT, ACT, 256, 256, 2, 4, 128, 2>(a, s);
+    if (tiles_of(128, 128) > 256) return tiled<OT, ACT, 128, 128, 2, 4, 128, 2>(a, s);
+    if (tiles_of(128, 128) >= 224) return tiled<OT, ACT, 128, 128, 2, 4, 128, 4>(a, s);
+    if (tiles_of(64, 128) >= 256) return tiled<OT, ACT, 64, 128, 2, 4, 128, 3>(a, s);
     return tiled<OT, ACT, 64, 64, 2, 2, 128, 3>(a, s);
   }
-  const int64_t tiles = tiles_of(64);
+  const int64_t tiles = tiles_of(64, 64);
   linear_any_kernel<OT><<<grid_of(tiles), 256 * kAnyGroups, 0, s>>>(a, (a.n + 63) / 64, tiles);
   return hipGetLastError();
 }

@@ -104,7 +104,8 @@ def test_linear_int8_rows(ops, out, m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1500, 1100, 144), (1300, 1290, 16), (1290, 1281, 1040), (1411, 1024, 272), (3600, 3400, 208),
-                                   (3585, 3333, 128), (4000, 3700, 32), (2600, 5000, 656)])
+                                   (3585, 3333, 128), (4000, 3700, 32), (2600, 5000, 656), (2000, 1900, 144), (1000, 2300, 400),
+                                   (1900, 2000, 16)])
 @pytest.mark.parametrize("out", TYPES, ids=str)
 def test_linear_int8_many_tiles(ops, out, m, n, k):
     """Sizes of many tiles whose last rows, channels and inner columns fill none."""
