@@ -23,6 +23,10 @@ struct DeviceScope {
     err = hipGetDevice(&before);
     if (err == hipSuccess && before != device) err = hipSetDevice(device);
     else if (err == hipSuccess) before = -1;
+    if (err != hipSuccess) {
+      before = -1;
+      (void)hipGetLastError();   // (reported here: the next launch's check is not to find it)
+    }
   }
   ~DeviceScope() {
     if (before >= 0) (void)hipSetDevice(before);

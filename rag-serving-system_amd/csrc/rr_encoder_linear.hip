@@ -7,7 +7,8 @@ namespace {
 
 // ---- 8-bit rows ----------------------------------------------------------------------------------------------------
 // A row in the registers of W waves, S times 16 bytes a lane; W = 1: four rows a workgroup. cols_pad: columns written, zeros
-// behind the row's own.
+// behind the row's own. Bandwidth: 16384 x 4096 bf16 46 us, 4.4 TB/s (of 5.2 that a large copy reaches; a wave a row instead of
+// four changes nothing).
 template <int TY, int W, int S>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_rows_kernel(const void* xv, int64_t ldx, int64_t rows,
                                                                              int cols, int cols_pad, int8_t* q, int64_t ldq,
@@ -207,6 +208,8 @@ __global__ __launch_bounds__(256 * kAnyGroups) void linear_any_kernel(LinearArgs
 // 64 bytes of k, straight from memory into the matrix instruction's operands, and their integer sums, exact in any order, meet
 // in LDS. FUSED: x is floating point and every workgroup makes its own 8-bit rows in LDS while its first weights arrive: one
 // launch, where a short row would wait for two.
+// One row 4096 -> 1024 4.3 us (its 4 MiB of weights would take 0.8 at copy speed: the rest is a launch and three memory
+// latencies in a row), 16 rows 5.6; 1024 -> 4096 3.4 and 3.6.
 constexpr int kFewWaves = 8, kFewRows = 48;
 constexpr int kFusedRow = 8192;    // columns of a single row that every workgroup converts for itself, all waves at it,
 constexpr int kFusedWave = 1024;   // and of up to eight rows, a wave each
@@ -311,17 +314,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
 }
 
 // ---- the tiled product -----------------------------------------------------------------------------------------------
-// Workgroup tile: TN channels x TM rows, STEP bytes of k a step, both operands brought into LDS by the loads' LDS form (no
+// Workgroup tile: TN channels x TM rows, 128 bytes of k a step, both operands brought into LDS by the loads' LDS form (no
 // registers, no ds_write) into BUFS buffers in turn: BUFS - 1 steps are in flight while one is multiplied, one barrier a step.
 // Waves: WN x WM, each (TN / WN) x (TM / WM) in 32 x 32 x 32 instructions. LDS rows hold a step; the 16-byte column c of row r
 // lies at column c ^ swizzle(r), so that the 16 lanes that read a column of 16 rows at once meet all 64 banks.
 // Wants rows at 16-byte addresses and k a multiple of 16 (the loads' unit); columns behind k and rows behind the end are out
 // of the buffer's range and read as zeros.
-template <int STEP>
-__device__ __forceinline__ int swizzle(int r) {
-  static_assert(STEP == 256 || STEP == 128 || STEP == 64, "a row's share of the 256-byte bank cycle");
-  return STEP == 256 ? r % 16 : STEP == 128 ? r / 2 % 8 : r / 4 % 4;
-}
+// 16384 x 4096 -> 1024 (int8 rows, bf16 results) in 256 x 256 tiles: 70 us, 1.95 POP/s (the library's i8 product of these
+// sizes takes 75). A step's 2048 cycles of matrix instructions need as many of LDS (192 KiB of reads, 64 KiB of arriving
+// rows); tried and dropped: four waves of 128 x 128 (fewer LDS reads, 87 us), 64-byte steps in four buffers (87), operands
+// read one part ahead with the barrier inside the step (78). A quarter of the tiles on a quarter of the CUs take 51 us, so
+// the rest is the whole chip's clock under matrix load.
+constexpr int kStep = 128, kCols = kStep / 16;
+__device__ __forceinline__ int swizzle(int r) { return r / 2 % 8; }   // (two rows fill the banks once)
 
 __device__ __forceinline__ i32x4 buffer_of(const void* p, unsigned bytes) {
   const uint64_t at = (uint64_t)p;
@@ -344,10 +349,10 @@ __device__ __forceinline__ void step_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
-template <int OT, int ACT, int TN, int TM, int WN, int WM, int STEP, int BUFS>
+template <int OT, int ACT, int TN, int TM, int WN, int WM, int BUFS>
 __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs a, int tiles_n, int64_t tiles) {
-  constexpr int kWaves = WN * WM, kN = TN / WN / 32, kM = TM / WM / 32, kCols = STEP / 16;
-  constexpr int kBuf = (TN + TM) * STEP, kLoadsN = TN * STEP / (1024 * kWaves), kLoadsM = TM * STEP / (1024 * kWaves);
+  constexpr int kWaves = WN * WM, kN = TN / WN / 32, kM = TM / WM / 32;
+  constexpr int kBuf = (TN + TM) * kStep, kLoadsN = TN * kStep / (1024 * kWaves), kLoadsM = TM * kStep / (1024 * kWaves);
   using O = typename Elem<OT>::type;
   constexpr int kOutLd = kN * 32 * sizeof(O) + 16;   // bytes of an output row in LDS
   constexpr int kLds = BUFS * kBuf > kWaves * 32 * kOutLd ? BUFS * kBuf : kWaves * 32 * kOutLd;
@@ -377,13 +382,13 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
 #pragma unroll
   for (int j = 0; j < kLoadsN; ++j) {
     const int r = 64 / kCols * (j * kWaves + wave) + lane / kCols;
-    col_w[j] = 16 * (lane % kCols ^ swizzle<STEP>(r));
+    col_w[j] = 16 * (lane % kCols ^ swizzle(r));
     from_w[j] = (unsigned)(r * a.ldw + col_w[j]);
   }
 #pragma unroll
   for (int j = 0; j < kLoadsM; ++j) {
     const int r = 64 / kCols * (j * kWaves + wave) + lane / kCols;
-    col_x[j] = 16 * (lane % kCols ^ swizzle<STEP>(r));
+    col_x[j] = 16 * (lane % kCols ^ swizzle(r));
     from_x[j] = (unsigned)(r * a.ldx + col_x[j]);
   }
   auto fetch = [&](int k0, int buf) {
@@ -393,35 +398,35 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
       load_to_lds(bw, k0 + col_w[j] < a.k ? from_w[j] + k0 : ~15u, to + j * kWaves * 1024);
 #pragma unroll
     for (int j = 0; j < kLoadsM; ++j)
-      load_to_lds(bx, k0 + col_x[j] < a.k ? from_x[j] + k0 : ~15u, to + TN * STEP + j * kWaves * 1024);
+      load_to_lds(bx, k0 + col_x[j] < a.k ? from_x[j] + k0 : ~15u, to + TN * kStep + j * kWaves * 1024);
   };
   i32x16 acc[kN][kM] = {};
-  const int row = lane % 32, half = lane / 32, swz = swizzle<STEP>(row);
+  const int row = lane % 32, half = lane / 32, swz = swizzle(row);
   float sx[kM];
 #pragma unroll
   for (int j = 0; j < kM; ++j) {
     const int64_t m = m0 + (wm * kM + j) * 32 + row;
     sx[j] = a.x_scale[m < a.m ? m : a.m - 1];
   }
-  const int steps = (a.k + STEP - 1) / STEP;
+  const int steps = (a.k + kStep - 1) / kStep;
 #pragma unroll
   for (int s = 0; s < BUFS - 1; ++s)
-    if (s < steps) fetch(s * STEP, s);
+    if (s < steps) fetch(s * kStep, s);
   int buf = 0, next = BUFS - 1;
   for (int s = 0; s < steps; ++s) {
     if (s + BUFS - 2 < steps) step_barrier<(BUFS - 2) * (kLoadsN + kLoadsM)>();
     else step_barrier<0>();
-    if (s + BUFS - 1 < steps) fetch((s + BUFS - 1) * STEP, next);   // (its buffer was last read before this barrier)
-    const char* lw = lds + buf * kBuf + (wn * kN * 32 + row) * STEP;
-    const char* lx = lds + buf * kBuf + TN * STEP + (wm * kM * 32 + row) * STEP;
+    if (s + BUFS - 1 < steps) fetch((s + BUFS - 1) * kStep, next);   // (its buffer was last read before this barrier)
+    const char* lw = lds + buf * kBuf + (wn * kN * 32 + row) * kStep;
+    const char* lx = lds + buf * kBuf + TN * kStep + (wm * kM * 32 + row) * kStep;
 #pragma unroll
-    for (int kk = 0; kk < STEP / 32; ++kk) {
+    for (int kk = 0; kk < kStep / 32; ++kk) {
       const int c = 16 * ((2 * kk + half) ^ swz);
       i32x4 fw[kN], fx[kM];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) fw[i] = *reinterpret_cast<const i32x4*>(lw + i * 32 * STEP + c);
+      for (int i = 0; i < kN; ++i) fw[i] = *reinterpret_cast<const i32x4*>(lw + i * 32 * kStep + c);
 #pragma unroll
-      for (int j = 0; j < kM; ++j) fx[j] = *reinterpret_cast<const i32x4*>(lx + j * 32 * STEP + c);
+      for (int j = 0; j < kM; ++j) fx[j] = *reinterpret_cast<const i32x4*>(lx + j * 32 * kStep + c);
 #pragma unroll
       for (int i = 0; i < kN; ++i)
 #pragma unroll
@@ -503,11 +508,11 @@ hipError_t launch_quantize_rows(int type, const void* x, int64_t ldx, int64_t ro
 }
 
 namespace {
-template <int OT, int ACT, int TN, int TM, int WN, int WM, int STEP, int BUFS>
+template <int OT, int ACT, int TN, int TM, int WN, int WM, int BUFS>
 hipError_t tiled(const LinearArgs& a, hipStream_t s) {
   const int tiles_n = (a.n + TN - 1) / TN;
   const int64_t tiles = (int64_t)tiles_n * ((a.m + TM - 1) / TM);
-  linear_tile_kernel<OT, ACT, TN, TM, WN, WM, STEP, BUFS><<<dim3((unsigned)tiles), 64 * WN * WM, 0, s>>>(a, tiles_n, tiles);
+  linear_tile_kernel<OT, ACT, TN, TM, WN, WM, BUFS><<<dim3((unsigned)tiles), 64 * WN * WM, 0, s>>>(a, tiles_n, tiles);
   return hipGetLastError();
 }
 template <int OT, int ACT>
@@ -529,11 +534,11 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
   //     613 x 1024 -> 4096   64 x 128  9.0         128 x 128  9.5  64 x 64  10.0
   //     613 x 4096 -> 1024   64 x 64  11.5         128 x 128 19
   if (rows16 && tiles_of(64, 64) < (1 << 22)) {
-    if (tiles_of(256, 256) >= 192) return tiled<OT, ACT, 256, 256, 2, 4, 128, 2>(a, s);
-    if (tiles_of(128, 128) > 256) return tiled<OT, ACT, 128, 128, 2, 4, 128, 2>(a, s);
-    if (tiles_of(128, 128) >= 224) return tiled<OT, ACT, 128, 128, 2, 4, 128, 4>(a, s);
-    if (tiles_of(64, 128) >= 256) return tiled<OT, ACT, 64, 128, 2, 4, 128, 3>(a, s);
-    return tiled<OT, ACT, 64, 64, 2, 2, 128, 3>(a, s);
+    if (tiles_of(256, 256) >= 192) return tiled<OT, ACT, 256, 256, 2, 4, 2>(a, s);
+    if (tiles_of(128, 128) > 256) return tiled<OT, ACT, 128, 128, 2, 4, 2>(a, s);
+    if (tiles_of(128, 128) >= 224) return tiled<OT, ACT, 128, 128, 2, 4, 4>(a, s);
+    if (tiles_of(64, 128) >= 256) return tiled<OT, ACT, 64, 128, 2, 4, 3>(a, s);
+    return tiled<OT, ACT, 64, 64, 2, 2, 3>(a, s);
   }
   const int64_t tiles = tiles_of(64, 64);
   linear_any_kernel<OT><<<grid_of(tiles), 256 * kAnyGroups, 0, s>>>(a, (a.n + 63) / 64, tiles);

@@ -542,3 +542,128 @@ def test_layer_on_two_streams(ops):
     for j in range(2):
         for y in got[j]:
             assert torch.equal(y, want[j])
+
+
+def test_everything_in_a_graph_first(ops):
+    """Each kernel family captured, also the widest norm (dynamic LDS) and attention in pieces, and replayed on new inputs."""
+    g = gen(14)
+    x1, x2 = (rand(g, 40, 20000).to(torch.bfloat16).cuda() for _ in range(2))
+    w = torch.randint(-127, 128, (48, 20000), generator=g, dtype=torch.int8).cuda()
+    sw = torch.rand(48, generator=g).cuda() / 1000
+    q = rand(g, 2, 3, 4, 64).to(torch.bfloat16).cuda()
+    kv1, kv2 = (rand(g, 2, 5000, 4, 64).to(torch.bfloat16).cuda() for _ in range(2))
+
+    def run(x, kv):
+        n = ops.block_norm(x, x, next_norm="rms", rows8=True)
+        return (n.stream, n.normed, n.rows8, n.scale, ops.linear_int8(x, w, sw), ops.linear_int8(x[:1, :4096], w[:, :4096], sw),
+                ops.cross_attention(q, kv, kv), ops.cross_attention(q.float(), kv.float(), kv.float()))
+
+    want = [run(x1, kv1), run(x2, kv2)]
+    a, b = x1.clone(), kv1.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(a, b)
+    for i in (1, 0, 1):
+        a.copy_((x1, x2)[i])
+        b.copy_((kv1, kv2)[i])
+        graph.replay()
+        again = run(a, b)
+        torch.cuda.synchronize()
+        for y, z, v in zip(got, again, want[i]):
+            assert torch.equal(y, v) and torch.equal(z, v)
+
+
+# ---- the C-ABI itself -----------------------------------------------------------------------------------------------
+
+def test_abi_leaves_other_rows_alone_and_works_in_place(ops):
+    """Caller-owned results: packed rows that no sequence holds and columns behind a row are left as they were; a norm may
+    write its stream and its normed rows over its inputs; the thread's device and stream are its own."""
+    from rag_service_amd import _lib
+    lib, g = _lib.load_library(), gen(17)
+    stream = torch.cuda.current_stream().cuda_stream
+    qo, ko = torch.tensor([3, 10, 40], dtype=torch.int32).cuda(), torch.tensor([0, 5, 90], dtype=torch.int32).cuda()
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)):
+        q, k, v = (rand(g, n, 2, 64).to(dtype).cuda() for n in (50, 90, 90))
+        out = torch.full((50, 2, 72), 7.0, dtype=dtype, device="cuda")
+        for max_q in (30, 60):
+            need = lib.rr_cross_attention_workspace(code, 2, 2, 2, 64, max_q, 85)
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+            rc = lib.rr_cross_attention(0, stream, code, q.data_ptr(), 0, 128, 64, k.data_ptr(), 0, 128, 64, v.data_ptr(), 0, 128,
+                                        64, out.data_ptr(), 0, 144, 72, 2, 2, 2, 64, max_q, 85, 50, 90, qo.data_ptr(),
+                                        ko.data_ptr(), None, None, 0, 0.125, ws.data_ptr(), need)
+            assert rc == 0, lib.rr_last_error()
+            assert (out[:3] == 7).all() and (out[40:] == 7).all() and (out[..., 64:] == 7).all()
+            want = ops.cross_attention(q, k, v, q_offsets=qo, k_offsets=ko, max_q=max_q, max_k=85, scale=0.125)
+            assert torch.equal(out[3:40, :, :64], want[3:40])
+        x, y = rand(g, 6, 200).to(dtype).cuda(), rand(g, 6, 200).to(dtype).cuda()
+        r = ops.block_norm(y, x, residual_scale=0.5, post_norm="rms")
+        a, b = x.clone(), y.clone()
+        rc = lib.rr_block_norm(0, stream, code, 6, 200, b.data_ptr(), 200, a.data_ptr(), 200, 0.5, None, 0, 0, 1, 2, None, None,
+                               1, None, None, 1e-5, a.data_ptr(), 200, b.data_ptr(), 200, None, 0, None)
+        assert rc == 0, lib.rr_last_error()
+        assert torch.equal(a, r.stream) and torch.equal(b, r.normed)
+        wide = torch.full((6, 300), 3, dtype=torch.int8, device="cuda")
+        scale = torch.empty(6, device="cuda")
+        assert lib.rr_quantize_rows(0, stream, code, x.data_ptr(), 200, 6, 200, wide.data_ptr(), 300, scale.data_ptr()) == 0
+        q8, s8 = ops.quantize_rows(x)
+        assert torch.equal(wide[:, :200], q8) and torch.equal(scale, s8) and (wide[:, 200:] == 3).all()
+    for m, n, k in ((2, 70, 64), (70, 70, 64), (70, 70, 65), (700, 1500, 64), (3600, 3400, 32)):
+        q8 = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int8).cuda()
+        w, sw, _ = (t.cuda() for t in weights(g, n, k))
+        sx = torch.rand(m, generator=g).cuda()
+        out = torch.full((m, n + 9), 5.0, dtype=torch.bfloat16, device="cuda")
+        assert lib.rr_linear_i8(0, stream, 3, q8.data_ptr(), k, sx.data_ptr(), w.data_ptr(), k, sw.data_ptr(), None, 0, 1,
+                                out.data_ptr(), n + 9, m, n, k, None, 0) == 0
+        assert torch.equal(out[:, :n], ops.linear_int8(q8, w, sw, x_scale=sx, out_dtype=torch.bfloat16)) and (out[:, n:] == 5).all()
+    with pytest.raises(Exception, match="device"):
+        _lib._check(lib.rr_quantize_rows(99, None, 0, q.data_ptr(), 200, 6, 200, wide.data_ptr(), 300, scale.data_ptr()))
+    assert torch.cuda.current_device() == 0
+
+
+# ---- beyond 32 bits -------------------------------------------------------------------------------------------------
+
+def test_linear_and_norm_beyond_32_bit_offsets(ops):
+    """More than 2^32 bytes and 2^31 elements of rows and results: the last rows are as right as the first."""
+    g = gen(15)
+    m, k, n = 2_200_000, 1024, 1024
+    q = torch.zeros(m, k, dtype=torch.int8, device="cuda")
+    rows = torch.tensor([0, 1, 5000, m // 2, m - 2, m - 1])
+    some = torch.randint(-127, 128, (len(rows), k), generator=g, dtype=torch.int8)
+    q[rows.cuda()] = some.cuda()
+    sx = torch.full((m,), 0.01, device="cuda")
+    w, sw, b = weights(g, n, k)
+    y = ops.linear_int8(q, w.cuda(), sw.cuda(), x_scale=sx, bias=b.cuda(), out_dtype=torch.bfloat16)
+    want, tol = plain.linear(some, torch.full((len(rows),), 0.01), w, sw, b, "none", torch.bfloat16)
+    assert ((y[rows.cuda()].double().cpu() - want).abs() <= tol).all()
+    assert torch.equal(y[2:4000], b.to(torch.bfloat16).cuda().expand(3998, -1))
+    r = ops.block_norm(y, y, rows8=True)
+    for at in (slice(0, 3), slice(m - 3, m)):
+        ref = plain.block_norm(y[at], y[at], 1.0, None, 1, "none", None, None, "layer", None, None, 1e-5)
+        plain.within(r.stream[at], *ref["stream"], torch.bfloat16)
+        plain.within(r.normed[at], *ref["normed"], torch.bfloat16)
+        few = ops.block_norm(y[at], y[at], rows8=True)     # a row's result does not depend on the others
+        assert torch.equal(r.rows8[at], few.rows8) and torch.equal(r.scale[at], few.scale)
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_attention_beyond_32_bit_offsets(ops, lq):
+    """A sequence whose keys fill more than 2^32 bytes; the weight lies on its last keys."""
+    g = gen(16)
+    lk, h, d = 1_100_000, 16, 128
+    k = torch.zeros(1, lk, h, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros(1, lk, h, d, dtype=torch.bfloat16, device="cuda")
+    q = rand(g, 1, lq, h, d).to(torch.bfloat16)
+    tail_k, tail_v = rand(g, 1, 50, h, d).to(torch.bfloat16), rand(g, 1, 50, h, d).to(torch.bfloat16)
+    k[:, -50:], v[:, -50:] = (4 * tail_k).cuda(), tail_v.cuda()
+    got = ops.cross_attention(q.cuda(), k, v)
+    kk = torch.cat([torch.zeros(1, 1, h, d, dtype=torch.bfloat16), 4 * tail_k], 1).double()
+    s = (q.double().transpose(1, 2) @ kk.permute(0, 2, 3, 1)) * d ** -0.5                # (1, h, lq, 51)
+    w = torch.exp(s - s.amax(-1, keepdim=True))
+    w[..., 0] *= lk - 50                                                                # the zero keys, all alike
+    want = ((w[..., 1:] / w.sum(-1, keepdim=True)) @ tail_v.double().transpose(1, 2)).transpose(1, 2)
+    # a weight is rounded to 16 bits (2^-8), a score is off by 132 U of sum |q k| d ** -0.5 <= 4 |q| |k| d ** -0.5 < 400, and
+    # the sum of a million weights of 32 lanes or waves in turn by lk / 128 of its last places: below 2^-8 + 4e-3 + 6e-4
+    size = ((w[..., 1:] / w.sum(-1, keepdim=True)) @ tail_v.double().abs().transpose(1, 2)).transpose(1, 2)
+    tol = (2.0 ** -8 + 4e-3 + 6e-4) * 2 * size + 2.0 ** -8 * want.abs() + 2.0 ** -133
+    assert ((got.double().cpu() - want).abs() <= tol).all()
