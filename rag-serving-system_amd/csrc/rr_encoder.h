@@ -33,6 +33,11 @@ struct LinearArgs {
   int m, n, k;
 };
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
+// Inner sizes that are no multiple of 16, many products: x8 (null: it is padded already) and w copied to rows of k rounded up
+// to 16, zeros behind k.
+bool linear_repacks(int64_t m, int n, int k);
+hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const int8_t* w, int64_t ldw, int n, int8_t* to_w,
+                         int k, hipStream_t s);
 // Few short floating-point rows: one launch makes their 8-bit rows too (x holds the floating-point rows, x_scale is unused).
 bool linear_fuses_rows(int64_t m, int k);
 hipError_t launch_linear_fused(int x_type, const LinearArgs& a, hipStream_t s);

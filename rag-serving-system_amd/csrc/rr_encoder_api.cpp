@@ -79,6 +79,23 @@ int linear_sizes(int x_type, int64_t m, int32_t n, int32_t k) {
   return RR_OK;
 }
 
+// What a product's workspace holds, each part on 256 bytes: the rows' scales, the 8-bit rows, the weights' copy.
+struct LinearScratch {
+  bool fused, rows, repack;
+  int64_t kp, x_at, w_at, bytes;
+};
+LinearScratch linear_scratch(int x_type, int64_t m, int32_t n, int32_t k) {
+  LinearScratch l{};
+  l.fused = x_type != RR_TYPE_I8 && linear_fuses_rows(m, k);
+  l.rows = x_type != RR_TYPE_I8 && !l.fused && m > 0;
+  l.repack = linear_repacks(m, n, k);
+  l.kp = round_up(k, 16);
+  l.x_at = l.rows ? round_up(m * 4, 256) : 0;
+  l.w_at = l.x_at + (l.rows || l.repack ? round_up(m * l.kp, 256) : 0);
+  l.bytes = l.w_at + (l.repack ? n * l.kp : 0);
+  return l;
+}
+
 constexpr int64_t kTsMost = (1 << 23) - 1;   // 64 rows of up to 4-byte elements within 32-bit byte offsets
 
 int attention_sizes(int type, int32_t batch, int32_t heads, int32_t kv_heads, int32_t d, int32_t max_q, int32_t max_k) {
@@ -122,8 +139,7 @@ int rr_quantize_rows(int device, void* stream, int type, const void* x, int64_t 
 
 int64_t rr_linear_i8_workspace(int x_type, int64_t m, int32_t n, int32_t k) {
   if (int rc = linear_sizes(x_type, m, n, k); rc != RR_OK) return rc;
-  if (x_type == RR_TYPE_I8 || m == 0 || linear_fuses_rows(m, k)) return 0;
-  return round_up(m * 4, 256) + m * round_up(k, 16);   // the rows' scales, then the 8-bit rows
+  return linear_scratch(x_type, m, n, k).bytes;
 }
 
 int rr_linear_i8(int device, void* stream, int x_type, const void* x, int64_t ldx, const float* x_scale, const int8_t* w,
@@ -143,19 +159,26 @@ int rr_linear_i8(int device, void* stream, int x_type, const void* x, int64_t ld
   if ((x_type == RR_TYPE_I8) != (x_scale != nullptr))
     return fail(RR_E_INVALID, "%s: x_scale goes with 8-bit rows, and only with them", me);
   if (x_scale) TRY(bad_rows(me, "x_scale", x_scale, 1, 1, 4));
-  TRY(bad_scratch(me, workspace, workspace_bytes, rr_linear_i8_workspace(x_type, m, n, k)));
+  const LinearScratch l = linear_scratch(x_type, m, n, k);
+  TRY(bad_scratch(me, workspace, workspace_bytes, l.bytes));
   hipStream_t s = static_cast<hipStream_t>(stream);
   return enqueue(me, device, [&]() -> hipError_t {
     LinearArgs a{static_cast<const int8_t*>(x), ldx, x_scale, w, ldw, w_scale, bias, act, out_type, out, ldo, (int)m, n, k};
-    if (x_type != RR_TYPE_I8 && linear_fuses_rows(m, k)) return launch_linear_fused(x_type, a, s);
-    if (x_type != RR_TYPE_I8) {
+    if (l.fused) return launch_linear_fused(x_type, a, s);
+    int8_t* at = static_cast<int8_t*>(workspace);
+    if (l.rows) {
       float* sc = static_cast<float*>(workspace);
-      int8_t* q = static_cast<int8_t*>(workspace) + round_up(m * 4, 256);
-      const int64_t kp = round_up(k, 16);
-      if (hipError_t e = launch_quantize_rows(x_type, x, ldx, m, k, (int)kp, q, kp, sc, s)) return e;
-      a.x = q;
-      a.ldx = kp;
+      if (hipError_t e = launch_quantize_rows(x_type, x, ldx, m, k, (int)l.kp, at + l.x_at, l.kp, sc, s)) return e;
+      a.x = at + l.x_at;
+      a.ldx = l.kp;
       a.x_scale = sc;
+    }
+    if (l.repack) {
+      if (hipError_t e = launch_repack(l.rows ? nullptr : a.x, ldx, m, at + l.x_at, w, ldw, n, at + l.w_at, k, s)) return e;
+      a.x = at + l.x_at;
+      a.w = at + l.w_at;
+      a.ldx = a.ldw = l.kp;
+      a.k = (int)l.kp;
     }
     return launch_linear(a, s);
   });

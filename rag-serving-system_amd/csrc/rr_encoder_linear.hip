@@ -115,6 +115,25 @@ __device__ __forceinline__ u32x4 load_row16(const int8_t* row, int at, int k) {
   return v;
 }
 
+// Copies of up to two matrices of `k` columns with rows of `kp` = k rounded up to 16, zeros behind k: what the tiled product
+// takes. A thread a 16-byte column; blocks loop over 256 of them.
+struct Repack {
+  const int8_t* from;
+  int64_t ld, rows;
+  int8_t* to;
+};
+__global__ __launch_bounds__(256) void repack_kernel(Repack one, Repack two, int64_t blocks_one, int64_t blocks, int k, int kp) {
+  const unsigned cols = kp / 16;
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const Repack& p = b < blocks_one ? one : two;
+    const int64_t at = (b < blocks_one ? b : b - blocks_one) * 256;
+    const unsigned in = (unsigned)(at % cols) + threadIdx.x;
+    const int64_t r = at / cols + in / cols;
+    const int c = (int)(in % cols) * 16;
+    if (r < p.rows) store_as(p.to + r * kp + c, load_row16(p.from + r * p.ld, c, k));
+  }
+}
+
 // 64 x 64 tiles, any size and alignment: through registers into LDS, the next two steps' loads in flight during a step's matrix
 // instructions. Two groups of four waves take every other 128 bytes of k, since such calls have few tiles and wait for their
 // chain of steps; each group then finishes half of the tile, with scales that it asked for before the first step
@@ -560,6 +579,23 @@ hipError_t fused(int x_type, const LinearArgs& a, hipStream_t s) {
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
   if (a.act) return a.out_type == T_F32 ? linear<T_F32, 1>(a, s) : a.out_type == T_BF16 ? linear<T_BF16, 1>(a, s) : linear<T_F16, 1>(a, s);
   return a.out_type == T_F32 ? linear<T_F32, 0>(a, s) : a.out_type == T_BF16 ? linear<T_BF16, 0>(a, s) : linear<T_F16, 0>(a, s);
+}
+
+// The tiled product of copies, where it saves more than they cost (int8 rows, GPU time, any sizes / copies and tiles):
+//   613 x 4001 -> 1024   20.4 / 21.1 us     613 x 1307 -> 3637   25.1 / 21.1     4000 x 1000 -> 777   26.3 / 15.2
+//   16000 x 4001 -> 1024  249 / 93          2000 x 1307 -> 3637  57.8 / 27.6     2000 x 1000 -> 777   11.9 / no copies: 7.4 + 5
+bool linear_repacks(int64_t m, int n, int k) {
+  const int64_t tiles = ((int64_t)n + 63) / 64 * ((m + 63) / 64);
+  return k % 16 && m > kFewRows && tiles < (1 << 22) && m * n * k >= (int64_t)1 << 31;
+}
+
+hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const int8_t* w, int64_t ldw, int n, int8_t* to_w,
+                         int k, hipStream_t s) {
+  const int kp = (int)round_up(k, 16);
+  auto blocks_of = [&](int64_t rows) { return (rows * (kp / 16) + 255) / 256; };
+  const int64_t one = x ? blocks_of(m) : 0, all = one + blocks_of(n);
+  repack_kernel<<<grid_of(all), 256, 0, s>>>(Repack{x, ldx, m, to_x}, Repack{w, ldw, n, to_w}, one, all, k, kp);
+  return hipGetLastError();
 }
 
 // One launch instead of two, as long as every workgroup's own conversion costs less than the second launch (bf16, GPU time

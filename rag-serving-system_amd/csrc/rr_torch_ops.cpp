@@ -241,7 +241,7 @@ PyObject* linear_int8(PyObject* const* args) {
     x_scale = hold[2].data_ptr();
   }
   const int32_t n = as_int32("w: rows", wr.rows), k = as_int32("x: a row", xr.cols);
-  const int64_t need = eight ? 0 : p_linear_i8_workspace(type, xr.rows, n, k);
+  const int64_t need = p_linear_i8_workspace(type, xr.rows, n, k);
   Tensor ws = scratch(need, dev);
   auto sizes = x.sizes().vec();
   sizes.back() = n;

@@ -137,6 +137,28 @@ def test_linear_int8_inner_sizes(ops, k):
         assert ((got.double().cpu() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(49, 5000, 9001), (700, 4000, 777), (2100, 1024, 1001), (5000, 3001, 150), (70000, 70, 447),
+                                   (16000, 15000, 9), (800, 900, 3001)])
+def test_linear_int8_odd_inner_sizes_of_many_products(ops, m, n, k):
+    """The sizes at which rows and weights are copied for the tiled product, rows at any byte, and those just below."""
+    g = gen(m + n + k)
+    q = torch.randint(-128, 128, (m, k + 5), generator=g, dtype=torch.int8).cuda()[:, 3:3 + k]
+    w = torch.randint(-128, 128, (n, k + 1), generator=g, dtype=torch.int8).cuda()[:, :k]
+    sx, (_, sw, b) = (0.01 + torch.rand(m, generator=g)).cuda(), weights(g, n, 1)
+    sw, b = sw.cuda(), b.cuda()
+    rows = torch.unique(torch.cat([torch.arange(3), torch.randint(0, m, (40,), generator=g), torch.arange(m - 3, m)]))
+    got = ops.linear_int8(q, w, sw, x_scale=sx, bias=b, act="gelu")
+    want, tol = plain.linear(q[rows.cuda()], sx[rows.cuda()], w, sw, b, "gelu", torch.float32)
+    assert ((got[rows.cuda()].double().cpu() - want).abs() <= tol).all()
+    # the rows among others, in other kernels (up to 48 rows, and any size): every result is the same to the bit
+    for few in (48, 64):
+        assert torch.equal(got[:few], ops.linear_int8(q[:few], w, sw, x_scale=sx[:few], bias=b, act="gelu"))
+    x = rand(g, m, k).to(torch.bfloat16).cuda()
+    got = ops.linear_int8(x, w, sw)
+    q8, s8 = ops.quantize_rows(x)
+    assert torch.equal(got, ops.linear_int8(q8, w, sw, x_scale=s8, out_dtype=torch.bfloat16))
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_linear_int8_extremes(ops, m):
     """The longest inner size with every product at its largest: the 32-bit sum must still be exact. -128 is a valid value."""
