@@ -362,12 +362,13 @@ int rr_stream_queues(rr_handle* h, int i, uint64_t* out);
 #define RR_NORM_RMS   2   /* v / sqrt(mean(v^2) + eps) * weight + bias    */
 
 #define RR_LINEAR_KMAX 131071   /* inner size of rr_linear_i8: the 32-bit sum of k products of 8-bit values is exact */
+#define RR_LINEAR_LDMOST (1 << 22)   /* its 8-bit rows and weights lie less than this many bytes apart */
 #define RR_NORM_COLMAX 32768    /* row length of rr_block_norm */
 #define RR_ATTN_DMAX   128      /* head size of rr_cross_attention (a multiple of 8) */
 
 /* 8-bit rows: scale[r] = max|x[r]| * fl(1 / 127), q[r][c] = clamp(rint(x[r][c] / scale[r]), -127, 127), product and quotient
- * rounded to fp32, rint to even (the index's int8 copies divide by 127: their scales may differ in the last bit). A row of zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and q = 0, so every
- * product with it is NaN. x: [rows][cols] of `type` (F32, BF16, F16), row stride ldx; q: row stride ldq. */
+ * rounded to fp32, rint to even (the index's int8 copies divide by 127: their scales may differ in the last bit). A row of
+ * zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and q = 0, so every product with it is NaN. x: [rows][cols] of `type` (F32, BF16, F16), row stride ldx; q: row stride ldq. */
 int rr_quantize_rows(int device, void* stream, int type, const void* x, int64_t ldx, int64_t rows, int32_t cols,
                      int8_t* q, int64_t ldq, float* scale);
 

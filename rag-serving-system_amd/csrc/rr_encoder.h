@@ -15,8 +15,15 @@ constexpr int T_F32 = 0, T_BF16 = 1, T_F16 = 2, T_I8 = 3;   // RR_TYPE_*
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // ---- 8-bit rows and the 8-bit product (rr_encoder_linear.hip) ------------------------------------------------------
+struct WeightCopy {   // weights to copy to rows of k rounded up to 16, zeros behind k (w null: none)
+  const int8_t* w;
+  int64_t ldw;
+  int n;
+  int8_t* to;
+};
+// cols_pad: the columns of q that are written, zeros behind cols; with a copy, k rounded up to 16 of k = cols
 hipError_t launch_quantize_rows(int type, const void* x, int64_t ldx, int64_t rows, int cols, int cols_pad, int8_t* q,
-                                int64_t ldq, float* scale, hipStream_t s);
+                                int64_t ldq, float* scale, const WeightCopy& copy, hipStream_t s);
 
 struct LinearArgs {
   const int8_t* x;       // [m][k]
@@ -33,11 +40,9 @@ struct LinearArgs {
   int m, n, k;
 };
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
-// Inner sizes that are no multiple of 16, many products: x8 (null: it is padded already) and w copied to rows of k rounded up
-// to 16, zeros behind k.
-bool linear_repacks(int64_t m, int n, int k);
-hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const int8_t* w, int64_t ldw, int n, int8_t* to_w,
-                         int k, hipStream_t s);
+// Inner sizes that are no multiple of 16: whether the product takes copies of its weights, and of 8-bit rows, padded to one.
+bool linear_repacks(int x_type, int64_t m, int n, int k);
+hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const WeightCopy& copy, int k, hipStream_t s);
 // Few short floating-point rows: one launch makes their 8-bit rows too (x holds the floating-point rows, x_scale is unused).
 bool linear_fuses_rows(int64_t m, int k);
 hipError_t launch_linear_fused(int x_type, const LinearArgs& a, hipStream_t s);

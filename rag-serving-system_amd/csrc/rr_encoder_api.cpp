@@ -88,7 +88,7 @@ LinearScratch linear_scratch(int x_type, int64_t m, int32_t n, int32_t k) {
   LinearScratch l{};
   l.fused = x_type != RR_TYPE_I8 && linear_fuses_rows(m, k);
   l.rows = x_type != RR_TYPE_I8 && !l.fused && m > 0;
-  l.repack = linear_repacks(m, n, k);
+  l.repack = linear_repacks(x_type, m, n, k);
   l.kp = round_up(k, 16);
   l.x_at = l.rows ? round_up(m * 4, 256) : 0;
   l.w_at = l.x_at + (l.rows || l.repack ? round_up(m * l.kp, 256) : 0);
@@ -133,7 +133,7 @@ int rr_quantize_rows(int device, void* stream, int type, const void* x, int64_t 
   TRY(bad_rows(me, "q", q, ldq, cols, 1));
   TRY(bad_rows(me, "scale", scale, 1, 1, 4));
   return enqueue(me, device, [&] {
-    return launch_quantize_rows(type, x, ldx, rows, cols, cols, q, ldq, scale, static_cast<hipStream_t>(stream));
+    return launch_quantize_rows(type, x, ldx, rows, cols, cols, q, ldq, scale, {}, static_cast<hipStream_t>(stream));
   });
 }
 
@@ -153,6 +153,9 @@ int rr_linear_i8(int device, void* stream, int x_type, const void* x, int64_t ld
   if (m == 0) return RR_OK;
   TRY(bad_rows(me, "x", x, ldx, k, bytes_of(x_type)));
   TRY(bad_rows(me, "w", w, ldw, k, 1));
+  if ((n > 1 && ldw >= RR_LINEAR_LDMOST) || (x_type == RR_TYPE_I8 && m > 1 && ldx >= RR_LINEAR_LDMOST))
+    return fail(RR_E_UNSUPPORTED, "%s: 8-bit rows %lld and weights %lld bytes apart, not below %d", me, (long long)ldx,
+                (long long)ldw, RR_LINEAR_LDMOST);
   TRY(bad_rows(me, "w_scale", w_scale, 1, 1, 4));
   if (bias) TRY(bad_rows(me, "bias", bias, 1, 1, 4));
   TRY(bad_rows(me, "out", out, ldo, n, bytes_of(out_type)));
@@ -166,15 +169,18 @@ int rr_linear_i8(int device, void* stream, int x_type, const void* x, int64_t ld
     LinearArgs a{static_cast<const int8_t*>(x), ldx, x_scale, w, ldw, w_scale, bias, act, out_type, out, ldo, (int)m, n, k};
     if (l.fused) return launch_linear_fused(x_type, a, s);
     int8_t* at = static_cast<int8_t*>(workspace);
+    const WeightCopy copy = l.repack ? WeightCopy{w, ldw, n, at + l.w_at} : WeightCopy{};
     if (l.rows) {
       float* sc = static_cast<float*>(workspace);
-      if (hipError_t e = launch_quantize_rows(x_type, x, ldx, m, k, (int)l.kp, at + l.x_at, l.kp, sc, s)) return e;
+      if (hipError_t e = launch_quantize_rows(x_type, x, ldx, m, k, (int)l.kp, at + l.x_at, l.kp, sc, copy, s))
+        return e;
       a.x = at + l.x_at;
       a.ldx = l.kp;
       a.x_scale = sc;
     }
     if (l.repack) {
-      if (hipError_t e = launch_repack(l.rows ? nullptr : a.x, ldx, m, at + l.x_at, w, ldw, n, at + l.w_at, k, s)) return e;
+      if (!l.rows)
+        if (hipError_t e = launch_repack(a.x, ldx, m, at + l.x_at, copy, k, s)) return e;
       a.x = at + l.x_at;
       a.w = at + l.w_at;
       a.ldx = a.ldw = l.kp;

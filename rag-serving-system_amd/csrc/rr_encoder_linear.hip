@@ -1,9 +1,85 @@
 // rr_encoder_linear.hip — 8-bit rows and the 8-bit matrix product (rr_quantize_rows, rr_linear_i8).
 #include "rr_encoder_device.h"
 
+#include <algorithm>
+
 namespace rr {
 namespace enc {
 namespace {
+
+// ---- rows at any address ---------------------------------------------------------------------------------------------
+// Rows of `k` bytes that may start anywhere, `ld` apart, as a buffer of dwords: the loads' addresses are multiples of four
+// (16-byte loads at odd ones take 128 cycles an instruction here, which made 48 rows of 3769 take 20 us), and what lies behind
+// the last row is read as zeros. Rows are less than RR_LINEAR_LDMOST = 2^22 bytes apart and at
+// most 513 here: offsets below 2^32.
+struct RowBytes {
+  __amdgpu_buffer_rsrc_t r;
+  unsigned first, ld;   // first: where row 0 starts in the buffer
+  bool odd;             // whether a row may start between dwords
+  __device__ __forceinline__ RowBytes(const int8_t* rows, int64_t ld, int64_t count, int k)
+      : first((unsigned)(reinterpret_cast<uintptr_t>(rows) & 3)), ld((unsigned)ld), odd(first | (ld & 3)) {
+    r = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(rows - first), 0,
+                                          (int)((first + (unsigned)(count - 1) * this->ld + k + 3) & ~3u), 0x00020000);
+  }
+  __device__ __forceinline__ unsigned start(int row) const { return first + row * ld; }
+  // 16 bytes of the row that starts at `start`, in two parts: what is loaded (nothing behind column k) ...
+  struct Sixteen {
+    u32x4 four;
+    unsigned fifth;
+  };
+  __device__ __forceinline__ void load(Sixteen& to, unsigned start, int at, int k) const {
+    const unsigned from = at < k ? (start & ~3u) + at : ~31u;
+    to.four = __builtin_amdgcn_raw_buffer_load_b128(r, from, 0, 0);
+    if (odd) to.fifth = __builtin_amdgcn_raw_buffer_load_b32(r, from + 16, 0, 0);
+  }
+  // ... and the bytes. Those behind column k may be anything: one factor of a product has to have zeros there, see below.
+  __device__ __forceinline__ u32x4 get(const Sixteen& of, unsigned start) const {
+    if (!odd) return of.four;
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_alignbyte(i < 3 ? of.four[i + 1] : of.fifth, of.four[i], start & 3);
+    return v;
+  }
+};
+// zeros behind column k
+__device__ __forceinline__ u32x4 cut(u32x4 v, int at, int k) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int left = k - at - 4 * i;
+    v[i] = left >= 4 ? v[i] : left <= 0 ? 0u : v[i] & ((1u << 8 * left) - 1);
+  }
+  return v;
+}
+
+// ---- copies for the tiled product -------------------------------------------------------------------------------------
+// A matrix of `k` columns copied to rows of `kp` = k rounded up to 16, zeros behind k. A thread a 16-byte column; block `b`
+// takes the b-th columns, as many as it has threads.
+struct Repack {
+  const int8_t* from;
+  int64_t ld, rows;
+  int8_t* to;
+  int k, kp;
+  __host__ __device__ int64_t blocks(int threads) const { return from ? (rows * (kp / 16) + threads - 1) / threads : 0; }
+};
+__device__ __forceinline__ void repack(const Repack& p, int64_t b) {
+  const unsigned cols = p.kp / 16;
+  const int64_t at = b * blockDim.x;
+  const unsigned in = (unsigned)(at % cols) + threadIdx.x;
+  const int64_t r = at / cols + in / cols;
+  const int c = (int)(in % cols) * 16;
+  const int64_t r0 = at / cols, most = blockDim.x / cols + 2;
+  const RowBytes rows(p.from + r0 * p.ld, p.ld, p.rows - r0 < most ? p.rows - r0 : most, p.k);
+  if (r >= p.rows) return;
+  const unsigned start = rows.start((int)(r - r0));
+  RowBytes::Sixteen v;
+  rows.load(v, start, c, p.k);
+  store_as(p.to + r * p.kp + c, cut(rows.get(v, start), c, p.k));
+}
+__global__ __launch_bounds__(256) void repack_kernel(Repack one, Repack two, int64_t blocks_one, int64_t blocks) {
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x)
+    if (b < blocks_one) repack(one, b);
+    else repack(two, b - blocks_one);
+}
 
 // ---- 8-bit rows ----------------------------------------------------------------------------------------------------
 // A row in the registers of W waves, S times 16 bytes a lane; W = 1: four rows a workgroup. cols_pad: columns written, zeros
@@ -12,13 +88,18 @@ namespace {
 template <int TY, int W, int S>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_rows_kernel(const void* xv, int64_t ldx, int64_t rows,
                                                                              int cols, int cols_pad, int8_t* q, int64_t ldq,
-                                                                             float* scale) {
+                                                                             float* scale, unsigned blocks, Repack also) {
   using E = typename Elem<TY>::type;
   constexpr int N = Chunk<E>::N, kGroups = W == 1 ? 4 : 1;
+  if (blockIdx.x >= blocks) {
+    const int64_t all = also.blocks(blockDim.x);
+    for (int64_t b = blockIdx.x - blocks; b < all; b += gridDim.x - blocks) repack(also, b);
+    return;
+  }
   __shared__ float red[2 * W];
   RowReduce<W> over{red};
   const int t = threadIdx.x % (64 * W);
-  for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / (64 * W); r < rows; r += (int64_t)gridDim.x * kGroups) {
+  for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / (64 * W); r < rows; r += (int64_t)blocks * kGroups) {
     const E* x = static_cast<const E*>(xv) + r * ldx;
     Chunk<E> c[S];
 #pragma unroll
@@ -44,11 +125,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_rows_kernel(co
 // Rows of any length: one workgroup per row, two passes over it (the second one from cache).
 template <int TY>
 __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const void* xv, int64_t ldx, int64_t rows, int cols,
-                                                                 int cols_pad, int8_t* q, int64_t ldq, float* scale) {
+                                                                 int cols_pad, int8_t* q, int64_t ldq, float* scale,
+                                                                 unsigned blocks, Repack also) {
   using E = typename Elem<TY>::type;
   __shared__ float red[8];
+  if (blockIdx.x >= blocks) {
+    const int64_t all = also.blocks(blockDim.x);
+    for (int64_t b = blockIdx.x - blocks; b < all; b += gridDim.x - blocks) repack(also, b);
+    return;
+  }
   RowReduce<4> over{red};
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+  for (int64_t r = blockIdx.x; r < rows; r += blocks) {
     const E* x = static_cast<const E*>(xv) + r * ldx;
     unsigned m = 0;
     for (int c = threadIdx.x; c < cols; c += 256) {
@@ -101,39 +188,6 @@ __device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, i3
   }
 }
 
-// 16 bytes of a row of `k`, zeros behind its end: there the row's last 16 bytes, moved down.
-__device__ __forceinline__ u32x4 load_row16(const int8_t* row, int at, int k) {
-  if (at + 16 <= k) return load_as<u32x4>(row + at);
-  if (at >= k) return u32x4{0, 0, 0, 0};
-  if (k >= 16)
-    return __builtin_bit_cast(u32x4, load_as<unsigned __int128>(row + k - 16) >> 8 * (at + 16 - k));
-  u32x4 v;
-  int8_t b[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) b[i] = at + i < k ? row[at + i] : 0;
-  __builtin_memcpy(&v, b, 16);
-  return v;
-}
-
-// Copies of up to two matrices of `k` columns with rows of `kp` = k rounded up to 16, zeros behind k: what the tiled product
-// takes. A thread a 16-byte column; blocks loop over 256 of them.
-struct Repack {
-  const int8_t* from;
-  int64_t ld, rows;
-  int8_t* to;
-};
-__global__ __launch_bounds__(256) void repack_kernel(Repack one, Repack two, int64_t blocks_one, int64_t blocks, int k, int kp) {
-  const unsigned cols = kp / 16;
-  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const Repack& p = b < blocks_one ? one : two;
-    const int64_t at = (b < blocks_one ? b : b - blocks_one) * 256;
-    const unsigned in = (unsigned)(at % cols) + threadIdx.x;
-    const int64_t r = at / cols + in / cols;
-    const int c = (int)(in % cols) * 16;
-    if (r < p.rows) store_as(p.to + r * kp + c, load_row16(p.from + r * p.ld, c, k));
-  }
-}
-
 // 64 x 64 tiles, any size and alignment: through registers into LDS, the next two steps' loads in flight during a step's matrix
 // instructions. Two groups of four waves take every other 128 bytes of k, since such calls have few tiles and wait for their
 // chain of steps; each group then finishes half of the tile, with scales that it asked for before the first step
@@ -147,27 +201,28 @@ __global__ __launch_bounds__(256 * kAnyGroups) void linear_any_kernel(LinearArgs
   const int wn = (wave & 1) * 32, wm = (wave >> 1) * 32;
   int8_t *lw = lds[group][0], *lx = lds[group][1];
   struct Step {
-    u32x4 w[2], x[2];
+    RowBytes::Sixteen w[2], x[2];
   };
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int n0 = (int)(tile % tiles_n) * 64;
     const int64_t m0 = tile / tiles_n * 64;
-    const int8_t* wr = a.w + (int64_t)(n0 + row < a.n ? n0 + row : a.n - 1) * a.ldw;
-    const int8_t* xr = a.x + (m0 + row < a.m ? m0 + row : a.m - 1) * a.ldx;
-    auto fetch = [&](Step& s, int k0) {   // (zeros behind k)
+    const RowBytes rw(a.w + n0 * a.ldw, a.ldw, a.n - n0 < 64 ? a.n - n0 : 64, a.k);
+    const RowBytes rx(a.x + m0 * a.ldx, a.ldx, a.m - m0 < 64 ? a.m - m0 : 64, a.k);
+    const unsigned w_at = rw.start(row), x_at = rx.start(row);
+    auto fetch = [&](Step& s, int k0) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        s.w[h] = load_row16(wr, k0 + 64 * h + col, a.k);
-        s.x[h] = load_row16(xr, k0 + 64 * h + col, a.k);
+        rw.load(s.w[h], w_at, k0 + 64 * h + col, a.k);
+        rx.load(s.x[h], x_at, k0 + 64 * h + col, a.k);
       }
     };
     i32x4 acc[2][2] = {};
-    auto take = [&](Step& s, int next) {   // and asks for the step at `next`
+    auto take = [&](Step& s, int k0, int next) {   // and asks for the step at `next`
       __syncthreads();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        *reinterpret_cast<u32x4*>(lw + row * kPad + 64 * h + col) = s.w[h];
-        *reinterpret_cast<u32x4*>(lx + row * kPad + 64 * h + col) = s.x[h];
+        *reinterpret_cast<u32x4*>(lw + row * kPad + 64 * h + col) = rw.get(s.w[h], w_at);
+        *reinterpret_cast<u32x4*>(lx + row * kPad + 64 * h + col) = cut(rx.get(s.x[h], x_at), k0 + 64 * h + col, a.k);
       }
       __syncthreads();
       fetch(s, next);
@@ -205,8 +260,8 @@ __global__ __launch_bounds__(256 * kAnyGroups) void linear_any_kernel(LinearArgs
       row_scales[j] = a.x_scale[m < a.m ? m : a.m - 1];
     }
     for (int k0 = 0; k0 < a.k; k0 += 2 * kRound) {
-      take(one, first + k0 + 2 * kRound);
-      if (k0 + kRound < a.k) take(two, first + k0 + 3 * kRound);
+      take(one, first + k0, first + k0 + 2 * kRound);
+      if (k0 + kRound < a.k) take(two, first + k0 + kRound, first + k0 + 3 * kRound);
     }
     __syncthreads();
     i32x4* other = reinterpret_cast<i32x4*>(lds[0][0]);   // [group][wave][j][lane]
@@ -274,8 +329,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
   __shared__ float sc[16];
   __shared__ float red[2 * kFewWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, kp = (a.k + 63) / 64 * 64;
-  const int8_t* wr = a.w + (int64_t)(n0 + i < a.n ? n0 + i : a.n - 1) * a.ldw;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * R, kp = (a.k + 63) / 64 * 64;   // (fused: one block of rows)
+  const RowBytes rw(a.w + (int64_t)n0 * a.ldw, a.ldw, a.n - n0 < 16 ? a.n - n0 : 16, a.k);
+  const RowBytes rx(a.x + m0 * a.ldx, a.ldx, a.m - m0 < 16 * R ? a.m - m0 : 16 * R, a.k);   // (not fused)
+  const unsigned w_at = rw.start(i);
   i32x4 acc[R] = {};
   float scale[4], bias[4];   // of the four channels that this lane finishes
 #pragma unroll
@@ -289,16 +346,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
   if constexpr (kFused)
     if (mine < a.m) rows.load(reinterpret_cast<const typename Elem<XT>::type*>(a.x) + mine * a.ldx, a.k, t);
   for (int k0 = wave * 64; k0 < kp || (kFused && k0 == wave * 64); k0 += kAhead * kFewWaves * 64) {
-    u32x4 w[kAhead];
+    RowBytes::Sixteen w[kAhead], x[kFused ? 1 : kAhead][R];
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) w[s] = load_row16(wr, k0 + s * kFewWaves * 64 + 16 * g, a.k);
-    u32x4 x[kFused ? 1 : kAhead][R];
+    for (int s = 0; s < kAhead; ++s) rw.load(w[s], w_at, k0 + s * kFewWaves * 64 + 16 * g, a.k);
     if constexpr (!kFused)
 #pragma unroll
       for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          x[s][r] = load_row16(a.x + (16 * r + i < a.m ? 16 * r + i : a.m - 1) * a.ldx, k0 + s * kFewWaves * 64 + 16 * g, a.k);
+        for (int r = 0; r < R; ++r) rx.load(x[s][r], rx.start(16 * r + i), k0 + s * kFewWaves * 64 + 16 * g, a.k);
     if constexpr (kFused) {
       if (k0 == wave * 64) {   // (every wave comes here once, with or without weights to multiply)
         if (mine < a.m) rows.put(x8 + mine * kp, kp, sc + mine, t, red);
@@ -306,19 +361,21 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
       }
     }
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s)
+    for (int s = 0; s < kAhead; ++s) {
+      const int at = k0 + s * kFewWaves * 64 + 16 * g;
+      const u32x4 ws = rw.get(w[s], w_at);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         u32x4 v;
         if constexpr (kFused) {
-          const int at = k0 + s * kFewWaves * 64 + 16 * g;
           v = u32x4{0, 0, 0, 0};
           if (i < a.m && at < kp) v = *reinterpret_cast<const u32x4*>(x8 + i * kp + at);
         } else {
-          v = x[s][r];
+          v = cut(rx.get(x[s][r], rx.start(16 * r + i)), at, a.k);
         }
-        acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w[s]), __builtin_bit_cast(i32x4, v), acc[r], 0, 0, 0);
+        acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, ws), __builtin_bit_cast(i32x4, v), acc[r], 0, 0, 0);
       }
+    }
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) sums[wave][r][lane] = acc[r];
@@ -327,8 +384,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
     i32x4 c = sums[0][r][lane];
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) c += sums[w][r][lane];
-    const int m = 16 * r + i, n = n0 + 4 * g;
-    if (m < a.m && n < a.n) store4<OT>(a, m, n, c, kFused ? sc[m] : a.x_scale[m], scale, bias);
+    const int m = m0 + 16 * r + i, n = n0 + 4 * g;
+    if (m < a.m && n < a.n) store4<OT>(a, m, n, c, kFused ? sc[16 * r + i] : a.x_scale[m], scale, bias);
   }
 }
 
@@ -500,11 +557,12 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
 namespace {
 template <int TY>
 hipError_t quantize(const void* x, int64_t ldx, int64_t rows, int cols, int cols_pad, int8_t* q, int64_t ldq, float* scale,
-                    hipStream_t s) {
+                    const Repack& also, hipStream_t s) {
   constexpr int N = Chunk<typename Elem<TY>::type>::N;
   auto go = [&](auto kernel, int waves) {
-    const int groups = waves == 1 ? 4 : 1;
-    kernel<<<grid_of((rows + groups - 1) / groups), 64 * waves * groups, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale);
+    const int groups = waves == 1 ? 4 : 1, threads = 64 * waves * groups;
+    const unsigned blocks = grid_of((rows + groups - 1) / groups).x, more = (unsigned)std::min<int64_t>(also.blocks(threads), 1 << 16);
+    kernel<<<dim3(blocks + more), threads, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale, blocks, also);
     return hipGetLastError();
   };
   const int chunks = (cols_pad + N - 1) / N;
@@ -514,16 +572,16 @@ hipError_t quantize(const void* x, int64_t ldx, int64_t rows, int cols, int cols
   if (chunks <= 64 * 8) return go(quantize_rows_kernel<TY, 4, 2>, 4);
   if (chunks <= 64 * 16) return go(quantize_rows_kernel<TY, 4, 4>, 4);
   if (chunks <= 64 * 32) return go(quantize_rows_kernel<TY, 8, 4>, 8);
-  quantize_long_rows_kernel<TY><<<grid_of(rows), 256, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale);
-  return hipGetLastError();
+  return go(quantize_long_rows_kernel<TY>, 4);
 }
 }  // namespace
 
 hipError_t launch_quantize_rows(int type, const void* x, int64_t ldx, int64_t rows, int cols, int cols_pad, int8_t* q,
-                                int64_t ldq, float* scale, hipStream_t s) {
-  return type == T_F32    ? quantize<T_F32>(x, ldx, rows, cols, cols_pad, q, ldq, scale, s)
-         : type == T_BF16 ? quantize<T_BF16>(x, ldx, rows, cols, cols_pad, q, ldq, scale, s)
-                          : quantize<T_F16>(x, ldx, rows, cols, cols_pad, q, ldq, scale, s);
+                                int64_t ldq, float* scale, const WeightCopy& copy, hipStream_t s) {
+  const Repack also{copy.w, copy.ldw, copy.n, copy.to, cols, cols_pad};
+  return type == T_F32    ? quantize<T_F32>(x, ldx, rows, cols, cols_pad, q, ldq, scale, also, s)
+         : type == T_BF16 ? quantize<T_BF16>(x, ldx, rows, cols, cols_pad, q, ldq, scale, also, s)
+                          : quantize<T_F16>(x, ldx, rows, cols, cols_pad, q, ldq, scale, also, s);
 }
 
 namespace {
@@ -537,23 +595,28 @@ hipError_t tiled(const LinearArgs& a, hipStream_t s) {
 template <int OT, int ACT>
 hipError_t linear(const LinearArgs& a, hipStream_t s) {
   auto tiles_of = [&](int64_t tn, int64_t tm) { return ((a.n + tn - 1) / tn) * ((a.m + tm - 1) / tm); };
-  if (a.m <= kFewRows) {
-    const dim3 grid((a.n + 15) / 16);
+  const bool rows16 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw | a.k) & 15) == 0;
+  // More rows in blocks of 48, as long as every workgroup has a CU: where the tiles' chain of steps is longer (4096 columns
+  // 11.6 us against 9.9, 3008 9.8 / 7.2, 1024 5.3 / 5.2, 400 4.3 / 4.6), or the rows fit no
+  // tile (192 x 3769 -> 1024 18.9 / 13.5, x 1001 9.1 / 6.7).
+  const int64_t few = ((int64_t)a.n + 15) / 16 * ((a.m + kFewRows - 1) / kFewRows);
+  if (a.m <= kFewRows || (few <= 256 && (!rows16 || a.k >= 1024))) {
+    const dim3 grid((a.n + 15) / 16, (a.m + kFewRows - 1) / kFewRows);
     if (a.m <= 16) linear_few_kernel<OT, 1, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     else if (a.m <= 32) linear_few_kernel<OT, 2, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     else linear_few_kernel<OT, 3, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     return hipGetLastError();
   }
-  const bool rows16 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw | a.k) & 15) == 0 &&
-                      a.ldx < (1 << 22) && a.ldw < (1 << 22);
   // The largest tile that still gives the 256 CUs one each, or nearly (int8 rows, GPU time; channels x rows, waves, buffers):
   //   16384 x 4096 -> 1024   256 x 256  70 us    128 x 128  85    64 x 64  125
   //    4096 x 4096 -> 1024   128 x 128, four buffers 24, two 27;  64 x 64  32
   //    2048 x 1024 -> 4096   128 x 128, four buffers 19, two 15;  64 x 64  22   (two tiles a CU: they fill each other's waits)
   //     613 x 1024 -> 4096   64 x 128  9.0         128 x 128  9.5  64 x 64  10.0
   //     613 x 4096 -> 1024   64 x 64  11.5         128 x 128 19
+  // Short rows are mostly results: two tiles a CU store while the other multiplies (256 x 256 / 128 x 128, two buffers):
+  //   14500 x 512 -> 3530   51.8 / 43.1, with GELU 80.7 / 58.1;  16384 x 512 -> 4096 with GELU 82 / 71, x 768 94 / 97
   if (rows16 && tiles_of(64, 64) < (1 << 22)) {
-    if (tiles_of(256, 256) >= 192) return tiled<OT, ACT, 256, 256, 2, 4, 2>(a, s);
+    if (tiles_of(256, 256) >= 192 && a.k > 512) return tiled<OT, ACT, 256, 256, 2, 4, 2>(a, s);
     if (tiles_of(128, 128) > 256) return tiled<OT, ACT, 128, 128, 2, 4, 2>(a, s);
     if (tiles_of(128, 128) >= 224) return tiled<OT, ACT, 128, 128, 2, 4, 4>(a, s);
     if (tiles_of(64, 128) >= 256) return tiled<OT, ACT, 64, 128, 2, 4, 3>(a, s);
@@ -584,17 +647,17 @@ hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
 // The tiled product of copies, where it saves more than they cost (int8 rows, GPU time, any sizes / copies and tiles):
 //   613 x 4001 -> 1024   20.4 / 21.1 us     613 x 1307 -> 3637   25.1 / 21.1     4000 x 1000 -> 777   26.3 / 15.2
 //   16000 x 4001 -> 1024  249 / 93          2000 x 1307 -> 3637  57.8 / 27.6     2000 x 1000 -> 777   11.9 / no copies: 7.4 + 5
-bool linear_repacks(int64_t m, int n, int k) {
+// Floating-point rows are made with the padding, and the launch that makes them copies the weights beside them.
+bool linear_repacks(int x_type, int64_t m, int n, int k) {
   const int64_t tiles = ((int64_t)n + 63) / 64 * ((m + 63) / 64);
-  return k % 16 && m > kFewRows && tiles < (1 << 22) && m * n * k >= (int64_t)1 << 31;
+  return k % 16 && m > kFewRows && tiles < (1 << 22) && m * n * k >= (x_type == T_I8 ? (int64_t)1 << 31 : 0);
 }
 
-hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const int8_t* w, int64_t ldw, int n, int8_t* to_w,
-                         int k, hipStream_t s) {
+hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const WeightCopy& copy, int k, hipStream_t s) {
   const int kp = (int)round_up(k, 16);
-  auto blocks_of = [&](int64_t rows) { return (rows * (kp / 16) + 255) / 256; };
-  const int64_t one = x ? blocks_of(m) : 0, all = one + blocks_of(n);
-  repack_kernel<<<grid_of(all), 256, 0, s>>>(Repack{x, ldx, m, to_x}, Repack{w, ldw, n, to_w}, one, all, k, kp);
+  const Repack one{x, ldx, m, to_x, k, kp}, two{copy.w, copy.ldw, copy.n, copy.to, k, kp};
+  const int64_t blocks = one.blocks(256) + two.blocks(256);
+  repack_kernel<<<grid_of(blocks), 256, 0, s>>>(one, two, one.blocks(256), blocks);
   return hipGetLastError();
 }
 

@@ -53,6 +53,7 @@ RR_NORM_NONE = 0
 RR_NORM_LAYER = 1
 RR_NORM_RMS = 2
 RR_LINEAR_KMAX = 131071
+RR_LINEAR_LDMOST = 1 << 22
 RR_NORM_COLMAX = 32768
 RR_ATTN_DMAX = 128
 

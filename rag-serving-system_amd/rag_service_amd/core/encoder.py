@@ -27,6 +27,31 @@ def _torch():
     return sys.modules["torch"]               # (the model handed over is torch's)
 
 
+def look(ids, mask, types, pad, words, kinds):
+    """The batch as the host has to know it, in one read: every sequence's number of tokens, as a list and on the device
+    (int32). Refuses batches that are not padded on the right by the pad token, sequences without tokens, and ids and token
+    types (None: all 0) that the embedding tables do not hold."""
+    torch = _torch()
+    real = mask.sum(1)
+    right = ((torch.arange(ids.shape[1], device=ids.device) < real[:, None]) == mask).all() & ((ids != pad) == mask).all()
+    seen = [real, torch.stack([right.long(), *(x.long() for x in torch.aminmax(ids))])]
+    if types is not None:
+        seen.append(torch.stack([*torch.aminmax(types), types.masked_fill(mask, 0).abs().amax()]).long())
+    lengths = torch.cat(seen).tolist()
+    if types is not None:
+        *lengths, low, high, pads = lengths
+        if low < 0 or high >= kinds or pads:
+            raise ValueError(f"HipEncoder: token types {low} to {high} of {kinds}; those of pads are 0")
+    *lengths, good, low, high = lengths
+    if low < 0 or high >= words:
+        raise ValueError(f"HipEncoder: token ids {low} to {high} of {words}")
+    if not all(lengths):
+        raise ValueError("HipEncoder: a sequence without tokens")
+    if not good:
+        raise ValueError("HipEncoder takes batches padded on the right with the pad token, and no pads elsewhere")
+    return lengths, real.to(torch.int32)
+
+
 class EncoderOutput:
     def __init__(self, last_hidden_state):
         self.last_hidden_state = last_hidden_state
@@ -95,13 +120,14 @@ class HipEncoder:
 
         with torch.no_grad():
             e = self._model.embeddings
-            self._words, self._positions, self._types = (
-                x.weight.detach().to(device) for x in (e.word_embeddings, e.position_embeddings, e.token_type_embeddings))
-            self._embedding_norm = norm(e.LayerNorm, torch.float32)
-            self._layers = [{"q": linear(x.attention.self.query), "kv": linear(x.attention.self.key, x.attention.self.value),
-                             "o": linear(x.attention.output.dense), "norm1": norm(x.attention.output.LayerNorm, t),
-                             "up": linear(x.intermediate.dense), "down": linear(x.output.dense),
-                             "norm2": norm(x.output.LayerNorm, t)} for x in self._model.encoder.layer]
+            tables = [x.weight.detach().to(device) for x in (e.word_embeddings, e.position_embeddings, e.token_type_embeddings)]
+            embedding_norm = norm(e.LayerNorm, torch.float32)
+            layers = [{"q": linear(x.attention.self.query), "kv": linear(x.attention.self.key, x.attention.self.value),
+                       "o": linear(x.attention.output.dense), "norm1": norm(x.attention.output.LayerNorm, t),
+                       "up": linear(x.intermediate.dense), "down": linear(x.output.dense),
+                       "norm2": norm(x.output.LayerNorm, t)} for x in self._model.encoder.layer]
+        self._words, self._positions, self._types = tables      # (all of it, or nothing)
+        self._embedding_norm, self._layers = embedding_norm, layers
         self._t, self._device = t, device
         return self
 
@@ -123,22 +149,15 @@ class HipEncoder:
         with torch.no_grad(), torch.cuda.device(self._device):
             ids = input_ids.to(self._device)
             mask = ids != self.pad if attention_mask is None else attention_mask.to(self._device) != 0
-            # one look at the batch from the host: its lengths, and whether it is padded on the right, by pads
-            real = mask.sum(1)
-            right = ((torch.arange(length, device=self._device) < real[:, None]) == mask).all() & ((ids != self.pad) == mask).all()
-            *lengths, good = torch.cat([real, right[None].to(real.dtype)]).tolist()
-            if not all(lengths):
-                raise ValueError("HipEncoder: a sequence without tokens")
-            if not good:
-                raise ValueError("HipEncoder takes batches padded on the right with the pad token, and no pads elsewhere")
+            types = None if token_type_ids is None else token_type_ids.to(self._device)
+            lengths, lens = look(ids, mask, types, self.pad, self._words.shape[0], self._types.shape[0])
             offsets, source, place, spread = pack(lengths, length)
             move = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self._device)  # noqa: E731
             rows = move(np.stack([source, np.where(place < 0, self.pad, self.pad + 1 + place)]))
             offs, spread = move(offsets), move(spread)
-            lens = real.to(torch.int32)
             tokens = ids.reshape(-1)[rows[0]]
             other = self._positions[rows[1]].float()
-            kind = 0 if token_type_ids is None else token_type_ids.to(self._device).reshape(-1)[rows[0]]
+            kind = 0 if token_type_ids is None else types.reshape(-1)[rows[0]]
             other = other + self._types[kind].float()
             h = self._forward(self._words[tokens].float(), other, offs, lens, int(np.diff(offsets).max()), max(lengths))
             return EncoderOutput(h.float()[spread].view(batch, length, -1))

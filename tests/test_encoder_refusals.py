@@ -69,6 +69,13 @@ def test_linear_unsupported(lib):
     assert lib.rr_linear_i8_workspace(3, 4, 16, 64) == 0
     refused(lib, linear(lib, n=(1 << 26) + 1, ldo=1 << 27), _lib.RR_E_UNSUPPORTED, "2^26")
     assert lib.rr_linear_i8_workspace(1, 40, 16, 64) >= 40 * (64 + 4)
+    refused(lib, linear(lib, ldw=_lib.RR_LINEAR_LDMOST), _lib.RR_E_UNSUPPORTED, "apart")
+    refused(lib, linear(lib, x_type=3, x_scale=P, ldx=_lib.RR_LINEAR_LDMOST), _lib.RR_E_UNSUPPORTED, "apart")
+    # odd inner sizes: copies of the weights beside floating-point rows, of both sides for many products of 8-bit rows
+    assert lib.rr_linear_i8_workspace(1, 40, 16, 65) < 40 * (80 + 4) + 512
+    assert lib.rr_linear_i8_workspace(1, 64, 16, 65) >= 64 * (80 + 4) + 16 * 80
+    assert lib.rr_linear_i8_workspace(3, 64, 16, 65) == 0
+    assert lib.rr_linear_i8_workspace(3, 1 << 14, 1 << 11, 65) >= ((1 << 14) + (1 << 11)) * 80
 
 
 def norm(lib, device=0, type=0, rows=4, cols=8, y=P, ldy=8, x=P, ldx=8, rs=1.0, gate=NULL, ldg=8, gate_rows=1,

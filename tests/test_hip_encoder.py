@@ -70,6 +70,34 @@ def test_refuses_models_it_does_not_run():
         HipEncoder(make_model(64, 2, 1, 64))(torch.zeros(1, 3, dtype=torch.long))
 
 
+def test_look_reads_the_batch_and_refuses_what_it_cannot_run():
+    from rag_service_amd.core.encoder import look
+    ids, mask = batch_of([3, 5, 1], 5)
+    for t in (torch.int64, torch.int32):
+        lengths, lens = look(ids.to(t), mask != 0, None, 1, 500, 1)
+        assert lengths == [3, 5, 1] and lens.tolist() == [3, 5, 1] and lens.dtype == torch.int32
+    types = torch.zeros_like(ids)
+    assert look(ids, mask != 0, types, 1, 500, 1)[0] == [3, 5, 1]
+    types[0, 1] = 1                                        # a real token's
+    assert look(ids, mask != 0, types, 1, 500, 2)[0] == [3, 5, 1]
+    with pytest.raises(ValueError, match="token types 0 to 1 of 1"):
+        look(ids, mask != 0, types, 1, 500, 1)
+    types[0, 4] = 1                                        # a pad's: pads of a sequence would no longer be alike
+    with pytest.raises(ValueError, match="pads are 0"):
+        look(ids, mask != 0, types, 1, 500, 2)
+    with pytest.raises(ValueError, match="token types -1"):
+        look(ids, mask != 0, -mask, 1, 500, 2)
+    for bad in (-1, 500, 2 ** 40):
+        other = ids.clone()
+        other[1, 2] = bad
+        with pytest.raises(ValueError, match="token ids"):
+            look(other, mask != 0, None, 1, 500, 1)
+    with pytest.raises(ValueError, match="without tokens"):
+        look(ids, torch.zeros_like(mask) != 0, None, 1, 500, 1)
+    with pytest.raises(ValueError, match="right"):
+        look(ids.flip(1), mask.flip(1) != 0, None, 1, 500, 1)
+
+
 def test_batch_processor_refuses_it_off_the_gpu():
     from rag_service_amd.core.batch_processor import BatchProcessor
     with pytest.raises(ValueError, match="GPU only"):
