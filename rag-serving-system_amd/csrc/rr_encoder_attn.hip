@@ -82,6 +82,7 @@ template <int TY, int DP> struct Core;
 template <int TY, int DP>
 struct Core16 {
   static constexpr int kKeys = 32, kMine = 8, kTiles = DP / 16, kSteps = DP / 32;
+  static constexpr int kRun = kTiles;
   static constexpr int VW = DP / 16;   // values of a V row a lane loads: tile t's row i is dimension VW i + t
   using E = typename Elem<TY>::type;
   typedef E e8 __attribute__((ext_vector_type(8)));
@@ -175,15 +176,21 @@ template <int DP> struct Core<T_F16, DP> : Core16<T_F16, DP> {};
 // fp32: 16 keys a block, contractions of four; lane i, g holds the scores of query i with keys 4g + r.
 template <int DP>
 struct Core<T_F32, DP> {
-  static constexpr int kKeys = 16, kMine = 4, kTiles = DP / 16, kSteps = DP / 16, kWide = DP / 64;
+  // a V row's dimensions: kWide times 64, of which a lane loads four, then kPair times 32, of which it loads two
+  static constexpr int kKeys = 16, kMine = 4, kTiles = DP / 16, kSteps = DP / 16, kWide = DP / 64, kPair = DP / 32 % 2;
+  static constexpr int kRun = 4;
   using E = float;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
   struct Keys {
-    f32x4 k[kSteps], v[4][kWide];
+    f32x4 k[kSteps], v[4][kWide ? kWide : 1];
+    f32x2 pair[kPair ? 4 : 1];
   };
   f32x4 q[kSteps];
 
   static __device__ __forceinline__ int key(int g, int j) { return 4 * g + j; }
-  static __device__ __forceinline__ int dim(int t, int i) { return 64 * (t / 4) + 4 * i + t % 4; }
+  static __device__ __forceinline__ int dim(int t, int i) {
+    return t < 4 * kWide ? 64 * (t / 4) + 4 * i + t % 4 : 64 * kWide + 2 * i + t % 2;
+  }
   __device__ __forceinline__ void load_q(const float* row, bool there, bool flip, int d, int g) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -205,6 +212,10 @@ struct Core<T_F32, DP> {
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int w = 0; w < kWide; ++w) to.v[j][w] = __builtin_bit_cast(f32x4, v.load<16>(at + 4 * j * ts + 256 * w));
+    if constexpr (kPair)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        to.pair[j] = __builtin_bit_cast(f32x2, v.load<8>(at - 8 * (threadIdx.x & 15) + 4 * j * ts + 256 * kWide));
   }
   __device__ __forceinline__ void scores(const Keys& of, float* s) const {
     f32x4 c = {0, 0, 0, 0};
@@ -219,12 +230,11 @@ struct Core<T_F32, DP> {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int w = 0; w < kWide; ++w)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const float v = (valid >> j & 1) ? of.v[j][w][t] : 0.f;
-          acc[4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[j], acc[4 * w + t], 0, 0, 0);
-        }
+      for (int t = 0; t < kTiles; ++t) {
+        const float x = t < 4 * kWide ? of.v[j][t < 4 * kWide ? t / 4 : 0][t % 4] : of.pair[kPair ? j : 0][t % 2];
+        const float v = (valid >> j & 1) ? x : 0.f;
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[j], acc[t], 0, 0, 0);
+      }
   }
 };
 
@@ -239,12 +249,38 @@ __device__ __forceinline__ E* out_row(const AttnParams& p, const Span& sq, int b
   return static_cast<E*>(a.out) + (a.q_offsets ? sq.first * a.o_ts : b * a.o_bs) + qi * a.o_ts + h * a.o_hs;
 }
 
+// A row of sums times `scale`, dimensions below d (a multiple of 8)
+template <class C>
+__device__ __forceinline__ void store_row(typename C::E* to, const f32x4* acc, float scale, int d, int g) {
+  using E = typename C::E;
+  // tiles whose rows are neighbouring dimensions; kLeft: the narrower run of fp32's last two
+  constexpr int kRun = C::kRun, kLeft = C::kTiles % kRun;
+  typedef E run __attribute__((ext_vector_type(kRun)));
+  typedef E left __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int t = 0; t < C::kTiles - kLeft; t += kRun) {
+      run v;
+#pragma unroll
+      for (int x = 0; x < kRun; ++x) v[x] = (E)(acc[t + x][r] * scale);
+      const int at = C::dim(t, 4 * g + r);
+      if (at < d) store_as(to + at, v);
+    }
+    if constexpr (kLeft != 0) {
+      const int at = C::dim(C::kTiles - 2, 4 * g + r);
+      const left v = {(E)(acc[C::kTiles - 2][r] * scale), (E)(acc[C::kTiles - 1][r] * scale)};
+      if (at < d) store_as(to + at, v);
+    }
+  }
+}
+
 // Tiles of 16 query rows. WK = 1: four tiles a workgroup, a wave each, which takes all keys of its own; nothing is shared. WK
 // waves: one tile and one piece of the keys a workgroup, each wave every WK-th block of keys, their sums joined in LDS. Either
 // way a wave has its next block of keys on the way while it works on one, straight from memory into registers.
 // Short sequences and fp32. 32 x 20 queries x 20 keys, 16 heads of 64: bf16 4.2 us, fp32 6.1 (a launch and the latencies of
-// offsets, rows and result); fp32 8 x 512 x 512: 102 us, 84 TFLOP/s of the 153 an fp32 library product reaches; fp32 one query
-// x 16384 keys x 4, 16 heads of 128: 182 us, 5.9 TB/s.
+// offsets, rows and result); fp32 41 x 70 x 1668, 16 heads of 32: 178 us, 55 TFLOP/s; fp32 one query x 16384 keys x 4, 16 heads
+// of 128: 184 us, 5.8 TB/s.
 template <int TY, int DP, int WK>
 __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(AttnParams p) {
   using C = Core<TY, DP>;
@@ -336,19 +372,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
     if constexpr (WK == 1) {
       E* to = out_row<E>(p, sq, b, kvh, tile * kRows + i);
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      constexpr int kRun = TY == T_F32 ? 4 : C::kTiles;   // tiles whose rows are neighbouring dimensions
-      typedef E run __attribute__((ext_vector_type(kRun)));
-      if (to)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int t = 0; t < C::kTiles; t += kRun) {
-            run v;
-#pragma unroll
-            for (int x = 0; x < kRun; ++x) v[x] = (E)(acc[t + x][r] * inv);
-            const int d = C::dim(t, 4 * g + r);
-            if (d < a.d) store_as(to + d, v);
-          }
+      if (to) store_row<C>(to, acc, inv, a.d, g);
     } else {
       __syncthreads();   // (a tile before this one may still be read)
 #pragma unroll
@@ -707,13 +731,202 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
   }
 }
 
+// ---- fp32, keys through LDS ---------------------------------------------------------------------------------------------
+// 64 query rows a workgroup, 16 a wave; every wave takes every key, 32 a step, in the products of Core<T_F32>: K and V rows lie in
+// LDS (two buffers, as above), where 16 lanes read a column of 16 K rows, or a V row's 16 columns, in all 64 banks at once.
+// Bound by the matrix instructions, in whose chains few workgroups wait: 8 x 512 x 512, 16 heads of 64: 80 us, 108 of the 153
+// TFLOP/s that an fp32 library product reaches (98 us with a wave for itself); 8 x 1024 x 1024, 8 heads of 128: 290 us, 118 (415).
+// Reading K and V ahead of the products, as the 16-bit kernel does, changes nothing where four workgroups share a CU.
+constexpr int kTileRows32 = 64;
+
+template <int DP, bool DMA>
+__global__ __launch_bounds__(256, DP > 64 ? 2 : 4) void attn_tile32_kernel(AttnParams p) {
+  using C = Core<T_F32, DP>;
+  constexpr int kKeys = 32, kCols = DP / 4, kLoads = kKeys * kCols / 256, kHalf = kKeys * DP * 4, kBuf = 2 * kHalf;
+  __shared__ __align__(1024) char lds[2 * kBuf];
+  const AttnArgs& a = p.a;
+  const unsigned each = p.tiles * p.splits, heads = p.units / p.tiles;   // (the 8 XCDs' caches, as above)
+  const unsigned at = heads % 8 ? blockIdx.x : (blockIdx.x / 8 / each * 8 + blockIdx.x % 8) * each + blockIdx.x / 8 % each;
+  const int split = at % p.splits, tile0 = at / p.splits % p.tiles;
+  const int kvh = at / each % a.kv_heads, b = at / each / a.kv_heads;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+  const Span sq = queries_of(a, b), sk = keys_of(a, b);
+  const int rows = sq.n * p.group;
+  const float* kbase = static_cast<const float*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
+  const float* vbase = static_cast<const float*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
+  const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+  auto byte_of = [&](int kb) -> unsigned char { return mask && lane < 32 && kb + lane < sk.n ? mask[kb + lane] : 1; };
+  auto bits_of = [&](int kb, unsigned char there) { return (unsigned)__ballot(lane < 32 && kb + lane < sk.n && there); };
+  auto column = [](unsigned r, unsigned c) { return c ^ (DP % 64 ? r / 2 % 8 : r % 16); };
+  // this lane's 16 bytes of load j: key row `key` at LDS column chunk % kCols
+  unsigned key[kLoads], from_k[kLoads], from_v[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const unsigned chunk = (4 * j + wave) * 64 + lane, c = column(chunk / kCols, chunk % kCols);
+    key[j] = chunk / kCols;
+    const bool in = (int)(4 * c) < a.d;
+    from_k[j] = in ? 4 * (key[j] * (unsigned)a.k_ts + 4 * c) : kNowhere;
+    from_v[j] = in ? 4 * (key[j] * (unsigned)a.v_ts + 4 * c) : kNowhere;
+  }
+  const unsigned lds0 = (unsigned)(uintptr_t)lds;
+
+  for (int tile = tile0; tile < (rows + kTileRows32 - 1) / kTileRows32; tile += p.tiles) {
+    const bool whole = p.splits == 1 || tile >= (int)p.tiles;
+    if (whole && split) break;
+    const int pieces = whole ? 1 : p.splits;
+    const unsigned row = tile * kTileRows32 + wave * 16 + i;
+    const bool busy = tile * kTileRows32 + wave * 16 < rows;   // (of this wave)
+    u32x4 kr[DMA ? 1 : kLoads], vr[DMA ? 1 : kLoads];
+    auto fetch = [&](int kb, unsigned bits, int buf) {
+      const int n = sk.n - kb < kKeys ? sk.n - kb : kKeys;
+      const RowBuffer<float> k(kbase, a.k_ts, kb, n, a.d), v(vbase, a.v_ts, kb, n, a.d);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const bool there = bits >> key[j] & 1;
+        const unsigned at_k = there ? from_k[j] : kNowhere, at_v = there ? from_v[j] : kNowhere;
+        if constexpr (DMA) {
+          const unsigned to = lds0 + buf * kBuf + (4 * j + wave) * 1024;
+          k.to_lds(at_k, to);
+          v.to_lds(at_v, to + kHalf);
+        } else {
+          kr[j] = k.template load<16>(at_k);
+          vr[j] = v.template load<16>(at_v);
+        }
+      }
+    };
+    auto keep = [&](int buf) {
+      if constexpr (!DMA)
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          char* to = lds + buf * kBuf + (4 * j + wave) * 1024 + lane * 16;
+          *reinterpret_cast<u32x4*>(to) = kr[j];
+          *reinterpret_cast<u32x4*>(to + kHalf) = vr[j];
+        }
+    };
+    const int step = pieces * kKeys;
+    int kb = split * kKeys, buf = 0;
+    unsigned char ahead = byte_of(kb + step);
+    unsigned valid = bits_of(kb, byte_of(kb));
+    C core;
+    {
+      const unsigned qi = row / p.group, h = kvh * p.group + row % p.group;
+      const float* q = static_cast<const float*>(a.q) + (a.q_offsets ? sq.first * a.q_ts : b * a.q_bs) + qi * a.q_ts + h * a.q_hs;
+      core.load_q(q, (int)qi < sq.n, p.flip, a.d, g);
+    }
+    if (kb < sk.n) {
+      fetch(kb, valid, 0);
+      keep(0);
+    }
+    f32x4 acc[C::kTiles] = {};
+    float m = -INFINITY, l = 0.f;
+    auto take = [&](const char* k_rows, unsigned here) {
+      f32x4 s[2] = {};
+#pragma unroll
+      for (int st = 0; st < C::kSteps; ++st) {
+        f32x4 kf[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          kf[h] = *reinterpret_cast<const f32x4*>(k_rows + ((16 * h + i) * kCols + column(16 * h + i, 4 * st + g)) * 16);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[h][x], core.q[st][x], s[h], 0, 0, 0);
+      }
+      if (here != ~0u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[h][r] = (here >> (16 * h + 4 * g + r) & 1) ? s[h][r] : -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[h][r]);
+      top = top == -INFINITY ? top : top * p.c;
+      if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float to = fmaxf(m, top);
+        const float f = to == m ? 1.f : exp2_fast(m - to);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < C::kTiles; ++t) acc[t] *= f;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      float w[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[h][r] = exp2_fast(fmaf(s[h][r], p.c, -ref));
+          l += w[h][r];
+        }
+      const char* v_rows = k_rows + kHalf;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned r = 16 * h + 4 * g + j;
+#pragma unroll
+          for (int x = 0; x < C::kWide; ++x) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(v_rows + (r * kCols + column(r, 16 * x + i)) * 16);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[4 * x + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t], w[h][j], acc[4 * x + t], 0, 0, 0);
+          }
+          if constexpr (C::kPair) {
+            const typename C::f32x2 v = *reinterpret_cast<const typename C::f32x2*>(
+                v_rows + (r * kCols + column(r, 16 * C::kWide + i / 2)) * 16 + 8 * (i % 2));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              acc[4 * C::kWide + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t], w[h][j], acc[4 * C::kWide + t], 0, 0, 0);
+          }
+        }
+    };
+    for (; kb < sk.n; kb += step, buf ^= 1) {
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (this step's rows are in LDS)
+      else __syncthreads();
+      const bool more = kb + step < sk.n;
+      const unsigned next = bits_of(kb + step, ahead);
+      if (more) {
+        ahead = byte_of(kb + 2 * step);
+        fetch(kb + step, next, buf ^ 1);   // (last read before the barrier above)
+      }
+      if (busy && valid) take(lds + buf * kBuf, valid);
+      if (more) keep(buf ^ 1);
+      valid = next;
+    }
+    __syncthreads();   // (a tile after this one writes the buffers again)
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (!busy) continue;
+    const int mine = wave * 16 + i;
+    float* to = out_row<float>(p, sq, b, kvh, row);
+    float scale = l == 0.f ? 0.f : 1.0f / l;
+    int d = a.d;
+    if (!whole) {   // this piece's part of the sums
+      const int64_t unit = ((int64_t)b * a.kv_heads + kvh) * p.tiles + tile;
+      float* ws = a.ws + (unit * p.splits + split) * kTileRows32 * (DP + 2);
+      if (g == 0) {
+        ws[mine] = m;
+        ws[kTileRows32 + mine] = l;
+      }
+      to = ws + 2 * kTileRows32 + mine * DP;
+      scale = 1.f;
+      d = DP;
+    }
+    if (to) store_row<C>(to, acc, scale, d, g);
+  }
+}
+
 // Joins the pieces of the tiles: a wave each row, the pieces' weights first (a lane each piece), then the pieces' sums, eight on
 // the way at a time.
 template <int TY, int DP, int ROWS>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   using E = typename Elem<TY>::type;
   const AttnArgs& a = p.a;
-  constexpr int kPiece = ROWS * (DP + 2), kPer = DP < 64 ? 1 : DP / 64;
+  constexpr int kPiece = ROWS * (DP + 2), kPer = (DP + 63) / 64;
   const int lane = threadIdx.x & 63, row = blockIdx.x % (ROWS / 4) * 4 + threadIdx.x / 64;
   const unsigned unit = blockIdx.x / (ROWS / 4);
   const int tile = unit % p.tiles, kvh = unit / p.tiles % a.kv_heads, b = unit / p.tiles / a.kv_heads;
@@ -759,32 +972,37 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     if (d + x < a.d) to[d + x] = (E)(o[x] * inv);
 }
 
-int padded_d(int type, int d) { return d > 64 ? 128 : d > 32 || type == T_F32 ? 64 : 32; }
+int padded_d(int type, int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 && type == T_F32 ? 96 : 128; }
 
 // How a launch is cut up.
 //   16-bit types  128-row tiles where a key head has more than 32 query rows, else 32-row tiles
-//   fp32          16-row tiles, eight waves each
-//   alone         16-row tiles, a wave each: with so few keys that a wave is done with them before a join would be (a 16-bit
-//                 type's key heads of at most 32 query rows, or fp32), or, fp32, tiles enough for two waves on each of 1024 SIMDs
-// and, where those leave CUs idle, pieces of the keys, each at least 512 long, up to two workgroups a CU.
+//   fp32          64-row tiles where a key head has more than 32 query rows and there is much to multiply, else 16-row tiles,
+//                 eight waves each (8 x 512 x 512, 16 heads of 64: 77 / 98 us; 1 x 512 x 512, 8 heads: 21 / 13, few workgroups
+//                 waiting for their chain of steps); heads of up to 32 are quicker without LDS (41 x 70 x 1668: 195 / 178)
+//   alone         16-row tiles, a wave each: so few keys that a wave is done with them before a join would be (16-bit types: and
+//                 at most 32 query rows a key head), or, fp32, tiles enough for two waves on each of 1024 SIMDs
+// and, where those leave CUs idle, pieces of the keys, each at least 256 long, up to what the CUs hold at once (one more in a
+// round of its own: 1 x 686 x 6136, 4 heads over 1 of 80, fp32: 473 workgroups 74 us, 516 98).
 enum class Way { kAlone, kRows, kFew, kTile };
 struct Plan {
   Way way;
   int tiles, splits, rows;
   int64_t units;
 };
-Plan plan(int type, int batch, int heads, int kv_heads, int max_q, int max_k) {
+Plan plan(int type, int batch, int heads, int kv_heads, int d, int max_q, int max_k) {
   Plan p;
   const int64_t rows = (int64_t)max_q * (heads / kv_heads);
   const int64_t sixteens = (rows + kRows - 1) / kRows * batch * kv_heads;
-  if (type == T_F32) p.way = max_k <= 128 || sixteens >= 2048 ? Way::kAlone : Way::kRows;
-  else p.way = rows > kFewRows ? Way::kTile : max_k <= 128 ? Way::kAlone : Way::kFew;
-  p.rows = p.way == Way::kTile ? kTileRows : p.way == Way::kFew ? kFewRows : kRows;
+  const bool much = max_k <= 128 || (double)rows * batch * kv_heads * max_k * d >= 1 << 28;
+  if (rows > kFewRows && (type != T_F32 || (d > 32 && much))) p.way = Way::kTile;
+  else if (type == T_F32) p.way = max_k <= 128 || sixteens >= 2048 ? Way::kAlone : Way::kRows;
+  else p.way = max_k <= 128 ? Way::kAlone : Way::kFew;
+  p.rows = p.way == Way::kTile ? (type == T_F32 ? kTileRows32 : kTileRows) : p.way == Way::kFew ? kFewRows : kRows;
   const int64_t tiles = (rows + p.rows - 1) / p.rows, most = ((int64_t)1 << 22) / ((int64_t)batch * kv_heads) + 1;
   p.tiles = (int)(tiles < most ? tiles : most);   // (a grid holds below 2^32 threads; workgroups loop over the rest)
   p.units = (int64_t)p.tiles * batch * kv_heads;
-  int64_t n = p.units && p.way != Way::kAlone ? (512 + p.units - 1) / p.units : 1;
-  const int64_t pieces = (int64_t)max_k / 512;
+  int64_t n = p.units && p.way != Way::kAlone ? (p.way == Way::kRows ? 256 : 512) / p.units : 1;
+  const int64_t pieces = (int64_t)max_k / 256;
   n = n < pieces ? n : pieces;
   p.splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
   return p;
@@ -804,13 +1022,20 @@ hipError_t run(const AttnParams& p, const Plan& n, hipStream_t s) {
     attn_rows_kernel<TY, DP, 1><<<dim3((unsigned)((p.units + 3) / 4)), 256, 0, s>>>(p);
     return hipGetLastError();
   }
+  const AttnArgs& a = p.a;
+  constexpr int kBytes = sizeof(typename Elem<TY>::type);
+  const bool dma = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                     kBytes * (a.k_ts | a.k_hs | a.v_ts | a.v_hs | (a.k_offsets ? 0 : a.k_bs | a.v_bs))) & 15) == 0;
   if constexpr (TY == T_F32) {
+    if constexpr (DP > 32)
+      if (n.way == Way::kTile) {
+        if (dma) attn_tile32_kernel<DP, true><<<grid, 256, 0, s>>>(p);
+        else attn_tile32_kernel<DP, false><<<grid, 256, 0, s>>>(p);
+        return join<TY, DP, kTileRows32>(p, s);
+      }
     attn_rows_kernel<TY, DP, 8><<<grid, 512, 0, s>>>(p);
     return join<TY, DP, kRows>(p, s);
   } else {
-    const AttnArgs& a = p.a;
-    const bool dma = ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | 2 * (a.k_ts | a.k_hs | a.v_ts | a.v_hs) |
-                       (a.k_offsets ? 0 : 2 * (a.k_bs | a.v_bs))) & 15) == 0;
     if (n.way == Way::kTile) {
       if (dma) attn_tile_kernel<TY, DP, 1, true><<<grid, 256, 0, s>>>(p);
       else attn_tile_kernel<TY, DP, 1, false><<<grid, 256, 0, s>>>(p);
@@ -826,17 +1051,21 @@ hipError_t run(const AttnParams& p, const Plan& n, hipStream_t s) {
 
 int64_t attention_workspace(int type, int batch, int heads, int kv_heads, int d, int max_q, int max_k) {
   if (batch == 0) return 0;
-  const Plan p = plan(type, batch, heads, kv_heads, max_q, max_k);
+  const Plan p = plan(type, batch, heads, kv_heads, d, max_q, max_k);
   return p.splits == 1 ? 0 : p.units * p.splits * p.rows * (padded_d(type, d) + 2) * 4;
 }
 
 hipError_t launch_attention(int type, const AttnArgs& a, hipStream_t s) {
-  const Plan n = plan(type, a.batch, a.heads, a.kv_heads, a.max_q, a.max_k);
+  const Plan n = plan(type, a.batch, a.heads, a.kv_heads, a.d, a.max_q, a.max_k);
   // (never 0: a masked score of -inf stays one)
   const float c = fmaxf((float)(fabs((double)a.scale) * 1.4426950408889634), __FLT_DENORM_MIN__);
   const AttnParams p{a, c, a.scale < 0, (unsigned)(a.heads / a.kv_heads), (unsigned)n.tiles, (unsigned)n.units, (unsigned)n.splits};
   const int dp = padded_d(type, a.d);
-  if (type == T_F32) return dp == 64 ? run<T_F32, 64>(p, n, s) : run<T_F32, 128>(p, n, s);
+  if (type == T_F32)
+    return dp == 32   ? run<T_F32, 32>(p, n, s)
+           : dp == 64 ? run<T_F32, 64>(p, n, s)
+           : dp == 96 ? run<T_F32, 96>(p, n, s)
+                      : run<T_F32, 128>(p, n, s);
   if (type == T_BF16) return dp == 32 ? run<T_BF16, 32>(p, n, s) : dp == 64 ? run<T_BF16, 64>(p, n, s) : run<T_BF16, 128>(p, n, s);
   return dp == 32 ? run<T_F16, 32>(p, n, s) : dp == 64 ? run<T_F16, 64>(p, n, s) : run<T_F16, 128>(p, n, s);
 }

@@ -474,6 +474,37 @@ def test_attention_scales_signs_and_holes(ops, dtype, lq, lk, h, hkv, d):
         check_attention(got, q, k, v, there, scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("b,lq,lk,h,hkv,d", [(1, 700, 1500, 4, 1, 80), (2, 130, 2100, 8, 8, 64), (1, 260, 3001, 4, 4, 128),
+                                             (1, 2100, 501, 4, 4, 64), (3, 65, 90, 4, 2, 104), (2, 300, 2000, 8, 4, 32)])
+def test_attention_much_to_multiply(ops, dtype, b, lq, lk, h, hkv, d):
+    """Many rows and many keys, where tiles of rows share keys and pieces of the keys are joined: a mask with holes, a sequence
+    without keys, keys at odd elements; packed, with launches sized for less."""
+    g = gen(lq + lk + d)
+    q, k, v = qkv(g, b + 1, lq, lk, h, hkv, d, dtype)
+    there = torch.rand(b + 1, lk, generator=g) < 0.8
+    there[0, : lk // 2] = False
+    there[b] = False
+    k2 = torch.full((b + 1, lk, hkv, d + 1), float("nan"), dtype=dtype)
+    k2[..., 1:][there] = k[there]
+    v2 = torch.where(there[..., None, None], v, torch.full((), float("inf"), dtype=dtype))
+    got = ops.cross_attention(q.cuda(), k2.cuda()[..., 1:], v2.cuda(), key_mask=there.cuda(), scale=-0.11)
+    assert (got[b] == 0).all()
+    check_attention(got, q, k, v, there, -0.11)
+    aligned = ops.cross_attention(q.cuda(), k2[..., 1:].contiguous().cuda(), v2.cuda(), key_mask=there.cuda(), scale=-0.11)
+    assert torch.equal(aligned, got)
+    ql, kl = [0, lq, lq // 3], [7, lk // 2, lk]
+    qo, ko = (torch.tensor([0] + n).cumsum(0).to(torch.int32) for n in (ql, kl))
+    q, k, v = rand(g, sum(ql), h, d).to(dtype), rand(g, sum(kl), hkv, d).to(dtype), rand(g, sum(kl), hkv, d).to(dtype)
+    for max_q, max_k in ((lq, lk), (lq // 4, 2 * lk), (lq, 200)):
+        got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), q_offsets=qo.cuda(), k_offsets=ko.cuda(), max_q=max_q,
+                                  max_k=max_k)
+        for i in range(3):
+            x, y = slice(qo[i], qo[i + 1]), slice(ko[i], ko[i + 1])
+            want, err = plain.attention(q[x], k[y], v[y], torch.ones(kl[i], dtype=torch.bool), d ** -0.5)
+            plain.within(got[x], want, err, dtype)
+
+
 def test_attention_no_keys_no_queries(ops):
     q = torch.ones(2, 3, 2, 16).cuda()
     kv = torch.ones(2, 0, 2, 16).cuda()
