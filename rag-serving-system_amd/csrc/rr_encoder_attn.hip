@@ -45,6 +45,29 @@ __device__ __forceinline__ Span keys_of(const AttnArgs& a, int b) {
   return s;
 }
 
+// Keys of a mask's row up to the last one that takes part: a padded batch's masks end long before their rows do, and a step
+// without keys costs a wave nearly what one with keys waits for. 1024 keys at a time from the end, 16 a lane, as dwords
+// (none that holds no byte of the row).
+__device__ __forceinline__ int mask_end(const uint8_t* mask, int n) {
+  const int lane = threadIdx.x & 63, sh = (int)(reinterpret_cast<uintptr_t>(mask) & 3);   // byte 0 of the row in the buffer
+  const auto row = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(mask - sh), 0, (sh + n + 3) & ~3, 0x00020000);
+  for (int c0 = n > 0 ? (sh + n - 1) & ~1023 : -1; c0 >= 0; c0 -= 1024) {
+    const int at = c0 + 16 * lane;
+    const u32x4 bytes = __builtin_amdgcn_raw_buffer_load_b128(row, at, 0, 0);
+    int last = -1;   // this lane's last byte that is set, counted in the buffer
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int left = sh + n - (at + 4 * j);   // bytes of this dword before the row's end
+      unsigned v = left >= 4 ? bytes[j] : left <= 0 ? 0u : bytes[j] & ((1u << 8 * left) - 1);
+      if (at + 4 * j < sh) v &= ~0u << 8 * sh;
+      if (v) last = at + 4 * j + (31 - __builtin_clz(v)) / 8;
+    }
+    const uint64_t any = __ballot(last >= 0);
+    if (any) return __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(any)) - sh + 1;
+  }
+  return 0;
+}
+
 // Rows [first, first + count) of a tensor whose rows lie `ts` elements apart, as a buffer: reads behind the last row's end give
 // zeros, so that no lane has to ask whether its key is there, and 32-bit offsets reach every row of a block of keys (the
 // caller keeps ts below 2^23).
@@ -294,11 +317,13 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
   const int split = WK == 1 ? 0 : blockIdx.x % p.splits;
   if (unit >= p.units) return;
   const int tile0 = unit % p.tiles, kvh = unit / p.tiles % a.kv_heads, b = unit / p.tiles / a.kv_heads;
-  const Span sq = queries_of(a, b), sk = keys_of(a, b);
+  const Span sq = queries_of(a, b);
+  Span sk = keys_of(a, b);
   const int rows = sq.n * p.group;
   const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
   const E* vbase = static_cast<const E*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
   const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+  if (mask) sk.n = mask_end(mask, sk.n);
 
   // tiles behind the ones the launch was sized for (a sequence longer than max_q) take all keys in one piece
   const unsigned k_ts = (unsigned)a.k_ts, v_ts = (unsigned)a.v_ts;
@@ -471,11 +496,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
   const int split = at % p.splits, tile0 = at / p.splits % p.tiles;
   const int kvh = at / each % a.kv_heads, b = at / each / a.kv_heads;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), i = lane & 31, half = lane >> 5;
-  const Span sq = queries_of(a, b), sk = keys_of(a, b);
+  const Span sq = queries_of(a, b);
+  Span sk = keys_of(a, b);
   const int rows = sq.n * p.group;
   const E* kbase = static_cast<const E*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
   const E* vbase = static_cast<const E*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
   const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+  if (mask) sk.n = mask_end(mask, sk.n);
   // A step's keys as bits. The mask's bytes are asked for two steps ahead, before that step's rows, so that nothing waits
   // for more than the bytes themselves.
   struct Bytes {
@@ -750,11 +777,13 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 4) void attn_tile32_kernel(AttnP
   const int split = at % p.splits, tile0 = at / p.splits % p.tiles;
   const int kvh = at / each % a.kv_heads, b = at / each / a.kv_heads;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-  const Span sq = queries_of(a, b), sk = keys_of(a, b);
+  const Span sq = queries_of(a, b);
+  Span sk = keys_of(a, b);
   const int rows = sq.n * p.group;
   const float* kbase = static_cast<const float*>(a.k) + (a.k_offsets ? sk.first * a.k_ts : b * a.k_bs) + kvh * a.k_hs;
   const float* vbase = static_cast<const float*>(a.v) + (a.k_offsets ? sk.first * a.v_ts : b * a.v_bs) + kvh * a.v_hs;
   const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+  if (mask) sk.n = mask_end(mask, sk.n);
   auto byte_of = [&](int kb) -> unsigned char { return mask && lane < 32 && kb + lane < sk.n ? mask[kb + lane] : 1; };
   auto bits_of = [&](int kb, unsigned char there) { return (unsigned)__ballot(lane < 32 && kb + lane < sk.n && there); };
   auto column = [](unsigned r, unsigned c) { return c ^ (DP % 64 ? r / 2 % 8 : r % 16); };

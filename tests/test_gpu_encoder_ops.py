@@ -505,6 +505,25 @@ def test_attention_much_to_multiply(ops, dtype, b, lq, lk, h, hkv, d):
             plain.within(got[x], want, err, dtype)
 
 
+@pytest.mark.parametrize("lq", [1, 7, 50])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=str)
+def test_attention_masks_that_end_anywhere(ops, dtype, lq):
+    """A padded batch's masks, rows at any byte: they give what the lengths give, whatever lies behind the last key."""
+    g = gen(lq)
+    ends = [0, 1, 2, 3, 4, 5, 15, 16, 17, 63, 64, 65, 1020, 1021, 1022, 1023, 1024, 1025, 2047, 2049, 2051]
+    b, lk, h, d = len(ends), 2051, 2, 64
+    q, k, v = (t.cuda() for t in qkv(g, b, lq, lk, h, h, d, dtype))
+    lens = torch.tensor(ends, dtype=torch.int32).cuda()
+    want = ops.cross_attention(q, k, v, key_lengths=lens)
+    there = (torch.arange(lk) < torch.tensor(ends)[:, None])
+    k, v = (torch.where(there.cuda()[..., None, None], t, torch.full((), float("nan"), dtype=dtype).cuda()) for t in (k, v))
+    for off, wide in ((0, lk), (1, lk + 1), (2, lk + 2), (3, lk + 4)):
+        mask = torch.ones(b, wide + 3, dtype=torch.uint8)
+        mask[:, off:off + lk] = there * 7
+        got = ops.cross_attention(q, k, v, key_mask=mask.cuda()[:, off:off + lk])
+        assert torch.equal(got, want)
+
+
 def test_attention_no_keys_no_queries(ops):
     q = torch.ones(2, 3, 2, 16).cuda()
     kv = torch.ones(2, 0, 2, 16).cuda()
