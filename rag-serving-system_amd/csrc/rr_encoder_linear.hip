@@ -10,8 +10,7 @@ namespace {
 // ---- rows at any address ---------------------------------------------------------------------------------------------
 // Rows of `k` bytes that may start anywhere, `ld` apart, as a buffer of dwords: the loads' addresses are multiples of four
 // (16-byte loads at odd ones take 128 cycles an instruction here, which made 48 rows of 3769 take 20 us), and what lies behind
-// the last row is read as zeros. Rows are less than RR_LINEAR_LDMOST = 2^22 bytes apart and at
-// most 513 here: offsets below 2^32.
+// the last row is read as zeros. Rows are less than RR_LINEAR_LDMOST = 2^22 bytes apart and at most 514 here: offsets below 2^32.
 struct RowBytes {
   __amdgpu_buffer_rsrc_t r;
   unsigned first, ld;   // first: where row 0 starts in the buffer

@@ -203,8 +203,8 @@ hipError_t run(NormArgs a, hipStream_t s) {
   if (chunks <= 64 * 2) return go(block_norm_kernel<TY, 1, 2>, 1);
   if (chunks <= 64 * 4) return go(block_norm_kernel<TY, 1, 4>, 1);
   if (chunks <= 64 * 8) return go(block_norm_kernel<TY, 4, 2>, 4);
-  if (chunks <= 64 * 16) return go(block_norm_kernel<TY, 4, 4>, 4);
-  if (chunks <= 64 * 32) return go(block_norm_kernel<TY, 8, 4>, 8);
+  if (chunks <= 64 * 16) return go(block_norm_kernel<TY, 8, 2>, 8);
+  if (chunks <= 64 * 32) return go(block_norm_kernel<TY, 16, 2>, 16);
   const size_t lds = (size_t)a.cols * 4;
   auto wide = block_norm_wide_kernel<TY>;
   if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(wide), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds))

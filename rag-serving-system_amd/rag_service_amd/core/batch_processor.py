@@ -13,8 +13,7 @@ SURVEY.md §8a row a8), same result/error conventions. Differences, all on the r
 * the LLM prompt list is passed directly (the reference wraps it in ``datasets.Dataset`` only to read
   the same list back, :104-105).
 
-The embedding half (e5 forward) is PyTorch-ROCm by default, as BASELINE config 4 specifies; its semantics are kept
-exactly: "query: " prefix, tokenizer(padding=True, truncation=True), ``last_hidden_state.mean(dim=1)``
+The embedding half (e5 forward) is PyTorch-ROCm by default; its semantics are kept exactly: "query: " prefix, tokenizer(padding=True, truncation=True), ``last_hidden_state.mean(dim=1)``
 over ALL positions (pad tokens included, no attention-mask weighting) and no L2 normalisation
 (:83-91).
 """
