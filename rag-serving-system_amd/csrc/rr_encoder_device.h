@@ -47,12 +47,21 @@ constexpr int64_t kCacheBytes = 32 << 20;   // eight XCDs' L2 of 4 MiB
 
 // Sums and maxima over the W waves of a row, every lane gets them. `red`: LDS words, 2 W for each row of the workgroup, used
 // in turn (the first half, the second, ...): one barrier a call, since a half is written again only after a barrier that
-// follows its last reads.
-template <int W>
+// follows its last reads. A short row (W = 1) may have G lanes of a wave only, aligned.
+template <int W, int G = 64>
 struct RowReduce {
+  static_assert(W == 1 || G == 64, "whole waves");
   float* red;
   int turn = 0;
   __device__ __forceinline__ float sum(float v) {
+    if constexpr (G < 64) {
+      v = dpp_add_f32<0xB1>(v);                         // quad_perm [1,0,3,2]
+      v = dpp_add_f32<0x4E>(v);                         // quad_perm [2,3,0,1]
+      v = dpp_add_f32<0x141>(v);                        // row_half_mirror
+      if constexpr (G >= 16) v = dpp_add_f32<0x140>(v); // row_mirror
+      if constexpr (G >= 32) v += __shfl_xor(v, 16);
+      return v;
+    }
     v = wave_sum_f32(v);
     if constexpr (W == 1) return v;
     float* r = put(v);
@@ -62,6 +71,14 @@ struct RowReduce {
     return s;
   }
   __device__ __forceinline__ unsigned max(unsigned v) {
+    if constexpr (G < 64) {
+      v = group_max_u32<(G < 16 ? G : 16)>(v);
+      if constexpr (G >= 32) {
+        const unsigned t = __shfl_xor(v, 16);
+        v = v > t ? v : t;
+      }
+      return v;
+    }
     v = wave_max_u32(v);
     if constexpr (W == 1) return v;
     float* r = put(__uint_as_float(v));

@@ -81,28 +81,28 @@ __global__ __launch_bounds__(256) void repack_kernel(Repack one, Repack two, int
 }
 
 // ---- 8-bit rows ----------------------------------------------------------------------------------------------------
-// A row in the registers of W waves, S times 16 bytes a lane; W = 1: four rows a workgroup. cols_pad: columns written, zeros
-// behind the row's own. Bandwidth: 16384 x 4096 bf16 46 us, 4.4 TB/s (of 5.2 that a large copy reaches; a wave a row instead of
+// A row in the registers of W waves, or of G lanes of one, S times 16 bytes a lane. cols_pad: columns written, zeros behind the
+// row's own. Bandwidth: 16384 x 4096 bf16 46 us, 4.4 TB/s (of 5.2 that a large copy reaches; a wave a row instead of
 // four changes nothing).
-template <int TY, int W, int S>
+template <int TY, int W, int S, int G = 64>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_rows_kernel(const void* xv, int64_t ldx, int64_t rows,
                                                                              int cols, int cols_pad, int8_t* q, int64_t ldq,
                                                                              float* scale, unsigned blocks, Repack also) {
   using E = typename Elem<TY>::type;
-  constexpr int N = Chunk<E>::N, kGroups = W == 1 ? 4 : 1;
+  constexpr int N = Chunk<E>::N, kLanes = W == 1 ? G : 64 * W, kGroups = W == 1 ? 256 / G : 1;
   if (blockIdx.x >= blocks) {
     const int64_t all = also.blocks(blockDim.x);
     for (int64_t b = blockIdx.x - blocks; b < all; b += gridDim.x - blocks) repack(also, b);
     return;
   }
   __shared__ float red[2 * W];
-  RowReduce<W> over{red};
-  const int t = threadIdx.x % (64 * W);
-  for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / (64 * W); r < rows; r += (int64_t)blocks * kGroups) {
+  RowReduce<W, G> over{red};
+  const int t = threadIdx.x % kLanes;
+  for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes; r < rows; r += (int64_t)blocks * kGroups) {
     const E* x = static_cast<const E*>(xv) + r * ldx;
     Chunk<E> c[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) c[s].load(x + (s * 64 * W + t) * N, cols - (s * 64 * W + t) * N);
+    for (int s = 0; s < S; ++s) c[s].load(x + (s * kLanes + t) * N, cols - (s * kLanes + t) * N);
     unsigned m = 0;
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_rows_kernel(co
       float v[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = sc == sc ? c[s][i] : 0.f;
-      store_i8<N>(q + r * ldq + (s * 64 * W + t) * N, v, div, cols_pad - (s * 64 * W + t) * N);
+      store_i8<N>(q + r * ldq + (s * kLanes + t) * N, v, div, cols_pad - (s * kLanes + t) * N);
     }
     if (t == 0) scale[r] = sc;
   }
@@ -558,13 +558,16 @@ template <int TY>
 hipError_t quantize(const void* x, int64_t ldx, int64_t rows, int cols, int cols_pad, int8_t* q, int64_t ldq, float* scale,
                     const Repack& also, hipStream_t s) {
   constexpr int N = Chunk<typename Elem<TY>::type>::N;
-  auto go = [&](auto kernel, int waves) {
-    const int groups = waves == 1 ? 4 : 1, threads = 64 * waves * groups;
+  auto go = [&](auto kernel, int waves, int lanes = 64) {
+    const int groups = waves == 1 ? 256 / lanes : 1, threads = waves == 1 ? 256 : 64 * waves;
     const unsigned blocks = grid_of((rows + groups - 1) / groups).x, more = (unsigned)std::min<int64_t>(also.blocks(threads), 1 << 16);
     kernel<<<dim3(blocks + more), threads, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale, blocks, also);
     return hipGetLastError();
   };
   const int chunks = (cols_pad + N - 1) / N;
+  if (chunks <= 8) return go(quantize_rows_kernel<TY, 1, 1, 8>, 1, 8);
+  if (chunks <= 16) return go(quantize_rows_kernel<TY, 1, 1, 16>, 1, 16);
+  if (chunks <= 32) return go(quantize_rows_kernel<TY, 1, 1, 32>, 1, 32);
   if (chunks <= 64) return go(quantize_rows_kernel<TY, 1, 1>, 1);
   if (chunks <= 64 * 2) return go(quantize_rows_kernel<TY, 1, 2>, 1);
   if (chunks <= 64 * 4) return go(quantize_rows_kernel<TY, 1, 4>, 1);

@@ -6,22 +6,22 @@ namespace enc {
 namespace {
 
 // Bandwidth is all there is to it: a row is read once, stays in the registers of its W waves in fp32 (S times 16 bytes of
-// its type a lane; W = 1: four rows a workgroup, no barriers), and each result is written once. The variance is a second sum
+// its type a lane; W = 1: no barriers, and a short row has G lanes of a wave), and each result is written once. The variance is a second sum
 // over the registers, of centred values. Workgroups loop over rows, so that weights and biases are loaded once each.
 // 32768 x 4096 bf16, norms on both sides, 211 us: 5.1 TB/s, what a large copy reaches; 4097 x 1001 fp32 (rows at odd
 // addresses) 13.0 us, 5.05 TB/s; 613 x 1024 with 8-bit rows 4.2 us, a launch and four memory and reduction latencies.
-template <int TY, int W, int S>
+template <int TY, int W, int S, int G = 64>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void block_norm_kernel(NormArgs a) {
   using E = typename Elem<TY>::type;
-  constexpr int N = Chunk<E>::N, kGroups = W == 1 ? 4 : 1;
+  constexpr int N = Chunk<E>::N, kLanes = W == 1 ? G : 64 * W, kGroups = W == 1 ? 256 / G : 1;
   __shared__ float red[2 * W];
-  RowReduce<W> over{red};
-  const int t = threadIdx.x % (64 * W), cols = a.cols;
+  RowReduce<W, G> over{red};
+  const int t = threadIdx.x % kLanes, cols = a.cols;
 
   auto vector = [&](Chunk<E>* c, const void* p, float none) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int at = (s * 64 * W + t) * N;
+      const int at = (s * kLanes + t) * N;
       if (p) c[s].load(static_cast<const E*>(p) + at, cols - at);
       else c[s].fill(none);
     }
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void block_norm_kernel(NormA
     for (int s = 0; s < S; ++s)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        v[s][i] = (s * 64 * W + t) * N + i < cols ? v[s][i] - mean : 0.f;
+        v[s][i] = (s * kLanes + t) * N + i < cols ? v[s][i] - mean : 0.f;
         sum = fmaf(v[s][i], v[s][i], sum);
       }
     const float r = 1.0f / sqrtf(over.sum(sum) / (float)cols + a.eps);
@@ -71,11 +71,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void block_norm_kernel(NormA
       for (int i = 0; i < N; ++i) v[s][i] = fmaf(v[s][i] * r, w[s][i], b[s][i]);
   };
 
-  for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / (64 * W); r < a.rows; r += (int64_t)gridDim.x * kGroups) {
+  for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes; r < a.rows; r += (int64_t)gridDim.x * kGroups) {
     Chunk<E> y[S], x[S], g[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int at = (s * 64 * W + t) * N;
+      const int at = (s * kLanes + t) * N;
       y[s].load(static_cast<const E*>(a.y) + r * a.ldy + at, cols - at);
       if (a.x) x[s].load(static_cast<const E*>(a.x) + r * a.ldx + at, cols - at);
     }
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void block_norm_kernel(NormA
     if (a.post) norm(v, a.post, pw, pb, a.post_w, a.post_b);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int at = (s * 64 * W + t) * N;
+      const int at = (s * kLanes + t) * N;
       if (a.gate)
 #pragma unroll
         for (int i = 0; i < N; ++i) v[s][i] *= g[s][i];
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void block_norm_kernel(NormA
     if (a.normed)
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const int at = (s * 64 * W + t) * N;
+        const int at = (s * kLanes + t) * N;
         store_chunk(static_cast<E*>(a.normed) + r * a.ldn + at, v[s], cols - at, a.past);
       }
     if (!a.q) continue;
@@ -111,14 +111,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void block_norm_kernel(NormA
     for (int s = 0; s < S; ++s)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if ((s * 64 * W + t) * N + i >= cols) v[s][i] = 0.f;
+        if ((s * kLanes + t) * N + i >= cols) v[s][i] = 0.f;
         m = mag(v[s][i]) > m ? mag(v[s][i]) : m;
       }
     const float sc = row_scale(over.max(m));
     const float div = row_divisor(sc);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int at = (s * 64 * W + t) * N;
+      const int at = (s * kLanes + t) * N;
 #pragma unroll
       for (int i = 0; i < N; ++i) v[s][i] = sc == sc ? v[s][i] : 0.f;
       store_i8<N>(a.q + r * a.ldq + at, v[s], div, cols - at);
@@ -192,18 +192,25 @@ hipError_t run(NormArgs a, hipStream_t s) {
   // with plain stores, 212 so; 4097 x 1001 fp32 14.9 and 13.0). Below that the next operator finds them in L2.
   const int64_t values = (1 + (a.x != nullptr) + (a.stream != nullptr) + (a.normed != nullptr)) * a.rows * a.cols;
   a.past = values * (int64_t)sizeof(typename Elem<TY>::type) > kCacheBytes;
-  auto go = [&](auto kernel, int waves) {
-    const int groups = waves == 1 ? 4 : 1;
+  auto go = [&](auto kernel, int waves, int lanes = 64) {
+    const int groups = waves == 1 ? 256 / lanes : 1;
     const int64_t wgs = (a.rows + groups - 1) / groups, most = 256 * 8;
-    kernel<<<dim3((unsigned)(wgs < most ? wgs : most)), 64 * waves * groups, 0, s>>>(a);
+    kernel<<<dim3((unsigned)(wgs < most ? wgs : most)), waves == 1 ? 256 : 64 * waves, 0, s>>>(a);
     return hipGetLastError();
   };
+  // Lanes in proportion to the row, so that few idle (16000 x 192 bf16 with 8-bit rows: a wave a row 14.6 us, half a wave 9.8;
+  // x 50 14.2, with eight lanes 5.1; 2712 x 4608 with both norms and 8-bit rows: 1024 lanes' room 50 us, 768 43)
   const int chunks = (a.cols + N - 1) / N;
+  if (chunks <= 8) return go(block_norm_kernel<TY, 1, 1, 8>, 1, 8);
+  if (chunks <= 16) return go(block_norm_kernel<TY, 1, 1, 16>, 1, 16);
+  if (chunks <= 32) return go(block_norm_kernel<TY, 1, 1, 32>, 1, 32);
   if (chunks <= 64) return go(block_norm_kernel<TY, 1, 1>, 1);
   if (chunks <= 64 * 2) return go(block_norm_kernel<TY, 1, 2>, 1);
   if (chunks <= 64 * 4) return go(block_norm_kernel<TY, 1, 4>, 1);
   if (chunks <= 64 * 8) return go(block_norm_kernel<TY, 4, 2>, 4);
+  if (chunks <= 64 * 12) return go(block_norm_kernel<TY, 3, 4>, 3);
   if (chunks <= 64 * 16) return go(block_norm_kernel<TY, 8, 2>, 8);
+  if (chunks <= 64 * 24) return go(block_norm_kernel<TY, 12, 2>, 12);
   if (chunks <= 64 * 32) return go(block_norm_kernel<TY, 16, 2>, 16);
   const size_t lds = (size_t)a.cols * 4;
   auto wide = block_norm_wide_kernel<TY>;
