@@ -1030,7 +1030,12 @@ Plan plan(int type, int batch, int heads, int kv_heads, int d, int max_q, int ma
   const int64_t tiles = (rows + p.rows - 1) / p.rows, most = ((int64_t)1 << 22) / ((int64_t)batch * kv_heads) + 1;
   p.tiles = (int)(tiles < most ? tiles : most);   // (a grid holds below 2^32 threads; workgroups loop over the rest)
   p.units = (int64_t)p.tiles * batch * kv_heads;
-  int64_t n = p.units && p.way != Way::kAlone ? (p.way == Way::kRows ? 256 : 512) / p.units : 1;
+  // What 256 CUs hold at once; tiles of short heads are four a CU, which 16-bit types' need only where two would leave many of
+  // them empty (14 x 83 x 3593, 32 heads over 8 of 64, lengths from 31: 66 us whole, 61 in pieces; 8 x 128 x 2000, 16 heads:
+  // four pieces 27.5, seven 29.6; fp32 11 x 251 x 4844, 8 heads: 302 with one, 230 with two).
+  const bool four = p.way == Way::kTile && d <= 64 && (type == T_F32 || p.units > 256);
+  const int at_once = p.way == Way::kRows ? 256 : four ? 1024 : 512;
+  int64_t n = p.units && p.way != Way::kAlone ? at_once / p.units : 1;
   const int64_t pieces = (int64_t)max_k / 256;
   n = n < pieces ? n : pieces;
   p.splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
