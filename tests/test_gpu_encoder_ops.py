@@ -646,6 +646,47 @@ def test_everything_in_a_graph_first(ops):
             assert torch.equal(y, v) and torch.equal(z, v)
 
 
+def test_copies_and_tiles_in_a_graph(ops):
+    """The products that copy odd rows into scratch memory and fp32 attention in tiles and pieces, captured twice: the graphs
+    share no scratch memory, and every replay equals the eager result bit for bit."""
+    g = gen(15)
+    w = torch.randint(-127, 128, (2300, 1001), generator=g, dtype=torch.int8).cuda()
+    sw = torch.rand(2300, generator=g).cuda() / 1000
+    q8 = torch.randint(-127, 128, (1100, 1001), generator=g, dtype=torch.int8).cuda()
+    xs = [rand(g, 300, 1001).to(torch.bfloat16).cuda() for _ in range(4)]
+    kv = [rand(g, 1, 1100, 4, 80).cuda() for _ in range(4)]
+    q = rand(g, 1, 900, 4, 80).cuda()
+    mask = (torch.rand(1, 1100, generator=g) < 0.9).cuda()
+
+    def run(x, s, k):
+        return (ops.linear_int8(x, w, sw, act="gelu"), ops.linear_int8(q8, w, sw, x_scale=s), ops.quantize_rows(x)[0],
+                ops.cross_attention(q, k, k, key_mask=mask))
+
+    scales = [torch.rand(1100, generator=g).cuda() for _ in range(4)]
+    want = [run(xs[i], scales[i], kv[i]) for i in range(4)]
+    ins = [[xs[0].clone(), scales[0].clone(), kv[0].clone()] for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs = []
+    for a in ins:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = run(*a)
+        graphs.append((graph, y))
+    for i in range(4):
+        for j, a in enumerate(ins):
+            for t, u in zip(a, (xs[(i + j) % 4], scales[(i + j) % 4], kv[(i + j) % 4])):
+                t.copy_(u)
+        graphs[0][0].replay()
+        graphs[1][0].replay()
+        again = run(xs[i], scales[i], kv[i])
+        torch.cuda.synchronize()
+        for j in range(2):
+            for y, v in zip(graphs[j][1], want[(i + j) % 4]):
+                assert torch.equal(y, v)
+        for y, v in zip(again, want[i]):
+            assert torch.equal(y, v)
+
+
 # ---- the C-ABI itself -----------------------------------------------------------------------------------------------
 
 def test_abi_leaves_other_rows_alone_and_works_in_place(ops):
@@ -691,6 +732,45 @@ def test_abi_leaves_other_rows_alone_and_works_in_place(ops):
     with pytest.raises(Exception, match="device"):
         _lib._check(lib.rr_quantize_rows(99, None, 0, q.data_ptr(), 200, 6, 200, wide.data_ptr(), 300, scale.data_ptr()))
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("cols", [7, 50, 100, 200, 700, 1500, 4608, 9000, 20000])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_abi_norm_in_place(ops, dtype, cols):
+    """The stream over the residual and the normed rows over the block's output, at every number of lanes a row."""
+    from rag_service_amd import _lib
+    lib, g, rows = _lib.load_library(), gen(cols), 37
+    x, y = rand(g, rows, cols).to(dtype).cuda(), rand(g, rows, cols).to(dtype).cuda()
+    r = ops.block_norm(y, x, residual_scale=0.5, rows8=True)
+    q, sc = torch.empty_like(r.rows8), torch.empty_like(r.scale)
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    rc = lib.rr_block_norm(0, torch.cuda.current_stream().cuda_stream, code, rows, cols, y.data_ptr(), cols, x.data_ptr(), cols,
+                           0.5, None, 0, 0, 1, 0, None, None, 1, None, None, 1e-5, x.data_ptr(), cols, y.data_ptr(), cols,
+                           q.data_ptr(), cols, sc.data_ptr())
+    assert rc == 0, lib.rr_last_error()
+    assert torch.equal(x, r.stream) and torch.equal(y, r.normed) and torch.equal(q, r.rows8) and torch.equal(sc, r.scale)
+
+
+def test_abi_copied_product_leaves_other_columns_alone(ops):
+    """Odd inner sizes: results of a wider matrix, scratch memory of exactly the size asked for with guards behind it."""
+    from rag_service_amd import _lib
+    lib, g = _lib.load_library(), gen(21)
+    stream = torch.cuda.current_stream().cuda_stream
+    for code, m, n, k in ((3, 1500, 1600, 1001), (1, 60, 70, 33), (0, 333, 500, 1003), (2, 700, 90, 2050)):
+        dtype = (torch.float32, torch.bfloat16, torch.float16, torch.int8)[code]
+        x = torch.randint(-127, 128, (m, k), generator=g).to(dtype).cuda() if code == 3 else rand(g, m, k).to(dtype).cuda()
+        w, sw, b = (t.cuda() for t in weights(g, n, k))
+        sx = torch.rand(m, generator=g).cuda()
+        out = torch.full((m, n + 7), 5.0, device="cuda")
+        need = lib.rr_linear_i8_workspace(code, m, n, k)
+        assert need > 0
+        ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+        rc = lib.rr_linear_i8(0, stream, code, x.data_ptr(), k, sx.data_ptr() if code == 3 else None, w.data_ptr(), k,
+                              sw.data_ptr(), b.data_ptr(), 1, 0, out.data_ptr(), n + 7, m, n, k, ws.data_ptr(), need)
+        assert rc == 0, lib.rr_last_error()
+        assert (out[:, n:] == 5).all() and (ws[need:] == 77).all()
+        want = ops.linear_int8(x, w, sw, x_scale=sx if code == 3 else None, bias=b, act="gelu", out_dtype=torch.float32)
+        assert torch.equal(out[:, :n], want)
 
 
 # ---- beyond 32 bits -------------------------------------------------------------------------------------------------
