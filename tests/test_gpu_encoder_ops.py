@@ -616,6 +616,32 @@ def test_layer_on_two_streams(ops):
             assert torch.equal(y, want[j])
 
 
+def test_layer_from_threads(ops):
+    """Threads with a stream each, calling at once: nothing is shared between calls."""
+    import threading
+    g = gen(16)
+    st, t = layer_state(g, 256, 4, 512, [40, 3, 90, 17], torch.bfloat16)
+    xs = [rand(g, t, 256).to(torch.bfloat16).cuda() for _ in range(4)]
+    want = [layer(ops, x, st) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(j):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(20):
+                y = layer(ops, xs[(i + j) % 4], st)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[(i + j) % 4]):
+                    wrong.append((j, i))
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in range(4)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not wrong
+
+
 def test_everything_in_a_graph_first(ops):
     """Each kernel family captured, also the widest norm (dynamic LDS) and attention in pieces, and replayed on new inputs."""
     g = gen(14)
