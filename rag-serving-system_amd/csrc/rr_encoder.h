@@ -40,7 +40,7 @@ struct LinearArgs {
   int m, n, k;
 };
 hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
-// Inner sizes that are no multiple of 16: whether the product takes copies of its weights, and of 8-bit rows, padded to one.
+// Inner sizes that are no multiple of 4: whether the product takes copies of its weights, and of 8-bit rows, padded to 16.
 bool linear_repacks(int x_type, int64_t m, int n, int k);
 hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const WeightCopy& copy, int k, hipStream_t s);
 // Few short floating-point rows: one launch makes their 8-bit rows too (x holds the floating-point rows, x_scale is unused).

@@ -187,10 +187,11 @@ __device__ __forceinline__ void store4(const LinearArgs& a, int64_t m, int n, i3
   }
 }
 
-// 64 x 64 tiles, any size and alignment: through registers into LDS, the next two steps' loads in flight during a step's matrix
+// 64 x 64 tiles, rows at any byte: through registers into LDS, the next two steps' loads in flight during a step's matrix
 // instructions. Two groups of four waves take every other 128 bytes of k, since such calls have few tiles and wait for their
 // chain of steps; each group then finishes half of the tile, with scales that it asked for before the first step
-// (1031 x 1000 -> 777, GPU time: 10.3 us with one group and scales read at the end, 8.1 so).
+// (1031 rows of 1000 -> 777, GPU time: 10.3 us with one group and scales read at the end, 8.1 so; rows at 4-byte addresses take
+// the tiled product, 6.3).
 constexpr int kAnyStep = 128, kAnyGroups = 2, kPad = kAnyStep + 16;   // kPad: bytes from one LDS row to the next
 template <int OT>
 __global__ __launch_bounds__(256 * kAnyGroups) void linear_any_kernel(LinearArgs a, int64_t tiles_n, int64_t tiles) {
@@ -393,8 +394,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinearArgs a
 // registers, no ds_write) into BUFS buffers in turn: BUFS - 1 steps are in flight while one is multiplied, one barrier a step.
 // Waves: WN x WM, each (TN / WN) x (TM / WM) in 32 x 32 x 32 instructions. LDS rows hold a step; the 16-byte column c of row r
 // lies at column c ^ swizzle(r), so that the 16 lanes that read a column of 16 rows at once meet all 64 banks.
-// Wants rows at 16-byte addresses and k a multiple of 16 (the loads' unit); columns behind k and rows behind the end are out
-// of the buffer's range and read as zeros.
+// Wants rows at 4-byte addresses. What lies behind the last row is out of the buffer's range and read as zeros, and so is a
+// 16-byte column that starts behind k; the one that k ends in is cut in LDS, in the rows of x alone: zeros in one factor do.
 // 16384 x 4096 -> 1024 (int8 rows, bf16 results) in 256 x 256 tiles: 70 us, 1.95 POP/s (the library's i8 product of these
 // sizes takes 75). A step's 2048 cycles of matrix instructions need as many of LDS (192 KiB of reads, 64 KiB of arriving
 // rows); tried and dropped: four waves of 128 x 128 (fewer LDS reads, 87 us), 64-byte steps in four buffers (87), operands
@@ -443,8 +444,8 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
   const int n0 = (int)(tile % tiles_n) * TN;
   const int64_t m0 = tile / tiles_n * TM;
   const int rows_n = a.n - n0 < TN ? a.n - n0 : TN, rows_m = a.m - m0 < TM ? (int)(a.m - m0) : TM;
-  const i32x4 bw = buffer_of(a.w + (int64_t)n0 * a.ldw, (unsigned)((rows_n - 1) * a.ldw + a.k));
-  const i32x4 bx = buffer_of(a.x + m0 * a.ldx, (unsigned)((rows_m - 1) * a.ldx + a.k));
+  const i32x4 bw = buffer_of(a.w + (int64_t)n0 * a.ldw, (unsigned)((rows_n - 1) * a.ldw + a.k + 3) & ~3u);
+  const i32x4 bx = buffer_of(a.x + m0 * a.ldx, (unsigned)((rows_m - 1) * a.ldx + a.k + 3) & ~3u);
   for (int c = threadIdx.x; c < TN; c += 64 * kWaves) {
     const int n = n0 + c < a.n ? n0 + c : a.n - 1;
     chan[0][c] = a.w_scale[n];
@@ -492,6 +493,14 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void linear_tile_kernel(LinearArgs
     if (s + BUFS - 2 < steps) step_barrier<(BUFS - 2) * (kLoadsN + kLoadsM)>();
     else step_barrier<0>();
     if (s + BUFS - 1 < steps) fetch((s + BUFS - 1) * kStep, next);   // (its buffer was last read before this barrier)
+    if (s + 1 == steps && a.k % 16) {
+      for (int r = threadIdx.x; r < TM; r += 64 * kWaves) {
+        const int c = a.k % kStep / 16;
+        u32x4* at = reinterpret_cast<u32x4*>(lds + buf * kBuf + TN * kStep + r * kStep + 16 * (c ^ swizzle(r)));
+        *at = cut(*at, 16 * c, a.k % kStep);
+      }
+      __syncthreads();
+    }
     const char* lw = lds + buf * kBuf + (wn * kN * 32 + row) * kStep;
     const char* lx = lds + buf * kBuf + TN * kStep + (wm * kM * 32 + row) * kStep;
 #pragma unroll
@@ -597,12 +606,12 @@ hipError_t tiled(const LinearArgs& a, hipStream_t s) {
 template <int OT, int ACT>
 hipError_t linear(const LinearArgs& a, hipStream_t s) {
   auto tiles_of = [&](int64_t tn, int64_t tm) { return ((a.n + tn - 1) / tn) * ((a.m + tm - 1) / tm); };
-  const bool rows16 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw | a.k) & 15) == 0;
+  const bool rows4 = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.ldx | a.ldw) & 3) == 0;
   // More rows in blocks of 48, as long as every workgroup has a CU: where the tiles' chain of steps is longer (4096 columns
   // 11.6 us against 9.9, 3008 9.8 / 7.2, 1024 5.3 / 5.2, 400 4.3 / 4.6), or the rows fit no
   // tile (192 x 3769 -> 1024 18.9 / 13.5, x 1001 9.1 / 6.7).
   const int64_t few = ((int64_t)a.n + 15) / 16 * ((a.m + kFewRows - 1) / kFewRows);
-  if (a.m <= kFewRows || (few <= 256 && (!rows16 || a.k >= 1024))) {
+  if (a.m <= kFewRows || (few <= 256 && (!rows4 || a.k >= 1024))) {
     const dim3 grid((a.n + 15) / 16, (a.m + kFewRows - 1) / kFewRows);
     if (a.m <= 16) linear_few_kernel<OT, 1, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     else if (a.m <= 32) linear_few_kernel<OT, 2, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
@@ -617,7 +626,7 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
   //     613 x 4096 -> 1024   64 x 64  11.5 (four or six buffers change nothing)  128 x 128 19
   // Short rows are mostly results: two tiles a CU store while the other multiplies (256 x 256 / 128 x 128, two buffers):
   //   14500 x 512 -> 3530   51.8 / 43.1, with GELU 80.7 / 58.1;  16384 x 512 -> 4096 with GELU 82 / 71, x 768 94 / 97
-  if (rows16 && tiles_of(64, 64) < (1 << 22)) {
+  if (rows4 && tiles_of(64, 64) < (1 << 22)) {
     if (tiles_of(256, 256) >= 192 && a.k > 512) return tiled<OT, ACT, 256, 256, 2, 4, 2>(a, s);
     if (tiles_of(128, 128) > 256) return tiled<OT, ACT, 128, 128, 2, 4, 2>(a, s);
     if (tiles_of(128, 128) >= 224) return tiled<OT, ACT, 128, 128, 2, 4, 4>(a, s);
@@ -646,13 +655,14 @@ hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
   return a.out_type == T_F32 ? linear<T_F32, 0>(a, s) : a.out_type == T_BF16 ? linear<T_BF16, 0>(a, s) : linear<T_F16, 0>(a, s);
 }
 
-// The tiled product of copies, where it saves more than they cost (int8 rows, GPU time, any sizes / copies and tiles):
-//   613 x 4001 -> 1024   20.4 / 21.1 us     613 x 1307 -> 3637   25.1 / 21.1     4000 x 1000 -> 777   26.3 / 15.2
-//   16000 x 4001 -> 1024  249 / 93          2000 x 1307 -> 3637  57.8 / 27.6     2000 x 1000 -> 777   11.9 / no copies: 7.4 + 5
+// Rows that start between dwords: the tiled product of copies, where it saves more than they cost (int8 rows, GPU time, any
+// sizes / copies and tiles):
+//   613 x 4001 -> 1024   20.4 / 21.1 us     613 x 1307 -> 3637   25.1 / 21.1
+//   16000 x 4001 -> 1024  249 / 93          2000 x 1307 -> 3637  57.8 / 27.6
 // Floating-point rows are made with the padding, and the launch that makes them copies the weights beside them.
 bool linear_repacks(int x_type, int64_t m, int n, int k) {
   const int64_t tiles = ((int64_t)n + 63) / 64 * ((m + 63) / 64);
-  return k % 16 && m > kFewRows && tiles < (1 << 22) && m * n * k >= (x_type == T_I8 ? (int64_t)1 << 31 : 0);
+  return k % 4 && m > kFewRows && tiles < (1 << 22) && m * n * k >= (x_type == T_I8 ? (int64_t)1 << 31 : 0);
 }
 
 hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, const WeightCopy& copy, int k, hipStream_t s) {

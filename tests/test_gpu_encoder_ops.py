@@ -159,6 +159,25 @@ def test_linear_int8_odd_inner_sizes_of_many_products(ops, m, n, k):
     assert torch.equal(got, ops.linear_int8(q8, w, sw, x_scale=s8, out_dtype=torch.bfloat16))
 
 
+@pytest.mark.parametrize("m,n,k", [(70, 65, 4), (70, 65, 132), (613, 700, 1000), (1300, 1290, 20), (1500, 1100, 148), (2600, 5000, 260),
+                                   (1000, 2300, 404), (3600, 3400, 636), (16000, 3100, 1028), (4001, 4090, 516), (900, 300, 2044)])
+def test_linear_int8_rows_at_dwords(ops, m, n, k):
+    """Inner sizes that end inside a 16-byte column, in every tile: what lies between the rows is no part of them."""
+    g = gen(m + n + k)
+    q = torch.randint(-128, 128, (m + 1, k + 8), generator=g, dtype=torch.int8).cuda()[:m, 4:4 + k]
+    w = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8).cuda()
+    sx, (_, sw, b) = (0.01 + torch.rand(m, generator=g)).cuda(), weights(g, n, 1)
+    sw, b = sw.cuda(), b.cuda()
+    rows = torch.unique(torch.cat([torch.arange(3), torch.randint(0, m, (60,), generator=g), torch.arange(m - 3, m)])).cuda()
+    for out in (torch.float32, torch.bfloat16):
+        got = ops.linear_int8(q, w, sw, x_scale=sx, bias=b, out_dtype=out)
+        want, tol = plain.linear(q[rows], sx[rows], w, sw, b, "none", out)
+        assert ((got[rows].double().cpu() - want).abs() <= tol).all()
+    wide = torch.zeros(n, k + 13, dtype=torch.int8).cuda()      # the same at odd bytes, in the other kernels
+    wide[:, 1:k + 1] = w
+    assert torch.equal(ops.linear_int8(q, wide[:, 1:k + 1], sw, x_scale=sx, bias=b, out_dtype=torch.bfloat16), got)
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_linear_int8_extremes(ops, m):
     """The longest inner size with every product at its largest: the 32-bit sum must still be exact. -128 is a valid value."""
