@@ -340,7 +340,8 @@ int rr_stream_queues(rr_handle* h, int i, uint64_t* out);
  *     ..._workspace function returns, 16-byte aligned). It holds nothing between calls; calls that may run at the same
  *     time need one each.
  *   - Strides count elements. The last dimension is contiguous; rows may start at any address that is aligned to the
- *     element (rows at 16-byte addresses, 8-bit ones at 4-byte addresses, are read fastest). Outputs must not overlap inputs, except where said.
+ *     element (rows at 16-byte addresses, 8-bit ones at 4-byte addresses, are read fastest). Outputs must not overlap
+ *     inputs, except where said.
  *   - Any number of threads may call at once.
  * Arguments are checked before anything is enqueued (RR_E_INVALID / RR_E_UNSUPPORTED). Integers that live in device memory
  * (lengths, offsets) are not: the kernels clamp them to the buffers instead.

@@ -579,8 +579,11 @@ hipError_t quantize(const void* x, int64_t ldx, int64_t rows, int cols, int cols
   if (chunks <= 32) return go(quantize_rows_kernel<TY, 1, 1, 32>, 1, 32);
   if (chunks <= 64) return go(quantize_rows_kernel<TY, 1, 1>, 1);
   if (chunks <= 64 * 2) return go(quantize_rows_kernel<TY, 1, 2>, 1);
+  if (chunks <= 64 * 3) return go(quantize_rows_kernel<TY, 1, 3>, 1);
   if (chunks <= 64 * 4) return go(quantize_rows_kernel<TY, 1, 4>, 1);
+  if (chunks <= 64 * 6) return go(quantize_rows_kernel<TY, 3, 2>, 3);
   if (chunks <= 64 * 8) return go(quantize_rows_kernel<TY, 4, 2>, 4);
+  if (chunks <= 64 * 12) return go(quantize_rows_kernel<TY, 3, 4>, 3);
   if (chunks <= 64 * 16) return go(quantize_rows_kernel<TY, 4, 4>, 4);
   if (chunks <= 64 * 32) return go(quantize_rows_kernel<TY, 8, 4>, 8);
   return go(quantize_long_rows_kernel<TY>, 4);

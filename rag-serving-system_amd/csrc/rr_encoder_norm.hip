@@ -206,7 +206,9 @@ hipError_t run(NormArgs a, hipStream_t s) {
   if (chunks <= 32) return go(block_norm_kernel<TY, 1, 1, 32>, 1, 32);
   if (chunks <= 64) return go(block_norm_kernel<TY, 1, 1>, 1);
   if (chunks <= 64 * 2) return go(block_norm_kernel<TY, 1, 2>, 1);
+  if (chunks <= 64 * 3) return go(block_norm_kernel<TY, 1, 3>, 1);
   if (chunks <= 64 * 4) return go(block_norm_kernel<TY, 1, 4>, 1);
+  if (chunks <= 64 * 6) return go(block_norm_kernel<TY, 3, 2>, 3);
   if (chunks <= 64 * 8) return go(block_norm_kernel<TY, 4, 2>, 4);
   if (chunks <= 64 * 12) return go(block_norm_kernel<TY, 3, 4>, 3);
   if (chunks <= 64 * 16) return go(block_norm_kernel<TY, 8, 2>, 8);
