@@ -625,7 +625,8 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
   //   16384 x 4096 -> 1024   256 x 256  70 us    128 x 128  85    64 x 64  125
   //    4096 x 4096 -> 1024   128 x 128, four buffers 24, two 27;  64 x 64  32
   //    2048 x 1024 -> 4096   128 x 128, four buffers 19, two 15;  64 x 64  22   (two tiles a CU: they fill each other's waits)
-  //     613 x 1024 -> 4096   64 x 128  9.0 (with GELU two buffers 9.9, three 10.2, four 13.4)  128 x 128  9.5  64 x 64  10.0
+  //     613 x 1024 -> 4096   64 x 128  9.0 (with GELU two buffers 9.9, three 10.2, four 13.4; in an
+  //                          encoder, whose weights come from memory, two 13.1, three 11.3)  128 x 128  9.5  64 x 64  10.0
   //     613 x 4096 -> 1024   64 x 64  11.5 (four or six buffers change nothing)  128 x 128 19
   // Short rows are mostly results: two tiles a CU store while the other multiplies (256 x 256 / 128 x 128, two buffers):
   //   14500 x 512 -> 3530   51.8 / 43.1, with GELU 80.7 / 58.1;  16384 x 512 -> 4096 with GELU 82 / 71, x 768 94 / 97
@@ -633,7 +634,7 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
     if (tiles_of(256, 256) >= 192 && a.k > 512) return tiled<OT, ACT, 256, 256, 2, 4, 2>(a, s);
     if (tiles_of(128, 128) > 256) return tiled<OT, ACT, 128, 128, 2, 4, 2>(a, s);
     if (tiles_of(128, 128) >= 224) return tiled<OT, ACT, 128, 128, 2, 4, 4>(a, s);
-    if (tiles_of(64, 128) >= 256) return tiled<OT, ACT, 64, 128, 2, 4, 2>(a, s);
+    if (tiles_of(64, 128) >= 256) return tiled<OT, ACT, 64, 128, 2, 4, 3>(a, s);
     return tiled<OT, ACT, 64, 64, 2, 2, 3>(a, s);
   }
   const int64_t tiles = tiles_of(64, 64);
