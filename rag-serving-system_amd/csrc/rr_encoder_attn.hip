@@ -263,6 +263,16 @@ struct Core<T_F32, DP> {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The reference follows the running maximum: it moves when a score passes it by 2^8.
+__device__ __forceinline__ bool passes(float top, float m) { return top - m > 8.f; }   // (an exact difference)
+// Scores whose next fp32 number is far away are rounded to powers of two before the reference is taken off. In one step with the
+// subtraction they would keep what the reference lost to its rounding, which at 2^29 overflows fp16 and at 2^32 fp32.
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= 0x1p20f && m != -INFINITY; }
+__device__ __forceinline__ float in_powers(float s, float c) {
+#pragma clang fp contract(off)
+  return s * c;
+}
+
 // where the row's results go, null if the row is not there
 template <class E>
 __device__ __forceinline__ E* out_row(const AttnParams& p, const Span& sq, int b, int kvh, unsigned row) {
@@ -340,6 +350,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
     }
     f32x4 acc[C::kTiles] = {};
     float m = -INFINITY, l = 0.f;
+    bool far = false;   // (of the whole wave)
     struct Block {
       typename C::Keys keys;
       unsigned char there;   // of key `lane`, if there is a mask
@@ -360,23 +371,30 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
       core.scores(of.keys, s);
       float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < C::kMine; ++j) top = fmaxf(top, (valid >> j & 1) ? s[j] * p.c : -INFINITY);
-      // the maximum is a reference only: it moves when a score passes it by 2^8
-      if (__any(top > m + 8.f)) {
+      for (int j = 0; j < C::kMine; ++j) {
+        s[j] = (valid >> j & 1) ? s[j] : -INFINITY;
+        top = fmaxf(top, s[j]);
+      }
+      top = in_powers(top, p.c);
+      if (__any(passes(top, m))) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float to = fmaxf(m, top);
         const float f = to == m ? 1.f : exp2_fast(m - to);
         m = to;
+        far = __any(is_far(m));
         l *= f;
 #pragma unroll
         for (int t = 0; t < C::kTiles; ++t) acc[t] *= f;
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m, c = far ? 1.f : p.c;
+      if (far)
+#pragma unroll
+        for (int j = 0; j < C::kMine; ++j) s[j] = in_powers(s[j], p.c);
       float w[C::kMine];
 #pragma unroll
       for (int j = 0; j < C::kMine; ++j) {
-        w[j] = (valid >> j & 1) ? exp2_fast(fmaf(s[j], p.c, -ref)) : 0.f;
+        w[j] = exp2_fast(fmaf(s[j], c, -ref));
         l += w[j];
       }
       C::accumulate(of.keys, w, valid, acc);
@@ -589,6 +607,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
       for (int s = 0; s < DP / 16; ++s) q[s] ^= 0x80008000u;
     f32x16 acc[DP / 32] = {};
     float m = -INFINITY, l = 0.f;
+    bool far = false;   // (of the whole wave)
     // 32 keys of the buffer, rows key0 and on, `here` those that take part
     auto take = [&](const char* k_rows, int key0, unsigned here) {
       // K is read before the first product, V before the softmax that its product waits for: the reads' latency is hidden
@@ -623,23 +642,27 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
       float top = -INFINITY;
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-      top = top == -INFINITY ? top : top * p.c;
-      if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
+      top = in_powers(top, p.c);
+      if (__any(passes(top, m))) {
         top = fmaxf(top, __shfl_xor(top, 32));
         const float to = fmaxf(m, top);
         const float f = to == m ? 1.f : exp2_fast(m - to);
         m = to;
+        far = __any(is_far(m));
         l *= f;
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) acc[t] *= f;
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m, c = far ? 1.f : p.c;
+      if (far)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = in_powers(s[r], p.c);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         e8 w, rest;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          const float e = exp2_fast(fmaf(s[8 * t + x], p.c, -ref));
+          const float e = exp2_fast(fmaf(s[8 * t + x], c, -ref));
           l += e;
           w[x] = (E)e;
           if constexpr (WK > 1) rest[x] = (E)(e - (float)w[x]);
@@ -848,6 +871,7 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 4) void attn_tile32_kernel(AttnP
     }
     f32x4 acc[C::kTiles] = {};
     float m = -INFINITY, l = 0.f;
+    bool far = false;   // (of the whole wave)
     auto take = [&](const char* k_rows, unsigned here) {
       f32x4 s[2] = {};
 #pragma unroll
@@ -872,24 +896,28 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 4) void attn_tile32_kernel(AttnP
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[h][r]);
-      top = top == -INFINITY ? top : top * p.c;
-      if (__any(top > m + 8.f)) {   // the maximum is a reference only: it moves when a score passes it by 2^8
+      top = in_powers(top, p.c);
+      if (__any(passes(top, m))) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float to = fmaxf(m, top);
         const float f = to == m ? 1.f : exp2_fast(m - to);
         m = to;
+        far = __any(is_far(m));
         l *= f;
 #pragma unroll
         for (int t = 0; t < C::kTiles; ++t) acc[t] *= f;
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m, c = far ? 1.f : p.c;
+      if (far)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r / 4][r % 4] = in_powers(s[r / 4][r % 4], p.c);
       float w[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          w[h][r] = exp2_fast(fmaf(s[h][r], p.c, -ref));
+          w[h][r] = exp2_fast(fmaf(s[h][r], c, -ref));
           l += w[h][r];
         }
       const char* v_rows = k_rows + kHalf;
