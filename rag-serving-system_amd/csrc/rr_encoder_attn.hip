@@ -167,7 +167,7 @@ struct Core16 {
   }
   // valid: bit j says whether key j of this lane takes part; the V rows of the others may hold anything and become zeros
   static __device__ __forceinline__ void accumulate(Keys& of, const float* p, unsigned valid, f32x4* acc) {
-    e8 pe, rest;   // the weights to twice the type's precision, as kFewRows' kernel takes them
+    e8 pe, rest;   // the weights in two parts, as kFewRows' kernel takes them
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       pe[j] = (E)p[j];
@@ -263,10 +263,22 @@ struct Core<T_F32, DP> {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The reference follows the running maximum: it moves when a score passes it by 2^8.
-__device__ __forceinline__ bool passes(float top, float m) { return top - m > 8.f; }   // (an exact difference)
+// The softmax's weights are 2^(c score - m). The reference m follows the running maximum: it moves when a score passes it by
+// kTop + kLag, and then to kTop below that score, so that a row's largest weight is at least 2^kTop and none above 2^(kTop + kLag).
+// Near 1 is right for types with fp32's exponents. fp16 weights begin at 2^13 and stay below its largest, 2^16: steps relative to
+// the weight reach down to 2^-14, 27 powers of two (18.7 nats) below the largest; what is smaller still is off by 2^-38 of it.
+template <int TY> constexpr float kTop = TY == T_F16 ? 13.f : 0.f;
+template <int TY> constexpr float kLag = TY == T_F16 ? 2.9f : 8.f;
+template <int TY>
+__device__ __forceinline__ bool passes(float top, float m) { return top - m > kTop<TY> + kLag<TY>; }   // (an exact difference)
+template <int TY>
+__device__ __forceinline__ float moved(float m, float top) {
+  float to = top - kTop<TY>;
+  if (kTop<TY> != 0.f && passes<TY>(top, to)) to = top;   // (a score so large that the difference was rounded)
+  return fmaxf(m, to);
+}
 // Scores whose next fp32 number is far away are rounded to powers of two before the reference is taken off. In one step with the
-// subtraction they would keep what the reference lost to its rounding, which at 2^29 overflows fp16 and at 2^32 fp32.
+// subtraction they would keep what the reference lost to its rounding, which at 2^28 overflows fp16 and at 2^32 fp32.
 __device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= 0x1p20f && m != -INFINITY; }
 __device__ __forceinline__ float in_powers(float s, float c) {
 #pragma clang fp contract(off)
@@ -376,10 +388,10 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
         top = fmaxf(top, s[j]);
       }
       top = in_powers(top, p.c);
-      if (__any(passes(top, m))) {
+      if (__any(passes<TY>(top, m))) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = fmaxf(m, top);
+        const float to = moved<TY>(m, top);
         const float f = to == m ? 1.f : exp2_fast(m - to);
         m = to;
         far = __any(is_far(m));
@@ -463,8 +475,9 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
 // Keys that do not take part are read as zeros, whatever they held. Lane (i = lane % 32, half = lane / 32) holds the scores
 // of query i with keys 8 (r / 4) + 4 half + r % 4 of a 32-key block, r < 16; eight of them in a row (r / 8 = t) are its slots
 // of the second product's 16-key contraction t. V lies in LDS as in memory; the transposing LDS read hands each lane four keys
-// of one dimension. The weights enter the second product rounded to the type, which is off by as much as the result's own
-// rounding; few rows, which wait for memory and not for arithmetic, add what the rounding left in a product of its own.
+// of one dimension. The weights enter the second product rounded to the type: off by at most half a step of each, which is half
+// a step of sum p |v| in the result, while their sum and the statistics are of the unrounded ones in fp32. Few rows, which
+// wait for memory and not for arithmetic, add what the rounding left in a product of its own (small fp16 rests in steps of 2^-24).
 // DMA: rows at 16-byte addresses go to LDS by the loads themselves; others through registers.
 // WK = 4 is bound by bandwidth: one query x 65536 keys x 4, 32 heads over 8 of 128, bf16: 199 us, 5.4 TB/s; x 512 keys x 32, 16
 // heads of 64: 14 us, 4.8 TB/s. WK = 1 is bound by the softmax's instructions (a 32-key block's 16 exponentials, multiply-adds and
@@ -643,9 +656,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
       top = in_powers(top, p.c);
-      if (__any(passes(top, m))) {
+      if (__any(passes<TY>(top, m))) {
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = fmaxf(m, top);
+        const float to = moved<TY>(m, top);
         const float f = to == m ? 1.f : exp2_fast(m - to);
         m = to;
         far = __any(is_far(m));
@@ -897,10 +910,10 @@ __global__ __launch_bounds__(256, DP > 64 ? 2 : 4) void attn_tile32_kernel(AttnP
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[h][r]);
       top = in_powers(top, p.c);
-      if (__any(passes(top, m))) {
+      if (__any(passes<T_F32>(top, m))) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = fmaxf(m, top);
+        const float to = moved<T_F32>(m, top);
         const float f = to == m ? 1.f : exp2_fast(m - to);
         m = to;
         far = __any(is_far(m));

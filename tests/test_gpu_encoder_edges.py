@@ -24,7 +24,36 @@ def rand(g, *shape, scale=1.0):
     return torch.randn(*shape, generator=g) * scale
 
 
-# ---- attention: scores of every size -------------------------------------------------------------------------------
+# ---- attention: one key far above the others ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("lq,lk", [(1, 100), (9, 100), (1, 4097), (30, 4097), (33, 100), (200, 1100), (130, 4097)])
+@pytest.mark.parametrize("gap", [8, 12, 14, 16, 17, 18, 22])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_attention_weights_far_below_the_largest(ops, dtype, gap, lq, lk):
+    """A key whose value is zero lies `gap` nats above all others, which carry the result: their weights are as exact as
+    weights near the largest, first or last among the keys. The bound is plain.attention's, half a step of each weight
+    relative to it. fp16 alone has weights that it does not hold so, those below 2^-27 of the largest (18.7 nats): its steps are
+    2^-24 there and a rounding 2^-25, which, the largest being at least 2^13, is 2^-38 of the largest, each times its value (below
+    1.5)."""
+    g = gen(gap + lq + lk)
+    h, d = 2, 64
+    for at in (0, lk // 2, lk - 1):
+        q = torch.zeros(1, lq, h, d)
+        q[..., 0] = 1
+        q[..., 1:9] = rand(g, 1, lq, h, 8, scale=0.25)
+        k = torch.zeros(1, lk, h, d)
+        k[..., 1:9] = rand(g, 1, lk, h, 8, scale=0.25)
+        k[0, at] = 0
+        k[0, at, :, 0] = gap
+        v = 0.5 + torch.rand(1, lk, h, d, generator=g)
+        v[0, at] = 0
+        q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+        got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)
+        want, err = plain.attention(q[0], k[0], v[0], torch.ones(lk, dtype=torch.bool), 1.0)
+        if dtype == torch.float16:
+            err = err + lk * 1.5 * 2.0 ** -38
+        plain.within(got[0], want, err, dtype)
+
 
 @pytest.mark.parametrize("lq,lk", [(1, 90), (20, 3000), (150, 700)])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
