@@ -100,6 +100,24 @@ constexpr unsigned kNowhere = 0xfffffff0u;   // an offset behind every buffer
 // Lane (i = lane % 16, g = lane / 16). DP: the head size rounded up to a whole tile.
 template <int TY, int DP> struct Core;
 
+// Two 16-bit values with infinities (and NaNs) as the largest finite number: what the second part of a weight multiplies, which
+// may be 0 or of the other sign and would make a NaN of the infinity that the first part's product has.
+template <int TY>
+__device__ __forceinline__ unsigned finite2(unsigned v) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  constexpr unsigned short kMost = TY == T_BF16 ? 0x7f7f : 0x7bff;
+  const s16x2 up = __builtin_elementwise_min(__builtin_bit_cast(s16x2, v), s16x2{(short)kMost, (short)kMost});
+  constexpr unsigned short kLeast = kMost | 0x8000;
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(u16x2, up), u16x2{kLeast, kLeast}));
+}
+template <int TY>
+__device__ __forceinline__ u32x4 finite8(u32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = finite2<TY>(v[i]);
+  return v;
+}
+
 // 16-bit types: 32 keys a block. Lane i, g holds the scores of query i with keys 4g + r and 16 + 4g + r (r < 4): the eight
 // keys that its slots 8g .. 8g + 7 of the second product's contraction stand for.
 template <int TY, int DP>
@@ -188,8 +206,8 @@ struct Core16 {
         lo[x] = __builtin_amdgcn_perm(of.v[2 * x + 1][w], of.v[2 * x][w], 0x05040100u);
         hi[x] = __builtin_amdgcn_perm(of.v[2 * x + 1][w], of.v[2 * x][w], 0x07060302u);
       }
-      acc[2 * w] = mma(lo, pr, mma(lo, pb, acc[2 * w]));
-      acc[2 * w + 1] = mma(hi, pr, mma(hi, pb, acc[2 * w + 1]));
+      acc[2 * w] = mma(finite8<TY>(lo), pr, mma(lo, pb, acc[2 * w]));
+      acc[2 * w + 1] = mma(finite8<TY>(hi), pr, mma(hi, pb, acc[2 * w + 1]));
     }
   }
 };
@@ -683,7 +701,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void attn_tile_kernel(AttnP
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) {
           acc[dt] = mma32<TY>(vf[t][dt], __builtin_bit_cast(u32x4, w), acc[dt]);
-          if constexpr (WK > 1) acc[dt] = mma32<TY>(vf[t][dt], __builtin_bit_cast(u32x4, rest), acc[dt]);
+          if constexpr (WK > 1) acc[dt] = mma32<TY>(finite8<TY>(vf[t][dt]), __builtin_bit_cast(u32x4, rest), acc[dt]);
         }
       }
     };

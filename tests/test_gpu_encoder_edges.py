@@ -74,3 +74,30 @@ def test_attention_of_scores_beyond_their_own_resolution(ops, dtype, lq, lk):
         scale = 2.0 ** power / 3843
         got = ops.cross_attention(q.to(dtype).cuda(), k.to(dtype).cuda(), v.cuda(), scale=scale)
         assert torch.equal(got.cpu(), v[:, at:at + 1].expand(-1, lq, -1, -1))
+
+
+@pytest.mark.parametrize("lq,lk", [(1, 1), (1, 90), (7, 128), (20, 3000), (40, 90), (150, 700)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_attention_of_infinite_values(ops, dtype, lq, lk):
+    """An infinity among the values is one in the result wherever its key takes part; both signs of it, or a NaN, are NaN. The
+    other dimensions do not see it, nor do sequences whose lengths leave it out."""
+    g = gen(lq + lk)
+    h, d = 2, 64
+    q, k, v = (rand(g, 3, n, h, d).to(dtype) for n in (lq, lk, lk))
+    v2 = v.clone()
+    v2[:, lk // 2, 0, 3] = float("inf")
+    v2[:, lk // 3, 0, 9] = float("-inf")
+    v2[:, lk // 2, 1, 17] = float("nan")
+    v2[:, 0, 1, 5], v2[:, lk - 1, 1, 5] = float("inf"), float("-inf")
+    lens = torch.tensor([lk, lk, 0], dtype=torch.int32)
+    got = ops.cross_attention(q.cuda(), k.cuda(), v2.cuda(), key_lengths=lens.cuda()).cpu()
+    assert (got[2] == 0).all()
+    got, bad = got[:2], torch.zeros(h, d, dtype=torch.bool)
+    assert (got[:, :, 0, 3] == float("inf")).all() and (got[:, :, 0, 9] == float("-inf")).all()
+    assert got[:, :, 1, 17].isnan().all()
+    assert got[:, :, 1, 5].isnan().all() if lk > 1 else (got[:, :, 1, 5] == float("-inf")).all()
+    for i, j in ((0, 3), (0, 9), (1, 17), (1, 5)):
+        bad[i, j] = True
+    for b in range(2):
+        want, err = plain.attention(q[b], k[b], v[b], torch.ones(lk, dtype=torch.bool), d ** -0.5)
+        plain.within(got[b][:, ~bad], want[:, ~bad], err[:, ~bad], dtype)
