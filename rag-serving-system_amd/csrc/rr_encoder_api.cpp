@@ -267,7 +267,7 @@ int rr_cross_attention(int device, void* stream, int type, const void* q, int64_
   for (const void* p : {static_cast<const void*>(q_offsets), static_cast<const void*>(k_offsets),
                         static_cast<const void*>(key_lengths)})
     if (misaligned(p, 4)) return fail(RR_E_INVALID, "%s: offsets or lengths are not aligned to their 4-byte elements", me);
-  if (batch == 0 || max_q == 0 || (q_offsets && total_q == 0)) return RR_OK;
+  if (batch == 0 || (q_offsets ? total_q : max_q) == 0) return RR_OK;
   TRY(bad_rows(me, "q", q, d, d, eb));
   TRY(bad_rows(me, "out", out, d, d, eb));
   if (max_k > 0 && !(k_offsets && total_k == 0)) {

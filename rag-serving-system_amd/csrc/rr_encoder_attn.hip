@@ -1079,6 +1079,7 @@ struct Plan {
 };
 Plan plan(int type, int batch, int heads, int kv_heads, int d, int max_q, int max_k) {
   Plan p;
+  if (max_q < 1) max_q = 1;   // (a hint, for packed queries: there may be some all the same)
   const int64_t rows = (int64_t)max_q * (heads / kv_heads);
   const int64_t sixteens = (rows + kRows - 1) / kRows * batch * kv_heads;
   const bool much = max_k <= 128 || (double)rows * batch * kv_heads * max_k * d >= 1 << 28;

@@ -1,0 +1,22 @@
+"""The embedding encoder's operators and their build at the edges, without a GPU: what is refused and what is not."""
+import ctypes
+
+import pytest
+
+from rag_service_amd import _lib
+from test_encoder_refusals import NULL, ODD, P, attention, lib, norm, quantize, refused  # noqa: F401
+
+
+# ---- attention: hints do not say what there is -----------------------------------------------------------------------
+
+def test_packed_queries_are_there_whatever_the_hint_says(lib):  # noqa: F811
+    """max_q = 0 with queries in the packed rows: there is work, so the arguments are looked at (it was taken for nothing to
+    do, and the results left as they were)."""
+    refused(lib, attention(lib, qo=P, total_q=4, max_q=0, q=NULL), _lib.RR_E_INVALID, "q is null")
+    refused(lib, attention(lib, qo=P, total_q=4, max_q=0, out=ODD), _lib.RR_E_INVALID, "aligned")
+    assert attention(lib, qo=P, total_q=0, max_q=7, q=NULL, out=NULL) == _lib.RR_OK
+    # the workspace asked for with this hint is what the call wants
+    need = lib.rr_cross_attention_workspace(1, 2, 2, 2, 16, 0, 4096)
+    assert need == lib.rr_cross_attention_workspace(1, 2, 2, 2, 16, 1, 4096) > 0
+    refused(lib, attention(lib, qo=P, total_q=4, max_q=0, max_k=4096, ks=(65536, 16, 16), vs=(65536, 16, 16)),
+            _lib.RR_E_INVALID, "workspace")

@@ -101,3 +101,19 @@ def test_attention_of_infinite_values(ops, dtype, lq, lk):
     for b in range(2):
         want, err = plain.attention(q[b], k[b], v[b], torch.ones(lk, dtype=torch.bool), d ** -0.5)
         plain.within(got[b][:, ~bad], want[:, ~bad], err[:, ~bad], dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_attention_packed_with_hints_of_nothing(ops, dtype):
+    """max_q and max_k size the launch of packed sides, whatever they say: 0 as well."""
+    g = gen(31)
+    h, d = 4, 64
+    ql, kl = [0, 1, 17, 130, 2], [5, 0, 16, 257, 600]
+    qo, ko = (torch.tensor([0] + n).cumsum(0).to(torch.int32) for n in (ql, kl))
+    q, k, v = (rand(g, n, h, d).to(dtype) for n in (sum(ql), sum(kl), sum(kl)))
+    for max_q, max_k in ((0, 0), (0, 600), (0, 5000)):
+        got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), q_offsets=qo.cuda(), k_offsets=ko.cuda(), max_q=max_q, max_k=max_k)
+        for i in range(len(ql)):
+            a, b, c, e = qo[i], qo[i + 1], ko[i], ko[i + 1]
+            want, err = plain.attention(q[a:b], k[c:e], v[c:e], torch.ones(kl[i], dtype=torch.bool), d ** -0.5)
+            plain.within(got[a:b], want, err, dtype)
