@@ -270,7 +270,7 @@ int rr_cross_attention(int device, void* stream, int type, const void* q, int64_
   if (batch == 0 || (q_offsets ? total_q : max_q) == 0) return RR_OK;
   TRY(bad_rows(me, "q", q, d, d, eb));
   TRY(bad_rows(me, "out", out, d, d, eb));
-  if (max_k > 0 && !(k_offsets && total_k == 0)) {
+  if ((k_offsets ? total_k : max_k) > 0) {
     TRY(bad_rows(me, "k", k, d, d, eb));
     TRY(bad_rows(me, "v", v, d, d, eb));
   }

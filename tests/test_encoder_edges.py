@@ -20,3 +20,9 @@ def test_packed_queries_are_there_whatever_the_hint_says(lib):  # noqa: F811
     assert need == lib.rr_cross_attention_workspace(1, 2, 2, 2, 16, 1, 4096) > 0
     refused(lib, attention(lib, qo=P, total_q=4, max_q=0, max_k=4096, ks=(65536, 16, 16), vs=(65536, 16, 16)),
             _lib.RR_E_INVALID, "workspace")
+
+
+def test_packed_keys_are_checked_whatever_the_hint_says(lib):  # noqa: F811
+    """max_k = 0 with keys in the packed rows: the kernels read them, so null and misaligned keys are refused."""
+    for change, word in (({"k": NULL}, "k is null"), ({"v": NULL}, "v is null"), ({"k": ODD}, "aligned")):
+        refused(lib, attention(lib, ko=P, total_k=4, max_k=0, **change), _lib.RR_E_INVALID, word)
