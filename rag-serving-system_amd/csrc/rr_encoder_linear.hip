@@ -121,7 +121,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quantize_rows_kernel(co
   }
 }
 
-// Rows of any length: one workgroup per row, two passes over it (the second one from cache).
+// Rows of any length: one workgroup per row, two passes over it (the second one from cache). Columns up to 2^31 - 1 are counted
+// in unsigned, where the step behind the last one still fits. 4096 x 40000 bf16 320 us, 1.5 TB/s, fp32 417 us, 2.0 TB/s (element
+// by element, of 5.2 that a large copy reaches); a single row is one CU's work: 2^25 columns 83 ms.
 template <int TY>
 __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const void* xv, int64_t ldx, int64_t rows, int cols,
                                                                  int cols_pad, int8_t* q, int64_t ldq, float* scale,
@@ -137,14 +139,14 @@ __global__ __launch_bounds__(256) void quantize_long_rows_kernel(const void* xv,
   for (int64_t r = blockIdx.x; r < rows; r += blocks) {
     const E* x = static_cast<const E*>(xv) + r * ldx;
     unsigned m = 0;
-    for (int c = threadIdx.x; c < cols; c += 256) {
+    for (unsigned c = threadIdx.x; c < (unsigned)cols; c += 256) {
       const unsigned t = mag((float)x[c]);
       m = t > m ? t : m;
     }
     const float s = row_scale(over.max(m));
     const float div = row_divisor(s);
-    for (int c = threadIdx.x; c < cols_pad; c += 256)
-      q[r * ldq + c] = c < cols && s == s ? (int8_t)to_i8((float)x[c], div) : 0;
+    for (unsigned c = threadIdx.x; c < (unsigned)cols_pad; c += 256)
+      q[r * ldq + c] = c < (unsigned)cols && s == s ? (int8_t)to_i8((float)x[c], div) : 0;
     if (threadIdx.x == 0) scale[r] = s;
   }
 }
@@ -573,7 +575,7 @@ hipError_t quantize(const void* x, int64_t ldx, int64_t rows, int cols, int cols
     kernel<<<dim3(blocks + more), threads, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale, blocks, also);
     return hipGetLastError();
   };
-  const int chunks = (cols_pad + N - 1) / N;
+  const int chunks = cols_pad / N + (cols_pad % N != 0);
   if (chunks <= 8) return go(quantize_rows_kernel<TY, 1, 1, 8>, 1, 8);
   if (chunks <= 16) return go(quantize_rows_kernel<TY, 1, 1, 16>, 1, 16);
   if (chunks <= 32) return go(quantize_rows_kernel<TY, 1, 1, 32>, 1, 32);

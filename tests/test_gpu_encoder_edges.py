@@ -117,3 +117,24 @@ def test_attention_packed_with_hints_of_nothing(ops, dtype):
             a, b, c, e = qo[i], qo[i + 1], ko[i], ko[i + 1]
             want, err = plain.attention(q[a:b], k[c:e], v[c:e], torch.ones(kl[i], dtype=torch.bool), d ** -0.5)
             plain.within(got[a:b], want, err, dtype)
+
+
+# ---- 8-bit rows: the longest --------------------------------------------------------------------------------------------
+
+def test_quantize_rows_of_the_longest_row(ops):
+    """A row of 2^31 - 1 columns: every one of them is converted, the largest being the last (about five seconds)."""
+    n = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GiB of GPU memory")
+    x = torch.zeros(1, n, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, 5000, n // 2, n - 300, n - 256, n - 2, n - 1], device="cuda")
+    some = torch.tensor([3.0, -60.0, 1.0, 100.0, -7.0, 9.0, 63.0, -127.0], device="cuda")
+    x[0, at] = some.to(torch.bfloat16)
+    q, s = ops.quantize_rows(x)
+    _, want = plain.rows8(some[None])
+    assert torch.equal(s.cpu(), want)
+    assert torch.equal(q[0, at].cpu(), plain.rows8(some[None])[0][0])
+    q[0, at] = 0
+    assert not any(bool(part.any()) for part in q[0].split(1 << 28))
+    del x, q
+    torch.cuda.empty_cache()
