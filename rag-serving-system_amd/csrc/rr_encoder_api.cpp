@@ -212,7 +212,7 @@ int rr_block_norm(int device, void* hip_stream, int type, int64_t rows, int32_t 
   if (post_norm == RR_NORM_NONE && (post_weight || post_bias))
     return fail(RR_E_INVALID, "%s: weights of a post norm that is not there", me);
   const int eb = bytes_of(type);
-  if (gate && (rows_per_gate < 1 || gate_rows < 0 || (rows + rows_per_gate - 1) / rows_per_gate > gate_rows))
+  if (gate && (rows_per_gate < 1 || gate_rows < rows / rows_per_gate + (rows % rows_per_gate != 0)))
     return fail(RR_E_INVALID, "%s: %lld gate rows of %lld rows each for %lld rows", me, (long long)gate_rows,
                 (long long)rows_per_gate, (long long)rows);
   if (rows == 0) return RR_OK;

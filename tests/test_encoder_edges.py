@@ -26,3 +26,11 @@ def test_packed_keys_are_checked_whatever_the_hint_says(lib):  # noqa: F811
     """max_k = 0 with keys in the packed rows: the kernels read them, so null and misaligned keys are refused."""
     for change, word in (({"k": NULL}, "k is null"), ({"v": NULL}, "v is null"), ({"k": ODD}, "aligned")):
         refused(lib, attention(lib, ko=P, total_k=4, max_k=0, **change), _lib.RR_E_INVALID, word)
+
+
+# ---- norm: gates -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("gate_rows,rows_per_gate", [(0, 2 ** 63 - 1), (0, 2 ** 63 - 3), (0, 4), (1, 3), (-1, 2 ** 63 - 1)])
+def test_gate_rows_are_counted_without_overflow(lib, gate_rows, rows_per_gate):  # noqa: F811
+    """A gate of too few rows for 4 rows, also where rows + rows_per_gate passes 2^63."""
+    refused(lib, norm(lib, gate=P, gate_rows=gate_rows, rows_per_gate=rows_per_gate), _lib.RR_E_INVALID, "gate rows")
