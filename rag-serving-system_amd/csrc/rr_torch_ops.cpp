@@ -275,6 +275,7 @@ PyObject* block_norm(PyObject* const* args) {
       throw BadValue("gate has shape " + shape_of(g) + "; expected (" + std::to_string(yr.cols) + ",) or (gate_rows, " +
                      std::to_string(yr.cols) + ")");
     gr = rows_of("gate", g);
+    if (gr.rows == 0 && yr.rows) throw BadValue("gate has no rows");   // (and no address, which would say that there is no gate)
     if (g.dim() == 1) per = yr.rows > 1 ? yr.rows : 1;
   }
   Tensor hold[4];

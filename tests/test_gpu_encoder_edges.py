@@ -138,3 +138,14 @@ def test_quantize_rows_of_the_longest_row(ops):
     assert not any(bool(part.any()) for part in q[0].split(1 << 28))
     del x, q
     torch.cuda.empty_cache()
+
+
+# ---- norm: gates ------------------------------------------------------------------------------------------------------
+
+def test_block_norm_refuses_a_gate_without_rows(ops):
+    """A gate of no rows for rows that need one is refused, and not taken for no gate; for no rows it is enough."""
+    y, none = torch.ones(4, 16).cuda(), torch.ones(0, 16).cuda()
+    for per in (1, 4, 2 ** 40):
+        with pytest.raises(ValueError, match="gate"):
+            ops.block_norm(y, gate=none, rows_per_gate=per)
+    assert ops.block_norm(y[:0], gate=none).normed.shape == (0, 16)
