@@ -23,8 +23,12 @@ template <> struct Elem<T_F32> { using type = float; };
 template <> struct Elem<T_BF16> { using type = __bf16; };
 template <> struct Elem<T_F16> { using type = _Float16; };
 
-// A launch's workgroups: one for each piece of work up to 2^22 (a grid holds below 2^32 threads); they loop over the rest.
-inline dim3 grid_of(int64_t pieces) { return dim3((unsigned)(pieces < (1 << 22) ? pieces : 1 << 22)); }
+// A launch's workgroups of so many threads: one for each piece of work up to 2^22 and below 2^32 threads in all, which is what a
+// grid holds; they loop over the rest.
+inline dim3 grid_of(int64_t pieces, int threads) {
+  const int64_t hold = ((int64_t(1) << 32) - 1) / threads, most = hold < (1 << 22) ? hold : 1 << 22;
+  return dim3((unsigned)(pieces < most ? pieces : most));
+}
 
 // N elements from an address that is aligned to one element only (one vector load: the hardware takes such addresses).
 template <class V>

@@ -571,7 +571,7 @@ hipError_t quantize(const void* x, int64_t ldx, int64_t rows, int cols, int cols
   constexpr int N = Chunk<typename Elem<TY>::type>::N;
   auto go = [&](auto kernel, int waves, int lanes = 64) {
     const int groups = waves == 1 ? 256 / lanes : 1, threads = waves == 1 ? 256 : 64 * waves;
-    const unsigned blocks = grid_of((rows + groups - 1) / groups).x, more = (unsigned)std::min<int64_t>(also.blocks(threads), 1 << 16);
+    const unsigned blocks = grid_of((rows + groups - 1) / groups, threads).x, more = (unsigned)std::min<int64_t>(also.blocks(threads), 1 << 16);
     kernel<<<dim3(blocks + more), threads, 0, s>>>(x, ldx, rows, cols, cols_pad, q, ldq, scale, blocks, also);
     return hipGetLastError();
   };
@@ -640,7 +640,7 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
     return tiled<OT, ACT, 64, 64, 2, 2, 3>(a, s);
   }
   const int64_t tiles = tiles_of(64, 64);
-  linear_any_kernel<OT><<<grid_of(tiles), 256 * kAnyGroups, 0, s>>>(a, (a.n + 63) / 64, tiles);
+  linear_any_kernel<OT><<<grid_of(tiles, 256 * kAnyGroups), 256 * kAnyGroups, 0, s>>>(a, (a.n + 63) / 64, tiles);
   return hipGetLastError();
 }
 template <int OT, int XT>
@@ -675,7 +675,7 @@ hipError_t launch_repack(const int8_t* x, int64_t ldx, int64_t m, int8_t* to_x, 
   const int kp = (int)round_up(k, 16);
   const Repack one{x, ldx, m, to_x, k, kp}, two{copy.w, copy.ldw, copy.n, copy.to, k, kp};
   const int64_t blocks = one.blocks(256) + two.blocks(256);
-  repack_kernel<<<grid_of(blocks), 256, 0, s>>>(one, two, one.blocks(256), blocks);
+  repack_kernel<<<grid_of(blocks, 256), 256, 0, s>>>(one, two, one.blocks(256), blocks);
   return hipGetLastError();
 }
 

@@ -218,7 +218,7 @@ hipError_t run(NormArgs a, hipStream_t s) {
   auto wide = block_norm_wide_kernel<TY>;
   if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(wide), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds))
     return e;
-  wide<<<grid_of(a.rows), 1024, lds, s>>>(a);
+  wide<<<grid_of(a.rows, 1024), 1024, lds, s>>>(a);
   return hipGetLastError();
 }
 

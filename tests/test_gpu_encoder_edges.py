@@ -149,3 +149,32 @@ def test_block_norm_refuses_a_gate_without_rows(ops):
         with pytest.raises(ValueError, match="gate"):
             ops.block_norm(y, gate=none, rows_per_gate=per)
     assert ops.block_norm(y[:0], gate=none).normed.shape == (0, 16)
+
+
+# ---- the largest numbers of rows ---------------------------------------------------------------------------------------
+
+def room(gib):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of GPU memory")
+
+
+def test_block_norm_of_four_million_wide_rows(ops):
+    """2^22 rows that do not fit the registers, written in place: as many workgroups of 1024 as rows would be 2^32 threads, more
+    than a launch may have."""
+    from rag_service_amd import _lib
+    lib, rows, cols = _lib.load_library(), 1 << 22, 16640
+    room(140)
+    y = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, 7, 2047, 2048, rows // 2, rows - 2, rows - 1], device="cuda")
+    some = rand(gen(5), len(at), cols).to(torch.bfloat16).cuda()
+    y[at] = some
+    rc = lib.rr_block_norm(0, torch.cuda.current_stream().cuda_stream, _lib.RR_TYPE_BF16, rows, cols, y.data_ptr(), cols, None, 0,
+                           1.0, None, 0, 0, 1, _lib.RR_NORM_NONE, None, None, _lib.RR_NORM_LAYER, None, None, 1e-5, None, 0,
+                           y.data_ptr(), cols, None, 0, None)
+    assert rc == _lib.RR_OK, lib.rr_last_error()
+    assert torch.equal(y[at], ops.block_norm(some).normed)
+    y[at] = 0
+    assert not any(bool(part.any()) for part in y.split(1 << 16))
+    del y
+    torch.cuda.empty_cache()
