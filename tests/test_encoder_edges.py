@@ -34,3 +34,31 @@ def test_packed_keys_are_checked_whatever_the_hint_says(lib):  # noqa: F811
 def test_gate_rows_are_counted_without_overflow(lib, gate_rows, rows_per_gate):  # noqa: F811
     """A gate of too few rows for 4 rows, also where rows + rows_per_gate passes 2^63."""
     refused(lib, norm(lib, gate=P, gate_rows=gate_rows, rows_per_gate=rows_per_gate), _lib.RR_E_INVALID, "gate rows")
+
+
+# ---- the build ---------------------------------------------------------------------------------------------------------
+
+def test_every_object_follows_the_headers_it_includes():
+    """A header that a unit includes, directly or through others, is a prerequisite of its object: make would rebuild it
+    (asked without building: -n, the header taken as new)."""
+    import os
+    import re
+    import subprocess
+    csrc = os.path.join(_lib.PKG_ROOT, "csrc")
+    where = [csrc, _lib.PKG_ROOT + "/../include"]                # (as the Makefile spells it)
+
+    def headers(path, seen):
+        for name in re.findall(r'^#include "([^"]+\.h)"', open(path).read(), flags=re.M):
+            at = next((os.path.join(d, name) for d in where if os.path.exists(os.path.join(d, name))), None)
+            if at and at not in seen:
+                seen.add(at)
+                headers(at, seen)
+        return seen
+
+    units = [f for f in sorted(os.listdir(csrc)) if f.endswith((".hip", ".cpp"))]
+    assert len(units) >= 12
+    needs = {f: headers(os.path.join(csrc, f), set()) for f in units}
+    for header in sorted(set().union(*needs.values())):
+        told = subprocess.run(["make", "-n", "-C", _lib.PKG_ROOT, "-W", header], capture_output=True, text=True).stdout
+        for unit in (f for f in units if header in needs[f]):
+            assert f"csrc/{unit}" in told, f"{unit} is not rebuilt when {os.path.basename(header)} changes"
