@@ -62,3 +62,38 @@ def test_every_object_follows_the_headers_it_includes():
         told = subprocess.run(["make", "-n", "-C", _lib.PKG_ROOT, "-W", header], capture_output=True, text=True).stdout
         for unit in (f for f in units if header in needs[f]):
             assert f"csrc/{unit}" in told, f"{unit} is not rebuilt when {os.path.basename(header)} changes"
+
+
+@pytest.fixture
+def fake_tree(tmp_path):
+    """The Makefile and the sources in a folder of their own, and a compiler that only makes the file it is asked for."""
+    import os
+    import shutil
+    import subprocess
+    pkg = tmp_path / "pkg"
+    pkg.mkdir()
+    (pkg / "rag_service_amd").mkdir()
+    shutil.copy(os.path.join(_lib.PKG_ROOT, "Makefile"), pkg / "Makefile")
+    os.symlink(os.path.join(_lib.PKG_ROOT, "csrc"), pkg / "csrc")
+    os.symlink(os.path.join(_lib.REPO_ROOT, "include"), tmp_path / "include")
+    cc = tmp_path / "cc"
+    cc.write_text('#!/bin/sh\nwhile [ $# -gt 0 ]; do [ "$1" = -o ] && touch "$2"; shift; done\n')
+    cc.chmod(0o755)
+
+    def make(python):
+        return subprocess.run(["make", "-C", str(pkg), f"HIPCC={cc}", f"CXX={cc}", f"PYTHON={python}"], capture_output=True,
+                              text=True)
+    return pkg, make
+
+
+def test_make_without_torch_builds_the_library(fake_tree):
+    """The retriever needs no torch: where there is none, make builds the library, says what it leaves out and succeeds."""
+    import sys
+    pkg, make = fake_tree
+    for none in (sys.executable + " -I -S", "/no/such/python"):
+        r = make(none)
+        assert r.returncode == 0, r.stdout + r.stderr
+        assert (pkg / "librag_retrieval.so").exists() and not (pkg / "rag_service_amd" / "_torch_ops.so").exists()
+        assert "torch" in r.stdout and "not built" in r.stdout
+    r = make(sys.executable)
+    assert r.returncode == 0 and (pkg / "rag_service_amd" / "_torch_ops.so").exists(), r.stdout + r.stderr
