@@ -6,6 +6,7 @@ raises ``HipRetrievalUnavailable``. The product path never routes through ``orac
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import subprocess
 import sys
@@ -18,6 +19,7 @@ PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))   # rag-s
 REPO_ROOT = os.path.dirname(PKG_ROOT)
 # RR_LIBRARY: another build of the same library (A/B measurements of kernel variants in one box call)
 LIB_PATH = os.environ.get("RR_LIBRARY") or os.path.join(PKG_ROOT, "librag_retrieval.so")
+TORCH_OPS_PATH = os.path.join(PKG_ROOT, "rag_service_amd", "_torch_ops.so")     # the torch side of .ops
 HEADER_PATH = os.path.join(REPO_ROOT, "include", "rag_retrieval.h")
 
 # mirrors include/rag_retrieval.h
@@ -134,8 +136,10 @@ _lib_lock = threading.Lock()
 
 
 def build(force: bool = False) -> str:
-    """Compile librag_retrieval.so for gfx950 with hipcc (in-tree)."""
-    if force or not os.path.exists(LIB_PATH):
+    """Compile librag_retrieval.so for gfx950 with hipcc and, where torch is installed, the torch side of ``ops`` (in-tree)."""
+    missing = not os.path.exists(LIB_PATH) or (not os.path.exists(TORCH_OPS_PATH)
+                                               and importlib.util.find_spec("torch") is not None)
+    if force or missing:
         subprocess.check_call(["make", "-C", PKG_ROOT, "-j8"])
     return LIB_PATH
 

@@ -97,3 +97,25 @@ def test_make_without_torch_builds_the_library(fake_tree):
         assert "torch" in r.stdout and "not built" in r.stdout
     r = make(sys.executable)
     assert r.returncode == 0 and (pkg / "rag_service_amd" / "_torch_ops.so").exists(), r.stdout + r.stderr
+
+
+def test_build_makes_what_is_missing(tmp_path, monkeypatch):
+    """build(): make runs if the library is missing, or the torch side where there is a torch; not if nothing is."""
+    import importlib.util
+    import subprocess
+    ran = []
+    monkeypatch.setattr(subprocess, "check_call", lambda cmd, **kw: ran.append(cmd))
+    lib_at, ops_at = tmp_path / "librag_retrieval.so", tmp_path / "_torch_ops.so"
+    monkeypatch.setattr(_lib, "LIB_PATH", str(lib_at))
+    monkeypatch.setattr(_lib, "TORCH_OPS_PATH", str(ops_at), raising=False)
+    there = object()
+    for have_lib, have_ops, torch, want in ((0, 0, there, 1), (1, 0, there, 1), (1, 1, there, 0), (0, 1, there, 1), (1, 0, None, 0),
+                                            (0, 0, None, 1)):
+        for p, have in ((lib_at, have_lib), (ops_at, have_ops)):
+            p.touch() if have else p.unlink(missing_ok=True)
+        monkeypatch.setattr(importlib.util, "find_spec", lambda name: torch)
+        ran.clear()
+        assert _lib.build() == str(lib_at)
+        assert len(ran) == want, (have_lib, have_ops, torch)
+    _lib.build(force=True)
+    assert len(ran) == want + 1
