@@ -615,9 +615,9 @@ hipError_t linear(const LinearArgs& a, hipStream_t s) {
   // More rows in blocks of 48, as long as every workgroup has a CU: where the tiles' chain of steps is longer (4096 columns
   // 11.6 us against 9.9, 3008 9.8 / 7.2, 1024 5.3 / 5.2, 400 4.3 / 4.6), or the rows fit no
   // tile (192 x 3769 -> 1024 18.9 / 13.5, x 1001 9.1 / 6.7).
-  const int64_t few = ((int64_t)a.n + 15) / 16 * ((a.m + kFewRows - 1) / kFewRows);
+  const int64_t blocks = ((int64_t)a.m + kFewRows - 1) / kFewRows, few = ((int64_t)a.n + 15) / 16 * blocks;
   if (a.m <= kFewRows || (few <= 256 && (!rows4 || a.k >= 1024))) {
-    const dim3 grid((a.n + 15) / 16, (a.m + kFewRows - 1) / kFewRows);
+    const dim3 grid((a.n + 15) / 16, (unsigned)blocks);
     if (a.m <= 16) linear_few_kernel<OT, 1, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     else if (a.m <= 32) linear_few_kernel<OT, 2, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);
     else linear_few_kernel<OT, 3, T_I8><<<grid, 64 * kFewWaves, 0, s>>>(a);

@@ -178,3 +178,19 @@ def test_block_norm_of_four_million_wide_rows(ops):
     assert not any(bool(part.any()) for part in y.split(1 << 16))
     del y
     torch.cuda.empty_cache()
+
+
+def test_linear_int8_of_two_billion_rows(ops):
+    """As many rows as the header allows, 2^31 - 1, at any byte: every result is right."""
+    m = 2 ** 31 - 1
+    room(40)
+    x = torch.arange(m, device="cuda", dtype=torch.int32).to(torch.int8)[:, None]
+    sx = torch.full((m,), 0.37, device="cuda")
+    w, sw = torch.tensor([[-3]], dtype=torch.int8).cuda(), torch.tensor([0.11]).cuda()
+    got = ops.linear_int8(x, w, sw, x_scale=sx, out_dtype=torch.bfloat16)
+    scale = torch.tensor(0.37) * torch.tensor(0.11)                  # the product rounded once, then the result: as the operator
+    for lo in range(0, m, 1 << 27):
+        want = (x[lo:lo + (1 << 27)].float() * -3 * scale.cuda()).to(torch.bfloat16)
+        assert torch.equal(got[lo:lo + (1 << 27)], want)
+    del x, sx, got, want
+    torch.cuda.empty_cache()
