@@ -11,11 +11,14 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <dlfcn.h>
 
@@ -68,6 +71,11 @@ const Tensor* tensor(const char* name, PyObject* o) {
   const Tensor& t = THPVariable_Unpack(o);
   if (t.requires_grad() && c10::GradMode::is_enabled())
     throw BadValue(std::string(name) + " requires a gradient; these operators are for inference (torch.no_grad())");
+  // What the operators would pass by without a word: a tangent, and values that a view's bit says are negated (or zeros).
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    throw BadValue(std::string(name) + " has a forward-mode tangent; these operators are for inference (unpack_dual(...).primal)");
+  if (t.is_neg() || t._is_zerotensor())
+    throw BadValue(std::string(name) + " is a negated view or has no values of its own; resolve_neg() or clone() it first");
   return &t;
 }
 void on_gpu(const char* name, const Tensor& t) {
@@ -178,6 +186,11 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   if (!p_cross_attention_workspace) {
     PyErr_SetString(PyExc_RuntimeError, "bind() has not been called");
+    return nullptr;
+  }
+  if (torch::jit::tracer::isTracing() ||
+      c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value()) {
+    PyErr_SetString(PyExc_ValueError, "these operators cannot be traced: a trace would keep their results as constants");
     return nullptr;
   }
   try {

@@ -2,7 +2,8 @@
 
 Thin wrappers of the C-ABI's handle-free calls (``rr_quantize_rows``, ``rr_linear_i8``, ``rr_block_norm``,
 ``rr_cross_attention`` in ``include/rag_retrieval.h``, which states the arithmetic). They stand for the forward pass of the
-reference's embedding half (``batch_processor.py:88-91``), for inference only: tensors that ask for gradients are refused.
+reference's embedding half (``batch_processor.py:88-91``), for inference only: tensors that ask for gradients or carry forward-mode
+tangents are refused, and so are negated views and calls under a tracer.
 
 Every call runs on the current stream of its tensors' device, allocates its results and scratch memory there through torch
 (so calls can be captured into a graph and run on several streams at once), and returns without waiting. Arguments that do

@@ -119,3 +119,43 @@ def test_build_makes_what_is_missing(tmp_path, monkeypatch):
         assert len(ran) == want, (have_lib, have_ops, torch)
     _lib.build(force=True)
     assert len(ran) == want + 1
+
+
+# ---- the torch side: what it would drop ---------------------------------------------------------------------------------
+
+def each_op(x):
+    """Every operator on x, as calls."""
+    import torch
+    from rag_service_amd import ops
+    n, k = x.shape
+    w, s, q = torch.zeros(n, k, dtype=torch.int8), torch.ones(n), x.view(1, n, 1, k)
+    return [lambda: ops.quantize_rows(x), lambda: ops.linear_int8(x, w, s), lambda: ops.block_norm(x),
+            lambda: ops.cross_attention(q, q, q)]
+
+
+def test_wrappers_refuse_what_they_would_drop():
+    """A tangent, a recording, a bit that says the values are negated: none of them goes through these operators, so a tensor that
+    has one is refused as one that asks for a gradient is (here the first operand, before its device is looked at)."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+    from rag_service_amd import ops
+    x = torch.zeros(4, 8)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in each_op(dual):
+            with pytest.raises(ValueError, match="forward"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="forward"):
+                call()
+        with pytest.raises(ValueError, match="GPU only"):            # its primal part is a tensor like any other
+            ops.quantize_rows(fwd.unpack_dual(dual).primal)
+    for call in each_op(torch._neg_view(x)):
+        with pytest.raises(ValueError, match="negat"):
+            call()
+    for i in range(4):
+        with pytest.raises(ValueError, match="trace"):
+            torch.jit.trace(lambda t: each_op(t)[i](), x)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for i in range(4):
+        with pytest.raises(ValueError, match="trace"):
+            make_fx(lambda t: each_op(t)[i]())(x)
