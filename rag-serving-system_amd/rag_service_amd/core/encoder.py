@@ -15,6 +15,7 @@ has any), len + 1 queries against len keys, and the result is spread to (batch, 
 from __future__ import annotations
 
 import sys
+import warnings
 
 import numpy as np
 
@@ -133,6 +134,8 @@ class HipEncoder:
 
     # -- forward -----------------------------------------------------------------------------------
     def __call__(self, input_ids, attention_mask=None, token_type_ids=None):
+        """The tokenizer's tensors, (batch, length) each. Without attention_mask the tokens that are not pads are the mask; a
+        transformers model would take all of them, pads too, as keys, so a batch with pads then warns."""
         torch = _torch()
         if self._device is None:
             raise RuntimeError("HipEncoder: call .to(device) first")
@@ -151,6 +154,9 @@ class HipEncoder:
             mask = ids != self.pad if attention_mask is None else attention_mask.to(self._device) != 0
             types = None if token_type_ids is None else token_type_ids.to(self._device)
             lengths, lens = look(ids, mask, types, self.pad, self._words.shape[0], self._types.shape[0])
+            if attention_mask is None and min(lengths) < length:
+                warnings.warn("HipEncoder: no attention_mask, and there are pads: they are left out as keys (the model itself would "
+                              "attend to them)", stacklevel=2)
             offsets, source, place, spread = pack(lengths, length)
             move = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self._device)  # noqa: E731
             rows = move(np.stack([source, np.where(place < 0, self.pad, self.pad + 1 + place)]))

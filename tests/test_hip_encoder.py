@@ -257,3 +257,23 @@ def test_batch_processor_on_the_hip_encoder(encoder_class, handoff):
             assert q.results[r["id"]] == {"result": f"<answer to: {prompt}>"}
     assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items())
     retr.close()
+
+
+@pytest.mark.gpu
+def test_pads_without_a_mask_are_said_to_be_left_out(encoder_class):
+    """Without attention_mask the pad tokens are the mask. The model itself would attend to them, so the call warns; what it
+    returns is the model's result with that mask, and without pads there is nothing to say."""
+    import warnings
+    model = make_model()
+    enc = encoder_class(model).to("cuda")
+    ids, mask = batch_of([4, 7], 9)
+    with pytest.warns(UserWarning, match="attention_mask"):
+        got = enc(input_ids=ids.cuda()).last_hidden_state
+    with torch.no_grad():
+        masked = model(input_ids=ids, attention_mask=mask).last_hidden_state.double()
+    off = (got.double().cpu() - masked).norm(dim=-1) / masked.norm(dim=-1)
+    assert off.max() <= 0.15                               # (the bound of test_near_the_fp32_model)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        enc(input_ids=ids[:, :4].cuda())
+        enc(input_ids=ids.cuda(), attention_mask=mask.cuda())
