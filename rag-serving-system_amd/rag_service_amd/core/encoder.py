@@ -77,8 +77,8 @@ class HipEncoder:
     """An XLM-R model's forward pass in 8-bit products on the MI355X (inference only)."""
 
     def __init__(self, model, dtype: str = "bf16"):
-        """model: a transformers XLMRobertaModel (or RobertaModel), whose tensors are read, not changed; the embedding
-        tables are used where they are. dtype: what stands between the products, "bf16", "fp16" or "fp32"."""
+        """model: a transformers XLMRobertaModel (or RobertaModel), whose tensors are read, not changed, and
+        copied by ``to()``. dtype: what stands between the products, "bf16", "fp16" or "fp32"."""
         cfg = model.config
         if cfg.model_type not in MODEL_TYPES:
             raise ValueError(f"HipEncoder runs {' / '.join(MODEL_TYPES)} models, not {cfg.model_type}")
@@ -100,7 +100,8 @@ class HipEncoder:
 
     # -- weights -----------------------------------------------------------------------------------
     def to(self, device):
-        """Lays the weights out on `device` (8-bit weights, fp32 biases, norms in `dtype`); needs a GPU."""
+        """Lays the weights out on `device` (8-bit weights, fp32 biases, norms in `dtype`, the embedding tables as they are), all
+        of them copies: a model that changes needs a new HipEncoder. Needs a GPU."""
         torch = _torch()
         device = torch.device(device)
         if device.type != "cuda":
@@ -117,11 +118,12 @@ class HipEncoder:
             return (*ops.quantize_rows(w), b)
 
         def norm(p, dtype):
-            return p.weight.detach().to(device, dtype), p.bias.detach().to(device, dtype)
+            return p.weight.detach().to(device, dtype, copy=True), p.bias.detach().to(device, dtype, copy=True)
 
         with torch.no_grad():
             e = self._model.embeddings
-            tables = [x.weight.detach().to(device) for x in (e.word_embeddings, e.position_embeddings, e.token_type_embeddings)]
+            tables = [x.weight.detach().to(device, copy=True)
+                      for x in (e.word_embeddings, e.position_embeddings, e.token_type_embeddings)]
             embedding_norm = norm(e.LayerNorm, torch.float32)
             layers = [{"q": linear(x.attention.self.query), "kv": linear(x.attention.self.key, x.attention.self.value),
                        "o": linear(x.attention.output.dense), "norm1": norm(x.attention.output.LayerNorm, t),

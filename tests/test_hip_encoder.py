@@ -277,3 +277,18 @@ def test_pads_without_a_mask_are_said_to_be_left_out(encoder_class):
         warnings.simplefilter("error")
         enc(input_ids=ids[:, :4].cuda())
         enc(input_ids=ids.cuda(), attention_mask=mask.cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_to_copies_all_weights(encoder_class, dtype):
+    """A model on the same device that changes afterwards changes nothing of the encoder's: neither its 8-bit layers nor its
+    embedding tables, norms and biases."""
+    model = make_model().cuda()
+    enc = encoder_class(model, dtype).to("cuda")
+    ids, mask = (t.cuda() for t in batch_of([4, 9], 9))
+    before = enc(input_ids=ids, attention_mask=mask).last_hidden_state
+    with torch.no_grad():
+        for p in model.parameters():
+            p.mul_(-1.5).add_(0.25)
+    assert torch.equal(enc(input_ids=ids, attention_mask=mask).last_hidden_state, before)
