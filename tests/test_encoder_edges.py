@@ -159,3 +159,31 @@ def test_wrappers_refuse_what_they_would_drop():
     for i in range(4):
         with pytest.raises(ValueError, match="trace"):
             make_fx(lambda t: each_op(t)[i]())(x)
+
+
+def test_inline_asm_of_the_encoder_units_is_hazard_free():
+    """The audit of test_abi's test_inline_asm_loads_are_hazard_free (tools/check_asm_loads.py) on every kernel of the encoder's
+    units: their inline-asm loads go to LDS, and nothing of the vector unit is written in inline asm."""
+    import os
+    import re
+    import subprocess
+    import sys
+    pkg = _lib.PKG_ROOT
+    sys.path.insert(0, os.path.join(_lib.REPO_ROOT, "tools"))
+    from check_asm_loads import check
+    csrc = os.path.join(pkg, "csrc")
+    newest = max(os.path.getmtime(os.path.join(csrc, f)) for f in os.listdir(csrc) if f.startswith("rr_encoder"))
+    with_loads = {"linear": 0, "norm": 0, "attn": 0}
+    for unit in with_loads:
+        s_file = os.path.join(pkg, "build", f"rr_encoder_{unit}-hip-amdgcn-amd-amdhsa-gfx950.s")
+        if not os.path.exists(s_file) or os.path.getmtime(s_file) < newest:
+            subprocess.check_call(["make", "-C", pkg, "-j8"], stdout=subprocess.DEVNULL)
+        text = open(s_file).read()
+        syms = re.findall(r"^(_ZN2rr3enc\w+kernel\w+):", text, flags=re.M)
+        assert len(syms) >= 20, (unit, len(syms))
+        lines = text.split("\n")
+        for sym in syms:
+            n_asm, bad = check(lines, sym)
+            assert not bad, (sym, bad[:5])
+            with_loads[unit] += n_asm > 0
+    assert with_loads["norm"] == 0 and with_loads["linear"] >= 20 and with_loads["attn"] >= 10, with_loads
