@@ -411,7 +411,8 @@ int rr_block_norm(int device, void* hip_stream, int type, int64_t rows, int32_t 
  * Keys and values: k_offsets null: [batch][max_k][kv_heads][d] (strides k_bs.., v_bs..); else packed, as the queries.
  * key_lengths ([batch] int32, or null): a sequence has at most that many keys, its first ones. key_mask ([batch][max_k]
  * bytes, row stride mask_stride, or null; dense keys only): keys with a zero byte do not take part. Keys that do not take
- * part may hold anything, NaN too. A query without a key gets zeros. d: a multiple of 8 up to RR_ATTN_DMAX. */
+ * part may hold anything, NaN too. A query without a key gets zeros. d: a multiple of 8 up to RR_ATTN_DMAX. A sequence's keys, and
+ * values, lie less than 2^23 elements apart (k_ts, v_ts); batch and kv_heads are up to 65535, their product up to 2^22. */
 int rr_cross_attention(int device, void* stream, int type, const void* q, int64_t q_bs, int64_t q_ts, int64_t q_hs,
                        const void* k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_bs, int64_t v_ts,
                        int64_t v_hs, void* out, int64_t o_bs, int64_t o_ts, int64_t o_hs, int32_t batch, int32_t heads,

@@ -257,6 +257,7 @@ int rr_cross_attention(int device, void* stream, int type, const void* q, int64_
   if (q_offsets && total_q * (heads / kv_heads) > 1 << 30)
     return fail(RR_E_UNSUPPORTED, "%s: %lld queries of %d heads a key head above 2^30 rows", me, (long long)total_q,
                 heads / kv_heads);
+  if ((k_offsets ? total_k : max_k) <= 1) k_ts = v_ts = d;   // (no step from key to key: its size may be anything)
   if (k_ts > kTsMost || v_ts > kTsMost)
     return fail(RR_E_UNSUPPORTED, "%s: keys %lld and values %lld elements apart, above %lld", me, (long long)k_ts,
                 (long long)v_ts, (long long)kTsMost);

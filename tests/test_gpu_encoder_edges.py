@@ -194,3 +194,34 @@ def test_linear_int8_of_two_billion_rows(ops):
         assert torch.equal(got[lo:lo + (1 << 27)], want)
     del x, sx, got, want
     torch.cuda.empty_cache()
+
+
+# ---- attention: strides that are never taken ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lq", [1, 40])
+def test_attention_of_one_key_in_front_of_a_large_batch(ops, dtype, lq):
+    """States of one token, the token in front of the batch: the step from key to key is a whole batch's, which no one takes. Of
+    two keys it is a step too far, and refused. A result is its one value times a weight, times the weight's reciprocal: a
+    rounding of 32 bits each, 3 U and their products, within 4 U."""
+    from rag_service_amd import HipRetrievalError
+    g = gen(lq)
+    b, h, d = 1100, 64, 128                                # 9.0 million elements from key to key, above 2^23
+    q = rand(g, b, lq, 1, d).to(dtype).cuda().expand(b, lq, h, d)
+    kv = rand(g, 2, 1, b, h, d).to(dtype).cuda()
+    k, v = kv[0].transpose(0, 1), kv[1].transpose(0, 1)
+
+    def near(got, want):
+        got, want = got[::37], want[::37]                  # (every 37th sequence, even and odd ones)
+        plain.within(got, want, 4 * plain.U * want.double().cpu().abs(), dtype)
+
+    near(ops.cross_attention(q, k, v), v.expand(b, lq, h, d))
+    lens = (torch.arange(b, dtype=torch.int32) % 2).cuda()
+    near(ops.cross_attention(q, k, v, key_lengths=lens), v.expand(b, lq, h, d) * lens[:, None, None, None])
+    offsets = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    one = k[:1].squeeze(0)                                 # (1, heads, d), packed
+    assert one.stride(0) > 1 << 23
+    near(ops.cross_attention(q[:1], one, v[:1].squeeze(0), k_offsets=offsets, max_k=1), v[:1].expand(1, lq, h, d))
+    two = kv.transpose(1, 2).reshape(2, b, h, d).transpose(0, 1)
+    with pytest.raises(HipRetrievalError, match="apart"):
+        ops.cross_attention(q, two, two)
