@@ -369,7 +369,9 @@ int rr_stream_queues(rr_handle* h, int i, uint64_t* out);
 
 /* 8-bit rows: scale[r] = max|x[r]| * fl(1 / 127), q[r][c] = clamp(rint(x[r][c] / scale[r]), -127, 127), product and quotient
  * rounded to fp32, rint to even (the index's int8 copies divide by 127: their scales may differ in the last bit). A row of
- * zeros has scale 0; a row that holds a NaN or an infinity has scale NaN and q = 0, so every product with it is NaN. x: [rows][cols] of `type` (F32, BF16, F16), row stride ldx; q: row stride ldq. */
+ * zeros, or of values so small that the scale is 0 in fp32, has scale 0 and q = 0; a row that holds a NaN or an infinity has scale
+ * NaN and q = 0, so every product with it is NaN. x: [rows][cols] of `type` (F32, BF16, F16), row stride ldx; q: row stride ldq.
+ * cols up to 2^31 - 1, rows too. */
 int rr_quantize_rows(int device, void* stream, int type, const void* x, int64_t ldx, int64_t rows, int32_t cols,
                      int8_t* q, int64_t ldq, float* scale);
 

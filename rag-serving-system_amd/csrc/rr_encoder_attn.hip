@@ -495,12 +495,14 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void attn_rows_kernel(Attn
 // of the second product's 16-key contraction t. V lies in LDS as in memory; the transposing LDS read hands each lane four keys
 // of one dimension. The weights enter the second product rounded to the type: off by at most half a step of each, which is half
 // a step of sum p |v| in the result, while their sum and the statistics are of the unrounded ones in fp32. Few rows, which
-// wait for memory and not for arithmetic, add what the rounding left in a product of its own (small fp16 rests in steps of 2^-24).
+// wait for memory and not for arithmetic, add what the rounding left in a product of its own (small fp16 rests in steps of 2^-24);
+// for many rows it costs more than the precision is worth: 32 x 512 x 512 by mask 46 -> 62 us.
 // DMA: rows at 16-byte addresses go to LDS by the loads themselves; others through registers.
-// WK = 4 is bound by bandwidth: one query x 65536 keys x 4, 32 heads over 8 of 128, bf16: 199 us, 5.4 TB/s; x 512 keys x 32, 16
-// heads of 64: 14 us, 4.8 TB/s. WK = 1 is bound by the softmax's instructions (a 32-key block's 16 exponentials, multiply-adds and
-// sums a lane take longer than its eight matrix instructions): 32 x 512 x 512, 16 heads of 64: 51 us, 670 TFLOP/s, of which 19
-// are there with 64 keys too (queries in, results out, latencies); 8 x 2048 x 2048, heads of 128: 300 us, 915 TFLOP/s.
+// WK = 4 is bound by bandwidth: one query x 65536 keys x 4, 32 heads over 8 of 128, bf16: 199 us, 5.4 TB/s; x 40 to 512 keys x 32,
+// 16 heads of 64: 12.4 us (a launch and four steps' latency). WK = 1 is bound by the softmax's instructions (a 32-key block's 16 exponentials, multiply-adds and
+// sums a lane take longer than its eight matrix instructions): 32 x 512 x 512, 16 heads of 64, bf16: 53 us, 650 TFLOP/s, of
+// which 19 are there with 64 keys too (queries in, results out, latencies); 8 x 2048 x 2048, 16 heads of 128: 300 us, 915
+// TFLOP/s. fp16, whose reference moves more often: 56 and 322 us.
 // Four workgroups a CU at 128 registers a wave (32 keys at a time) beat two with 64 at a time (54 against 68 us).
 constexpr int kTileRows = 128, kFewRows = 32;
 

@@ -152,9 +152,10 @@ __device__ __forceinline__ void store_chunk(E* p, const float* v, int left, bool
   }
 }
 
-// The 8-bit row rule: scale = max|x| times the fp32 neighbour of 1/127 (one multiplication: a row's scale is then the same
-// wherever it is made, also by code that divides by 127 through its reciprocal). The row's largest magnitude travels as its bit pattern: patterns of |x| order as their values do,
-// infinities above every finite value and NaNs above those.
+// The 8-bit row rule: scale = max|x| times the fp32 neighbour of 1/127. (One multiplication, as torch divides a GPU tensor by 127. An
+// IEEE quotient, which the index's int8 copies take, is another number in the last bit in one row of twenty.) The row's largest
+// magnitude travels as its bit pattern: patterns of |x| order as their values do, infinities above every finite value and NaNs above
+// those.
 __device__ __forceinline__ unsigned mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ float row_scale(unsigned m) {
   return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(m) * (1.0f / 127.0f);

@@ -158,7 +158,8 @@ template <int OT>
 __device__ __forceinline__ float gelu(float y) {
   if constexpr (OT == T_F32) return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
   // 16-bit results: erf to 1.5e-7 by Abramowitz and Stegun 7.1.26, a third of erff's instructions
-  // (613 x 4096 results of a 1024-long product: 18.2 us with erff, 9.9 with this)
+  // (613 x 4096 results of a 1024-long product: 18.2 us with erff, 10.2 with this); relative to 1 - erf it is off by
+  // 5e-5 at y = -3 and 4e-3 at -6, where 1 + erf in fp32 has lost all of it
   const float z = fabsf(y) * 0.70710678118654752f;
   const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
   const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
@@ -661,8 +662,10 @@ hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
   return a.out_type == T_F32 ? linear<T_F32, 0>(a, s) : a.out_type == T_BF16 ? linear<T_BF16, 0>(a, s) : linear<T_F16, 0>(a, s);
 }
 
-// Rows that start between dwords: the tiled product of copies, where it saves more than they cost (int8 rows, GPU time, any
-// sizes / copies and tiles):
+// Inner sizes that are no multiple of 4, whose contiguous rows start between dwords: the tiled product of copies, where it saves
+// more than they cost (int8 rows, GPU time, any sizes / copies and tiles). The choice is made by k, since the workspace's
+// size depends on it and k is all that the function that tells it sees: rows of such a k that lie on dwords are copied too, and
+// rows of another k that do not go to the kernel of any alignment.
 //   613 x 4001 -> 1024   20.4 / 21.1 us     613 x 1307 -> 3637   25.1 / 21.1
 //   16000 x 4001 -> 1024  249 / 93          2000 x 1307 -> 3637  57.8 / 27.6
 // Floating-point rows are made with the padding, and the launch that makes them copies the weights beside them.
